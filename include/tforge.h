@@ -65,8 +65,20 @@ enum tforge_workload {
   TFORGE_ADD = 5
 };
 
-/* Element types accepted for A and B by tforge_gemm. */
-enum tforge_dtype { TFORGE_F32 = 0, TFORGE_BF16 = 1 };
+/* Element types.  tforge_gemm takes f32 and bf16; E4M3 (8 bits: sign, 4 exponent and 3 mantissa
+ * bits, largest 448) is an operand type of tforge_linear and an output type of tforge_rms_norm
+ * and tforge_quantize_e4m3. */
+enum tforge_dtype { TFORGE_F32 = 0, TFORGE_BF16 = 1, TFORGE_E4M3 = 2 };
+
+/* Activations of tforge_linear.  GELU is z Phi(z) with the normal distribution's Phi; GELU_TANH its
+ * tanh form, z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2; SILU z / (1 + exp(-z)). */
+enum tforge_activation {
+  TFORGE_ACT_NONE = 0,
+  TFORGE_ACT_RELU = 1,
+  TFORGE_ACT_GELU = 2,
+  TFORGE_ACT_GELU_TANH = 3,
+  TFORGE_ACT_SILU = 4
+};
 
 /* Fused GEMM.  out = epilogue(A @ B).  Replaces the generated `entry_kernel` of the
  * tforge-gpu-pipeline (lib/Transforms/Gpu.cpp:219-316) launched at
@@ -124,6 +136,119 @@ int tforge_add(const float *X, const float *Y, float *Z, int64_t M, int64_t N, v
 /* Round f32 to bf16 (round to nearest even), n elements: converts a weight once for
  * repeated TFORGE_MODE_BF16 calls with b_dtype = TFORGE_BF16. */
 int tforge_convert_bf16(const float *x, uint16_t *y, int64_t n, void *stream);
+
+/* ---- transformer-layer operators --------------------------------------------------------------
+ * All asynchronous on `stream`, which belongs to the current device, as all pointers do.  Pitches
+ * are in elements, 0 = packed.  Any size, pitch and element-aligned pointer works; rows that start
+ * on 16-byte boundaries save an operand's copy (tforge_linear) or take wider accesses.  M = 0 or
+ * N = 0 is a no-op but for the gradients' sums over no rows, which are zeros.  Scratch comes from
+ * the library's stream-ordered pool. */
+
+/* The linear layer with its epilogue:
+ *   z = (A @ B) * a_scale[m] * b_scale[n] + bias[n];  out = act(z) + residual;  pre = z
+ * A is M x K; B is K x N, or N x K with trans_b = 1 (a row per output feature).  Operands: bf16 or
+ * f32 (rounded to bf16, as TFORGE_MODE_BF16 does), or both E4M3 with f32 scales a row of A and a
+ * column of B, as tforge_rms_norm and tforge_quantize_e4m3 write them (then trans_b = 1).  Products
+ * are accumulated and the epilogue computed in f32, and each output is rounded once.  bias, residual
+ * and pre may be NULL; pre has out's type.  out may be the residual itself (same pointer, pitch and
+ * type): a residual stream updated in place.  K = 0 gives z = bias. */
+typedef struct tforge_linear_args {
+  int32_t activation;      /* enum tforge_activation */
+  int32_t trans_b;         /* 0: B is K x N; 1: N x K */
+  int32_t a_dtype;         /* enum tforge_dtype */
+  int32_t b_dtype;
+  int32_t out_dtype;       /* TFORGE_F32 or TFORGE_BF16: out and pre */
+  int32_t residual_dtype;  /* TFORGE_F32 or TFORGE_BF16 */
+  const void *A;
+  const void *B;
+  const float *a_scale;    /* M (E4M3) */
+  const float *b_scale;    /* N (E4M3) */
+  const float *bias;       /* N or NULL */
+  const void *residual;    /* M x N or NULL */
+  void *out;               /* M x N */
+  void *pre;               /* M x N or NULL */
+  int64_t M, N, K;
+  int64_t lda, ldb, ldr, ldo, ldp;
+} tforge_linear_args;
+
+int tforge_linear(const tforge_linear_args *args, void *stream);
+
+/* The linear layer's gradient.  With dz = dout * act'(pre):
+ *   dA = dz @ B^T (M x K);  dB = A^T @ dz (laid out as B);  dbias[n] = sum over m of dz[m, n]
+ * The residual's gradient is dout itself.  dA, dB and dbias may each be NULL (not wanted).  A and B
+ * are bf16 or f32 (rounded to bf16); dz is rounded to bf16 for the two products, dbias sums it
+ * unrounded, in f32 and in a fixed order.  pre is needed but for TFORGE_ACT_NONE. */
+typedef struct tforge_linear_backward_args {
+  int32_t activation;
+  int32_t trans_b;
+  int32_t a_dtype;         /* TFORGE_F32 or TFORGE_BF16 */
+  int32_t b_dtype;
+  int32_t dtype;           /* TFORGE_F32 or TFORGE_BF16: dout and pre */
+  int32_t grad_dtype;      /* TFORGE_F32 or TFORGE_BF16: dA and dB */
+  const void *dout;        /* M x N */
+  const void *pre;         /* M x N */
+  const void *A;           /* M x K */
+  const void *B;
+  void *dA;
+  void *dB;
+  float *dbias;            /* N */
+  int64_t M, N, K;
+  int64_t lddo, ldp, lda, ldb, ldda, lddb;
+} tforge_linear_backward_args;
+
+int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream);
+
+/* Root-mean-square norm of rows, with the residual's addition before it:
+ *   s = x + residual (sum_out = s);  r = (mean(s^2) + eps)^-1/2 (rstd = r);  out = s r weight
+ * in f32, each output rounded once.  out is f32, bf16 or E4M3; E4M3 rows come with scale[m] =
+ * max(max|out| / 448, 2^-126), the f32 factor back to out's values; a row that holds a NaN, or an
+ * infinity in s, has a NaN scale and NaN values.  residual, weight (1), sum_out, rstd may be NULL.
+ * sum_out may be x or the residual itself (same pointer and pitch). */
+typedef struct tforge_rms_norm_args {
+  int32_t dtype;           /* TFORGE_F32 or TFORGE_BF16: x, residual, sum_out */
+  int32_t weight_dtype;    /* TFORGE_F32 or TFORGE_BF16 */
+  int32_t out_dtype;
+  float eps;               /* >= 0 */
+  const void *x;           /* M x N */
+  const void *residual;    /* M x N or NULL */
+  const void *weight;      /* N or NULL */
+  void *sum_out;           /* M x N or NULL */
+  void *out;               /* M x N */
+  float *scale;            /* M (E4M3) */
+  float *rstd;             /* M or NULL */
+  int64_t M, N;
+  int64_t ldx, ldr, lds, ldo;
+} tforge_rms_norm_args;
+
+int tforge_rms_norm(const tforge_rms_norm_args *args, void *stream);
+
+/* The norm's gradient, from s and rstd as the forward call gave them and out's gradient dy.  With
+ * h = s rstd and g = dy weight:
+ *   dx = rstd (g - h mean(g h)) + ds;  dweight[n] = sum over m of dy[m, n] h[m, n]
+ * dx is the gradient of x and of the residual alike; ds (may be NULL) is what reaches s on the
+ * residual stream, and dx may be ds itself (same pointer and pitch).  dweight may be NULL; it is
+ * summed in f32 and in a fixed order. */
+typedef struct tforge_rms_norm_backward_args {
+  int32_t dtype;           /* TFORGE_F32 or TFORGE_BF16: dy, s, ds, dx */
+  int32_t weight_dtype;    /* TFORGE_F32 or TFORGE_BF16 */
+  const void *dy;          /* M x N */
+  const void *s;           /* M x N */
+  const void *weight;      /* N or NULL */
+  const float *rstd;       /* M */
+  const void *ds;          /* M x N or NULL */
+  void *dx;                /* M x N */
+  float *dweight;          /* N or NULL */
+  int64_t M, N;
+  int64_t lddy, lds, ldds, lddx;
+} tforge_rms_norm_backward_args;
+
+int tforge_rms_norm_backward(const tforge_rms_norm_backward_args *args, void *stream);
+
+/* Rows of f32 or bf16 x (M x N, pitch ldx) in 8 bits: scale[m] = max(max|x[m]| / 448, 2^-126),
+ * q = e4m3(x / scale[m]) (pitch ldq).  Weights (N x K) are quantized once, activations before a
+ * product that tforge_rms_norm does not feed.  NaN and infinities as in tforge_rms_norm. */
+int tforge_quantize_e4m3(const void *x, int dtype, uint8_t *q, float *scale, int64_t M, int64_t N, int64_t ldx,
+                         int64_t ldq, void *stream);
 
 /* relu(A @ B + bias) in TFORGE_MODE_BF16 without allocating anything.  No counterpart in
  * the reference.  For callers that must not allocate device memory during a call (a
@@ -191,6 +316,12 @@ int tforge_set_wait_limit_ns(uint64_t ns);
 /* Test hook: 1 makes the next GEMM launches' producer skip its first stage's load, so
  * the consumer's bounded wait expires and reports TFORGE_ERR_TIMEOUT; 0 clears. */
 int tforge_debug_skip_load(int on);
+
+/* Test hook: the kernel that tforge_linear's and tforge_linear_backward's products take.  kernel 0:
+ * chosen by size; 1: one CTA per 128 columns x `tile` rows (16, 32, 64, 128 or 256), `splits` CTAs
+ * (1, 2, 4 or 8) sharing a tile's K.  A forced kernel that cannot take a product gives
+ * TFORGE_ERR_UNSUPPORTED. */
+int tforge_debug_linear_kernel(int kernel, int tile, int splits);
 
 /* Test hook: bytes of the library's scratch pool in use now and the high-water mark since
  * the last reset (reset_high = 1 resets it after reading).  Creates the pool if the

@@ -19,7 +19,10 @@ OK, ERR_SHAPE, ERR_ALIGN, ERR_ALIAS, ERR_MODE, ERR_CUDA, ERR_TIMEOUT, ERR_NULL, 
 MODES = {"fp32": 0, "tf32": 1, "bf16": 2, "fp32_exact": 3}
 # enum tforge_workload
 WORKLOADS = {"matmul": 0, "mbr": 1, "matmul_add": 2, "bias_add": 3, "relu": 4, "add": 5}
-F32, BF16 = 0, 1
+# enum tforge_dtype
+F32, BF16, E4M3 = 0, 1, 2
+# enum tforge_activation
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
 class GemmArgs(C.Structure):
@@ -28,6 +31,30 @@ class GemmArgs(C.Structure):
                 ("C_res", C.c_void_p), ("out", C.c_void_p), ("M", C.c_int64), ("N", C.c_int64),
                 ("K", C.c_int64), ("lda", C.c_int64), ("ldb", C.c_int64), ("ldc", C.c_int64),
                 ("out_dtype", C.c_int32)]
+
+
+class LinearArgs(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("activation", "trans_b", "a_dtype", "b_dtype", "out_dtype", "residual_dtype")]
+                + [(n, C.c_void_p) for n in ("A", "B", "a_scale", "b_scale", "bias", "residual", "out", "pre")]
+                + [(n, C.c_int64) for n in ("M", "N", "K", "lda", "ldb", "ldr", "ldo", "ldp")])
+
+
+class LinearBackwardArgs(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("activation", "trans_b", "a_dtype", "b_dtype", "dtype", "grad_dtype")]
+                + [(n, C.c_void_p) for n in ("dout", "pre", "A", "B", "dA", "dB", "dbias")]
+                + [(n, C.c_int64) for n in ("M", "N", "K", "lddo", "ldp", "lda", "ldb", "ldda", "lddb")])
+
+
+class RmsNormArgs(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "weight_dtype", "out_dtype")] + [("eps", C.c_float)]
+                + [(n, C.c_void_p) for n in ("x", "residual", "weight", "sum_out", "out", "scale", "rstd")]
+                + [(n, C.c_int64) for n in ("M", "N", "ldx", "ldr", "lds", "ldo")])
+
+
+class RmsNormBackwardArgs(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "weight_dtype")]
+                + [(n, C.c_void_p) for n in ("dy", "s", "weight", "rstd", "ds", "dx", "dweight")]
+                + [(n, C.c_int64) for n in ("M", "N", "lddy", "lds", "ldds", "lddx")])
 
 
 class Launch(C.Structure):
@@ -62,6 +89,12 @@ SIGNATURES = {
     "tforge_relu": (_I, [_P, _P, _I64, _I64, _P]),
     "tforge_add": (_I, [_P, _P, _P, _I64, _I64, _P]),
     "tforge_convert_bf16": (_I, [_P, _P, _I64, _P]),
+    "tforge_linear": (_I, [C.POINTER(LinearArgs), _P]),
+    "tforge_linear_backward": (_I, [C.POINTER(LinearBackwardArgs), _P]),
+    "tforge_rms_norm": (_I, [C.POINTER(RmsNormArgs), _P]),
+    "tforge_rms_norm_backward": (_I, [C.POINTER(RmsNormBackwardArgs), _P]),
+    "tforge_quantize_e4m3": (_I, [_P, _I, _P, _P, _I64, _I64, _I64, _I64, _P]),
+    "tforge_debug_linear_kernel": (_I, [_I, _I, _I]),
     "tforge_mbr_bf16_noalloc": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _P]),
     "tforge_describe": (_I, [_I, _I64, _I64, _I64, _I, C.POINTER(Launch)]),
     "tforge_set_config": (_I, [C.POINTER(Config)]),
@@ -155,6 +188,60 @@ def gemm_host(workload: str, A: int, B: int, out: int, M: int, N: int, K: int, m
                     M, N, K, lda, ldb, ldc)
     check(lib().tforge_gemm_host(C.byref(args), chunk_rows, stream),
           f"tforge_gemm_host({workload}, {M}x{N}x{K}, {mode})")
+
+
+def linear(A: int, B: int, out: int, M: int, N: int, K: int, activation: str = "none", bias: int | None = None,
+           residual: int | None = None, pre: int | None = None, a_scale: int | None = None, b_scale: int | None = None,
+           a_dtype: int = BF16, b_dtype: int = BF16, out_dtype: int = BF16, residual_dtype: int = BF16,
+           trans_b: bool = False, lda: int = 0, ldb: int = 0, ldr: int = 0, ldo: int = 0, ldp: int = 0,
+           stream: int | None = None) -> None:
+    """tforge_linear on device pointers (ints), asynchronous on `stream`: out = act(A @ B + bias) + residual."""
+    args = LinearArgs(ACTIVATIONS[activation], trans_b, a_dtype, b_dtype, out_dtype, residual_dtype, A, B, a_scale,
+                      b_scale, bias, residual, out, pre, M, N, K, lda, ldb, ldr, ldo, ldp)
+    rc = lib().tforge_linear(C.byref(args), stream)
+    if rc != OK:
+        raise TforgeError(rc, f"tforge_linear({M}x{N}x{K}, {activation})")
+
+
+def linear_backward(dout: int, A: int | None, B: int | None, M: int, N: int, K: int, activation: str = "none",
+                    pre: int | None = None, dA: int | None = None, dB: int | None = None, dbias: int | None = None,
+                    a_dtype: int = BF16, b_dtype: int = BF16, dtype: int = BF16, grad_dtype: int = BF16,
+                    trans_b: bool = False, lddo: int = 0, ldp: int = 0, lda: int = 0, ldb: int = 0, ldda: int = 0,
+                    lddb: int = 0, stream: int | None = None) -> None:
+    """tforge_linear_backward on device pointers (ints): the gradients that are not None."""
+    args = LinearBackwardArgs(ACTIVATIONS[activation], trans_b, a_dtype, b_dtype, dtype, grad_dtype, dout, pre, A, B, dA,
+                              dB, dbias, M, N, K, lddo, ldp, lda, ldb, ldda, lddb)
+    rc = lib().tforge_linear_backward(C.byref(args), stream)
+    if rc != OK:
+        raise TforgeError(rc, f"tforge_linear_backward({M}x{N}x{K}, {activation})")
+
+
+def rms_norm(x: int, out: int, M: int, N: int, eps: float, weight: int | None = None, residual: int | None = None,
+             sum_out: int | None = None, rstd: int | None = None, scale: int | None = None, dtype: int = BF16,
+             weight_dtype: int = F32, out_dtype: int = BF16, ldx: int = 0, ldr: int = 0, lds: int = 0, ldo: int = 0,
+             stream: int | None = None) -> None:
+    """tforge_rms_norm on device pointers (ints): out = (x + residual) * rstd * weight."""
+    args = RmsNormArgs(dtype, weight_dtype, out_dtype, eps, x, residual, weight, sum_out, out, scale, rstd, M, N, ldx,
+                       ldr, lds, ldo)
+    rc = lib().tforge_rms_norm(C.byref(args), stream)
+    if rc != OK:
+        raise TforgeError(rc, f"tforge_rms_norm({M}x{N})")
+
+
+def rms_norm_backward(dy: int, s: int, rstd: int, dx: int, M: int, N: int, weight: int | None = None,
+                      ds: int | None = None, dweight: int | None = None, dtype: int = BF16, weight_dtype: int = F32,
+                      lddy: int = 0, lds: int = 0, ldds: int = 0, lddx: int = 0, stream: int | None = None) -> None:
+    """tforge_rms_norm_backward on device pointers (ints)."""
+    args = RmsNormBackwardArgs(dtype, weight_dtype, dy, s, weight, rstd, ds, dx, dweight, M, N, lddy, lds, ldds, lddx)
+    rc = lib().tforge_rms_norm_backward(C.byref(args), stream)
+    if rc != OK:
+        raise TforgeError(rc, f"tforge_rms_norm_backward({M}x{N})")
+
+
+def quantize_e4m3(x: int, q: int, scale: int, M: int, N: int, dtype: int = BF16, ldx: int = 0, ldq: int = 0,
+                  stream: int | None = None) -> None:
+    """tforge_quantize_e4m3 on device pointers (ints): rows in 8 bits with a scale each."""
+    check(lib().tforge_quantize_e4m3(x, dtype, q, scale, M, N, ldx, ldq, stream), f"tforge_quantize_e4m3({M}x{N})")
 
 
 def device_status(stream: int | None = None) -> int:

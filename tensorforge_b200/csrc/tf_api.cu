@@ -574,7 +574,31 @@ int check_gemm_args(const tforge_gemm_args *a, int64_t *lda, int64_t *ldb, int64
   return check_gemm(a, lda, ldb, ldc);
 }
 
+// Row-major rows x cols of `esz`-byte elements (2: bf16, 1: 8-bit), pitch ld, boxes of box_cols x
+// box_rows in the 128-byte swizzle; what lies outside reads as zero.
+int encode_rows_map(CUtensorMap *m, const void *base, int esz, int64_t rows, int64_t cols, int64_t ld,
+                    uint32_t box_cols, uint32_t box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) {
+    g_last_error = "cuTensorMapEncodeTiled unavailable";
+    return TFORGE_ERR_CUDA;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * esz)};
+  cuuint32_t box[2] = {box_cols, box_rows}, estr[2] = {1, 1};
+  CUresult r = enc(m, esz == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
+                   const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    g_last_error = "cuTensorMapEncodeTiled failed for a linear operand (" + std::to_string((int)r) + ")";
+    return TFORGE_ERR_CUDA;
+  }
+  return TFORGE_OK;
+}
+
 int device_pool(cudaMemPool_t *out) { return scratch_pool(out); }
+int device_status_word(uint32_t **out) { return status_word(out); }
+int cuda_failure(cudaError_t e, const char *what) { return cuda_fail(e, what); }
 
 uint64_t wait_limit_ns() { return g_wait_limit_ns.load(); }
 int debug_skip_load() { return g_debug_skip.load(); }

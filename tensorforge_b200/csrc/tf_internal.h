@@ -166,4 +166,61 @@ cudaError_t launch_splitk_reduce(int epi, const float *ws, int splits, int64_t s
                                  const float *bias, const float *cres, float *out, int64_t ldc,
                                  cudaStream_t stream);
 
+// ---- transformer-layer operators (tf_layer.cu checks arguments and calls these) --------------------
+
+// The current device's status word for bounded waits, created on first use (tf_api.cu).
+int device_status_word(uint32_t **out);
+// The error text and TFORGE_ERR_CUDA of a failed CUDA call (tf_api.cu).
+int cuda_failure(cudaError_t e, const char *what);
+
+// Tensor map of bf16 (esz 2) or 8-bit (esz 1) rows, boxes in the 128-byte swizzle (tf_api.cu).
+int encode_rows_map(CUtensorMap *m, const void *base, int esz, int64_t rows, int64_t cols, int64_t ld,
+                    uint32_t box_cols, uint32_t box_rows);
+
+// One product of the linear layer and its epilogue (tf_epilogue.cuh).  Null pointers: absent.
+struct LinearParams {
+  const float *bias;              // N
+  const float *a_scale, *b_scale;  // M, N (8-bit operands)
+  const void *residual;           // M x N, pitch ldr
+  void *out, *pre;                // M x N, pitches ldo, ldp, bf16 if out_bf16 else f32
+  int32_t M, N, K;
+  int64_t ldr, ldo, ldp;
+  int32_t act;                    // enum tforge_activation
+  int32_t res_bf16, out_bf16;
+  uint32_t *status;               // device status word
+  uint64_t limit_ns;              // bounded-wait limit
+  int32_t debug_skip;             // test hook: skip the first stage's loads
+  int32_t splits;                 // slim kernel: CTAs that share a tile's k (1, 2, 4 or 8)
+};
+// One-CTA kernel of 128 columns x bt tokens (16, 32, 64, 128, 256; from 64 with t_mn).  tmT: A as
+// {128 B of k x bt rows} boxes, or with t_mn (A stored k x m) {64 columns x 64 rows}; tmW: B stored
+// n x k as {128 B x 128 rows} boxes, or with w_mn (stored k x n) {64 columns x 64 rows}.
+cudaError_t launch_linear_slim(bool f8, bool w_mn, bool t_mn, int bt, const CUtensorMap &tmT, const CUtensorMap &tmW,
+                               const LinearParams &p, cudaStream_t stream);
+
+// tforge_rms_norm / tforge_quantize_e4m3 with every pitch filled in (tf_norm.cu).
+struct NormArgs {
+  const void *x, *residual, *weight;
+  void *sum_out, *out;
+  float *scale, *rstd;
+  int64_t M, N, ldx, ldr, lds, ldo;
+  float eps;
+  int32_t x_bf16, w_bf16;
+  int32_t out_kind;  // 0 f32, 1 bf16, 2 e4m3
+};
+struct NormBwdArgs {
+  const void *dy, *s, *weight, *ds;
+  const float *rstd;
+  void *dx;
+  int64_t M, N, lddy, lds, ldds, lddx;
+  int32_t x_bf16, w_bf16;
+};
+// norm false: the row quantizer (out_kind 2).
+cudaError_t launch_rms_norm(const NormArgs &p, bool norm, cudaStream_t stream);
+// Blocks of the gradient kernel, and so rows of its scratch `part` (rows x N f32; null: no dweight).
+int rms_norm_bwd_parts(int64_t M, int64_t N);
+cudaError_t launch_rms_norm_bwd(const NormBwdArgs &p, float *part, int grid, cudaStream_t stream);
+// out[n] = sum over r < rows, in a fixed order, of part[r * N + n].
+cudaError_t launch_column_sum(const float *part, int rows, int64_t N, float *out, cudaStream_t stream);
+
 }  // namespace tf

@@ -1,0 +1,558 @@
+// tf_layer.cu -- C-ABI of the transformer-layer operators (include/tforge.h): argument checks,
+// operand copies where TMA cannot read the caller's rows, the choice of the product's kernel, and
+// the gradient's elementwise pass.  The kernels are in tf_linear_slim.cu and tf_norm.cu.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cmath>
+
+#include "tf_epilogue.cuh"
+#include "tf_internal.h"
+
+using namespace tf;
+
+namespace {
+
+// tforge_debug_linear_kernel: kernel | tile << 8 | splits << 24.
+std::atomic<uint32_t> g_force{0};
+
+bool at(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+int elem_size(int dtype) { return dtype == TFORGE_F32 ? 4 : (dtype == TFORGE_BF16 ? 2 : 1); }
+bool is_float(int dtype) { return dtype == TFORGE_F32 || dtype == TFORGE_BF16; }
+
+// A row-pitched array of the call, for the checks that every entry makes.
+struct Array {
+  const void *p;
+  int64_t rows, cols, ld;
+  int esz;
+  uint64_t bytes() const { return rows > 0 && cols > 0 ? ((uint64_t)(rows - 1) * ld + cols) * esz : 0; }
+};
+
+bool overlap(const Array &a, const Array &b) {
+  if (!a.p || !b.p || !a.bytes() || !b.bytes()) return false;
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.p), b0 = reinterpret_cast<uintptr_t>(b.p);
+  return a0 < b0 + b.bytes() && b0 < a0 + a.bytes();
+}
+bool same(const Array &a, const Array &b) { return a.p == b.p && a.ld == b.ld && a.esz == b.esz; }
+
+// Every array element-aligned; no output overlapping another output or an input, but that
+// outs[share] may be the same array as ins[with0] or ins[with1].
+template <int NI, int NO>
+int check_arrays(const Array (&ins)[NI], const Array (&outs)[NO], int share = -1, int with0 = -1, int with1 = -1) {
+  for (const Array &a : ins)
+    if (!at(a.p, a.esz)) return TFORGE_ERR_ALIGN;
+  for (const Array &a : outs)
+    if (!at(a.p, a.esz)) return TFORGE_ERR_ALIGN;
+  for (int o = 0; o < NO; ++o) {
+    for (int i = 0; i < NI; ++i)
+      if (overlap(outs[o], ins[i]) && !(o == share && (i == with0 || i == with1) && same(outs[o], ins[i])))
+        return TFORGE_ERR_ALIAS;
+    for (int q = 0; q < o; ++q)
+      if (overlap(outs[o], outs[q])) return TFORGE_ERR_ALIAS;
+  }
+  return TFORGE_OK;
+}
+
+bool dims_ok(int64_t a, int64_t b, int64_t c = 0) {
+  return a >= 0 && b >= 0 && c >= 0 && a <= INT32_MAX && b <= INT32_MAX && c <= INT32_MAX;
+}
+// Fills a zero pitch in; false when a pitch is shorter than its row (or unreasonably long: byte
+// offsets stay within 63 bits).
+bool pitch(int64_t &ld, int64_t cols) {
+  if (ld == 0) ld = cols;
+  return ld >= cols && ld <= (int64_t)1 << 31;
+}
+
+// Stream-ordered scratch of one call, released (in stream order) when the call returns.
+class Scratch {
+ public:
+  explicit Scratch(cudaStream_t st) : st_(st) {}
+  Scratch(const Scratch &) = delete;
+  ~Scratch() {
+    for (int i = 0; i < n_; ++i) cudaFreeAsync(p_[i], st_);
+  }
+  int get(void **out, uint64_t bytes) {
+    cudaMemPool_t pool = nullptr;
+    int rc = device_pool(&pool);
+    if (rc) return rc;
+    cudaError_t e = cudaMallocFromPoolAsync(out, bytes, pool, st_);
+    if (e != cudaSuccess) return cuda_failure(e, "cudaMallocFromPoolAsync(layer scratch)");
+    p_[n_++] = *out;
+    return TFORGE_OK;
+  }
+
+ private:
+  cudaStream_t st_;
+  void *p_[8];
+  int n_ = 0;
+};
+
+// ---- operand copies -------------------------------------------------------------------------------
+
+template <typename S, typename D>
+__device__ __forceinline__ D convert(S v) {
+  if constexpr (std::is_same<S, float>::value) return __float2bfloat16_rn(v);
+  else return v;
+}
+
+// dst[r * ldd + c] = src[r * lds + c], f32 rounded to bf16; rows of any alignment into rows on
+// 16-byte boundaries.  Eight elements a thread: single loads, one 16-byte (or 8-byte) store; what
+// lies beyond a row's end within the last group is written as 0.
+template <typename S, typename D>
+__global__ void __launch_bounds__(256) copy_rows_kernel(const S *__restrict__ src, int64_t lds, D *__restrict__ dst,
+                                                        int64_t ldd, int64_t rows, int64_t cols) {
+  const int64_t groups = (cols + 7) / 8, total = rows * groups;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / groups, c = (i - r * groups) * 8;
+    const S *s = src + r * lds + c;
+    __align__(16) D v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? convert<S, D>(s[j]) : D{};
+    if constexpr (sizeof(D) == 2) *reinterpret_cast<uint4 *>(dst + r * ldd + c) = *reinterpret_cast<const uint4 *>(v);
+    else *reinterpret_cast<uint2 *>(dst + r * ldd + c) = *reinterpret_cast<const uint2 *>(v);
+  }
+}
+
+int64_t padded(int64_t cols, int esz) { return (cols * esz + 15) / 16 * 16 / esz; }
+
+// An operand as the tensor core takes it: bf16 or e4m3 rows on 16-byte boundaries.
+struct Operand {
+  const void *p;
+  int64_t rows, cols, ld;  // as stored
+};
+
+int prepare_operand(Operand &o, int dtype, Scratch &scratch, cudaStream_t st) {
+  const int esz = dtype == TFORGE_E4M3 ? 1 : 2;
+  if (o.rows == 0 || o.cols == 0) return TFORGE_OK;
+  if (dtype != TFORGE_F32 && at(o.p, 16) && o.ld * esz % 16 == 0) return TFORGE_OK;
+  const int64_t ldd = padded(o.cols, esz);
+  void *q = nullptr;
+  int rc = scratch.get(&q, (uint64_t)o.rows * ldd * esz);
+  if (rc) return rc;
+  int64_t blocks = (o.rows * ((o.cols + 7) / 8) + 255) / 256;
+  if (blocks > 148 * 16) blocks = 148 * 16;
+  const unsigned g = (unsigned)blocks;
+  if (dtype == TFORGE_F32)
+    copy_rows_kernel<<<g, 256, 0, st>>>(static_cast<const float *>(o.p), o.ld, static_cast<__nv_bfloat16 *>(q), ldd, o.rows, o.cols);
+  else if (dtype == TFORGE_BF16)
+    copy_rows_kernel<<<g, 256, 0, st>>>(static_cast<const uint16_t *>(o.p), o.ld, static_cast<uint16_t *>(q), ldd, o.rows, o.cols);
+  else
+    copy_rows_kernel<<<g, 256, 0, st>>>(static_cast<const uint8_t *>(o.p), o.ld, static_cast<uint8_t *>(q), ldd, o.rows, o.cols);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_failure(e, "operand copy");
+  o.p = q;
+  o.ld = ldd;
+  return TFORGE_OK;
+}
+
+// ---- the products ---------------------------------------------------------------------------------
+
+struct Choice {
+  int tile;    // slim kernel: rows per tile
+  int splits;
+};
+
+// Slim kernel: the narrowest tile that holds all rows (an MN-major row operand comes in blocks of
+// 64), then as many CTAs per tile as the SMs hold at once -- two an SM, one of the widest tile --
+// with at least four stages of k each.
+Choice choose_slim(int64_t M, int64_t N, int64_t K, bool t_mn, int esz) {
+  Choice c{t_mn ? 64 : 16, 1};
+  while (c.tile < 256 && c.tile < M) c.tile *= 2;
+  const int64_t tiles = ((M + c.tile - 1) / c.tile) * ((N + 127) / 128);
+  const int64_t slots = c.tile == 256 ? 148 : 296, nkb = (K * esz + 127) / 128;
+  while (c.splits < 8 && tiles * c.splits * 2 <= slots && nkb / (c.splits * 2) >= 4) c.splits *= 2;
+  return c;
+}
+
+// out (M x N) = epilogue(rows . cols).  rows: M x K, or K x M with t_mn; cols: N x K, or K x N
+// with w_mn.  p carries the epilogue.
+int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool f8, int64_t M, int64_t N, int64_t K,
+            LinearParams p, cudaStream_t st) {
+  if (M == 0 || N == 0) return TFORGE_OK;
+  const int esz = f8 ? 1 : 2;
+  p.M = (int32_t)M;
+  p.N = (int32_t)N;
+  p.K = (int32_t)K;
+  int rc = device_status_word(&p.status);
+  if (rc) return rc;
+  p.limit_ns = wait_limit_ns();
+  p.debug_skip = debug_skip_load();
+  Choice c = choose_slim(M, N, K, t_mn, esz);
+  const uint32_t force = g_force.load();
+  if ((force & 255) == 1) {
+    c.tile = (force >> 8) & 0xFFFF;
+    c.splits = (int)(force >> 24);
+    if (t_mn && c.tile < 64) return TFORGE_ERR_UNSUPPORTED;
+  }
+  p.splits = c.splits;
+  CUtensorMap tmT{}, tmW{};
+  if (K > 0) {
+    const uint32_t bk = 128 / esz;
+    rc = t_mn ? encode_rows_map(&tmT, rows.p, esz, K, M, rows.ld, 64, 64)
+              : encode_rows_map(&tmT, rows.p, esz, M, K, rows.ld, bk, (uint32_t)c.tile);
+    if (rc) return rc;
+    rc = w_mn ? encode_rows_map(&tmW, cols.p, esz, K, N, cols.ld, 64, 64)
+              : encode_rows_map(&tmW, cols.p, esz, N, K, cols.ld, bk, 128);
+    if (rc) return rc;
+  }
+  cudaError_t e = launch_linear_slim(f8, w_mn, t_mn, c.tile, tmT, tmW, p, st);
+  return e == cudaSuccess ? TFORGE_OK : cuda_failure(e, "linear launch");
+}
+
+// ---- the gradient's elementwise pass ---------------------------------------------------------------
+
+// dz = dout * act'(pre) rounded to bf16 (dz null: not written), and part[b, n] = the f32 sum of the
+// unrounded dz over row block b (part null: not wanted).  A block takes 256 columns (a lane eight:
+// neighbouring ones with VEC, else 32 apart) and its 8 warps every 8th row of row block blockIdx.y.
+// Bound by HBM: reads 2 and writes 1 value an element.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+    activation_grad_kernel(int act, const T *__restrict__ dout, int64_t lddo, const T *__restrict__ pre, int64_t ldp,
+                           __nv_bfloat16 *__restrict__ dz, int64_t ldz, float *__restrict__ part, int64_t M, int64_t N) {
+  __shared__ float sm[8][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c0 = (int64_t)blockIdx.x * 256;
+  const int64_t per = (M + gridDim.y - 1) / gridDim.y, r0 = per * blockIdx.y, r1 = r0 + per < M ? r0 + per : M;
+  auto off = [&](int j) { return VEC ? lane * 8 + j : j * 32 + lane; };
+  float sum[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum[j] = 0.f;
+  auto read = [&](const T *row, float (&v)[8]) {
+    if constexpr (VEC) {
+      const bool in = c0 + lane * 8 < N;
+      if constexpr (sizeof(T) == 2) {
+        const uint4 u = in ? __ldg(reinterpret_cast<const uint4 *>(row + c0 + lane * 8)) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[2 * j] = __uint_as_float(w[j] << 16);
+          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 f = in ? __ldg(reinterpret_cast<const float4 *>(row + c0 + lane * 8) + h) : make_float4(0, 0, 0, 0);
+          v[4 * h] = f.x;
+          v[4 * h + 1] = f.y;
+          v[4 * h + 2] = f.z;
+          v[4 * h + 3] = f.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c0 + off(j) < N ? (float)row[c0 + off(j)] : 0.f;
+    }
+  };
+  with_activation(act, [&](auto a) {
+    constexpr int ACT = decltype(a)::value;
+#pragma unroll 2
+    for (int64_t m = r0 + warp; m < r1; m += 8) {
+      float g[8];
+      read(dout + m * lddo, g);
+      if constexpr (ACT != TFORGE_ACT_NONE) {
+        float z[8];
+        read(pre + m * ldp, z);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] *= activate_slope<ACT>(z[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] += g[j];
+      if (dz) {
+        if constexpr (VEC) {
+          if (c0 + lane * 8 < N)
+            *reinterpret_cast<uint4 *>(dz + m * ldz + c0 + lane * 8) =
+                make_uint4(pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]), pack_bf16x2(g[4], g[5]), pack_bf16x2(g[6], g[7]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (c0 + off(j) < N) dz[m * ldz + c0 + off(j)] = __float2bfloat16_rn(g[j]);
+        }
+      }
+    }
+  });
+  if (!part) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sm[warp][off(j)] = sum[j];
+  __syncthreads();
+  float v = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) v += sm[w][threadIdx.x];
+  const int64_t c = c0 + threadIdx.x;
+  if (c < N) part[(int64_t)blockIdx.y * N + c] = v;
+}
+
+template <typename T>
+cudaError_t launch_activation_grad(int act, const void *dout, int64_t lddo, const void *pre, int64_t ldp, void *dz,
+                                   int64_t ldz, float *part, int row_blocks, int64_t M, int64_t N, cudaStream_t st) {
+  const int e = sizeof(T);
+  const bool vec = N % 8 == 0 && at(dout, 16) && lddo * e % 16 == 0 &&
+                   (act == TFORGE_ACT_NONE || (at(pre, 16) && ldp * e % 16 == 0));
+  const dim3 g((unsigned)((N + 255) / 256), (unsigned)row_blocks);
+  auto kern = vec ? activation_grad_kernel<T, true> : activation_grad_kernel<T, false>;
+  kern<<<g, 256, 0, st>>>(act, static_cast<const T *>(dout), lddo, static_cast<const T *>(pre), ldp,
+                          static_cast<__nv_bfloat16 *>(dz), ldz, part, M, N);
+  return cudaGetLastError();
+}
+
+// Row blocks: about eight blocks an SM in all, each of at least 32 rows.
+int grad_row_blocks(int64_t M, int64_t N) {
+  const int64_t cols = (N + 255) / 256;
+  int64_t r = 148 * 8 / cols;
+  if (r > (M + 31) / 32) r = (M + 31) / 32;
+  return r < 1 ? 1 : (int)r;
+}
+
+int check_linear_types(int act, int trans_b, int a_dtype, int b_dtype) {
+  if (act < TFORGE_ACT_NONE || act > TFORGE_ACT_SILU || trans_b < 0 || trans_b > 1) return TFORGE_ERR_MODE;
+  return is_float(a_dtype) && is_float(b_dtype) ? TFORGE_OK : TFORGE_ERR_MODE;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tforge_linear(const tforge_linear_args *args, void *stream) {
+  if (!args) return TFORGE_ERR_NULL;
+  tforge_linear_args a = *args;
+  const bool f8 = a.a_dtype == TFORGE_E4M3 && a.b_dtype == TFORGE_E4M3;
+  int rc = f8 ? check_linear_types(a.activation, a.trans_b, TFORGE_BF16, TFORGE_BF16)
+              : check_linear_types(a.activation, a.trans_b, a.a_dtype, a.b_dtype);
+  if (rc) return rc;
+  if (!is_float(a.out_dtype) || (a.residual && !is_float(a.residual_dtype))) return TFORGE_ERR_MODE;
+  if (!f8 && (a.a_scale || a.b_scale)) return TFORGE_ERR_MODE;
+  if (f8 && !a.trans_b) return TFORGE_ERR_UNSUPPORTED;
+  if (!dims_ok(a.M, a.N, a.K)) return TFORGE_ERR_SHAPE;
+  const int64_t brows = a.trans_b ? a.N : a.K, bcols = a.trans_b ? a.K : a.N;
+  if (!pitch(a.lda, a.K) || !pitch(a.ldb, bcols) || !pitch(a.ldr, a.N) || !pitch(a.ldo, a.N) || !pitch(a.ldp, a.N))
+    return TFORGE_ERR_SHAPE;
+  if (a.M == 0 || a.N == 0) return TFORGE_OK;
+  if (!a.out || (a.K > 0 && (!a.A || !a.B)) || (f8 && (!a.a_scale || !a.b_scale))) return TFORGE_ERR_NULL;
+  const int eo = elem_size(a.out_dtype);
+  const Array ins[] = {{a.A, a.M, a.K, a.lda, elem_size(a.a_dtype)}, {a.B, brows, bcols, a.ldb, elem_size(a.b_dtype)},
+                       {a.a_scale, 1, a.M, a.M, 4}, {a.b_scale, 1, a.N, a.N, 4}, {a.bias, 1, a.N, a.N, 4},
+                       {a.residual, a.M, a.N, a.ldr, elem_size(a.residual_dtype)}};
+  const Array outs[] = {{a.out, a.M, a.N, a.ldo, eo}, {a.pre, a.M, a.N, a.ldp, eo}};
+  rc = check_arrays(ins, outs, 0, 5);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Scratch scratch(st);
+  Operand A{a.A, a.M, a.K, a.lda}, B{a.B, brows, bcols, a.ldb};
+  rc = prepare_operand(A, a.a_dtype, scratch, st);
+  if (!rc) rc = prepare_operand(B, a.b_dtype, scratch, st);
+  if (rc) return rc;
+  LinearParams p{};
+  p.bias = a.bias;
+  p.a_scale = a.a_scale;
+  p.b_scale = a.b_scale;
+  p.residual = a.residual;
+  p.ldr = a.ldr;
+  p.res_bf16 = a.residual_dtype == TFORGE_BF16;
+  p.out = a.out;
+  p.ldo = a.ldo;
+  p.pre = a.pre;
+  p.ldp = a.ldp;
+  p.out_bf16 = a.out_dtype == TFORGE_BF16;
+  p.act = a.activation;
+  return product(A, false, B, !a.trans_b, f8, a.M, a.N, a.K, p, st);
+}
+
+int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream) {
+  if (!args) return TFORGE_ERR_NULL;
+  tforge_linear_backward_args a = *args;
+  int rc = check_linear_types(a.activation, a.trans_b, a.a_dtype, a.b_dtype);
+  if (rc) return rc;
+  if (!is_float(a.dtype) || !is_float(a.grad_dtype)) return TFORGE_ERR_MODE;
+  if (!dims_ok(a.M, a.N, a.K)) return TFORGE_ERR_SHAPE;
+  const int64_t brows = a.trans_b ? a.N : a.K, bcols = a.trans_b ? a.K : a.N;
+  if (!pitch(a.lddo, a.N) || !pitch(a.ldp, a.N) || !pitch(a.lda, a.K) || !pitch(a.ldb, bcols) || !pitch(a.ldda, a.K) ||
+      !pitch(a.lddb, bcols))
+    return TFORGE_ERR_SHAPE;
+  const bool want_a = a.dA && a.M > 0 && a.K > 0, want_b = a.dB && a.N > 0 && a.K > 0, want_bias = a.dbias && a.N > 0;
+  if (!want_a && !want_b && !want_bias) return TFORGE_OK;
+  const bool some = a.M > 0 && a.N > 0;  // else every sum is over nothing
+  if (some && (!a.dout || (a.activation != TFORGE_ACT_NONE && !a.pre) || (want_a && !a.B) || (want_b && !a.A)))
+    return TFORGE_ERR_NULL;
+  const int ed = elem_size(a.dtype), eg = elem_size(a.grad_dtype);
+  const Array ins[] = {{a.dout, a.M, a.N, a.lddo, ed},
+                       {a.activation == TFORGE_ACT_NONE ? nullptr : a.pre, a.M, a.N, a.ldp, ed},
+                       {want_b ? a.A : nullptr, a.M, a.K, a.lda, elem_size(a.a_dtype)},
+                       {want_a ? a.B : nullptr, brows, bcols, a.ldb, elem_size(a.b_dtype)}};
+  const Array outs[] = {{a.dA, a.M, a.K, a.ldda, eg}, {a.dB, brows, bcols, a.lddb, eg}, {a.dbias, 1, a.N, a.N, 4}};
+  rc = check_arrays(ins, outs);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Scratch scratch(st);
+  // dz and the column sums, unless dout serves as it is.
+  Operand dz{a.dout, a.M, a.N, a.lddo};
+  const bool need_dz = some && (want_a || want_b) &&
+                       (a.activation != TFORGE_ACT_NONE || a.dtype == TFORGE_F32 || !at(a.dout, 16) || a.lddo % 8);
+  if (some && (need_dz || want_bias)) {
+    void *z = nullptr, *part = nullptr;
+    const int rb = grad_row_blocks(a.M, a.N);
+    if (need_dz) {
+      dz.ld = padded(a.N, 2);
+      rc = scratch.get(&z, (uint64_t)a.M * dz.ld * 2);
+      if (rc) return rc;
+      dz.p = z;
+    }
+    if (want_bias && rb > 1) {
+      rc = scratch.get(&part, (uint64_t)rb * a.N * 4);
+      if (rc) return rc;
+    }
+    float *sums = want_bias ? (rb > 1 ? static_cast<float *>(part) : a.dbias) : nullptr;
+    cudaError_t e = a.dtype == TFORGE_BF16
+                        ? launch_activation_grad<__nv_bfloat16>(a.activation, a.dout, a.lddo, a.pre, a.ldp, z, dz.ld, sums, rb, a.M, a.N, st)
+                        : launch_activation_grad<float>(a.activation, a.dout, a.lddo, a.pre, a.ldp, z, dz.ld, sums, rb, a.M, a.N, st);
+    if (e == cudaSuccess && part) e = launch_column_sum(static_cast<const float *>(part), rb, a.N, a.dbias, st);
+    if (e != cudaSuccess) return cuda_failure(e, "activation gradient");
+  } else if (want_bias) {
+    cudaError_t e = cudaMemsetAsync(a.dbias, 0, (size_t)a.N * 4, st);
+    if (e != cudaSuccess) return cuda_failure(e, "cudaMemsetAsync(dbias)");
+  }
+  LinearParams p{};
+  p.act = TFORGE_ACT_NONE;
+  p.out_bf16 = a.grad_dtype == TFORGE_BF16;
+  if (want_a) {
+    Operand B{a.B, brows, bcols, a.ldb};
+    if (some) rc = prepare_operand(B, a.b_dtype, scratch, st);
+    if (rc) return rc;
+    p.out = a.dA;
+    p.ldo = a.ldda;
+    rc = product(dz, false, B, a.trans_b != 0, false, a.M, a.K, a.N, p, st);
+    if (rc) return rc;
+  }
+  if (want_b) {
+    Operand A{a.A, a.M, a.K, a.lda};
+    if (some) rc = prepare_operand(A, a.a_dtype, scratch, st);
+    if (rc) return rc;
+    p.out = a.dB;
+    p.ldo = a.lddb;
+    rc = a.trans_b ? product(dz, true, A, true, false, a.N, a.K, a.M, p, st)
+                   : product(A, true, dz, true, false, a.K, a.N, a.M, p, st);
+    if (rc) return rc;
+  }
+  return TFORGE_OK;
+}
+
+int tforge_rms_norm(const tforge_rms_norm_args *args, void *stream) {
+  if (!args) return TFORGE_ERR_NULL;
+  tforge_rms_norm_args a = *args;
+  if (!is_float(a.dtype) || (a.weight && !is_float(a.weight_dtype)) ||
+      !(is_float(a.out_dtype) || a.out_dtype == TFORGE_E4M3))
+    return TFORGE_ERR_MODE;
+  if (!dims_ok(a.M, a.N) || !(a.eps >= 0.0f) || std::isinf(a.eps)) return TFORGE_ERR_SHAPE;
+  if (!pitch(a.ldx, a.N) || !pitch(a.ldr, a.N) || !pitch(a.lds, a.N) || !pitch(a.ldo, a.N)) return TFORGE_ERR_SHAPE;
+  if (a.M == 0 || a.N == 0) return TFORGE_OK;
+  if (!a.x || !a.out || (a.out_dtype == TFORGE_E4M3 && !a.scale)) return TFORGE_ERR_NULL;
+  const int e = elem_size(a.dtype);
+  const Array ins[] = {{a.x, a.M, a.N, a.ldx, e}, {a.residual, a.M, a.N, a.ldr, e},
+                       {a.weight, 1, a.N, a.N, elem_size(a.weight_dtype)}};
+  const Array outs[] = {{a.sum_out, a.M, a.N, a.lds, e}, {a.out, a.M, a.N, a.ldo, elem_size(a.out_dtype)},
+                        {a.out_dtype == TFORGE_E4M3 ? a.scale : nullptr, 1, a.M, a.M, 4}, {a.rstd, 1, a.M, a.M, 4}};
+  int rc = check_arrays(ins, outs, 0, 0, 1);
+  if (rc) return rc;
+  NormArgs p{};
+  p.x = a.x;
+  p.residual = a.residual;
+  p.weight = a.weight;
+  p.sum_out = a.sum_out;
+  p.out = a.out;
+  p.scale = a.scale;
+  p.rstd = a.rstd;
+  p.M = a.M;
+  p.N = a.N;
+  p.ldx = a.ldx;
+  p.ldr = a.ldr;
+  p.lds = a.lds;
+  p.ldo = a.ldo;
+  p.eps = a.eps;
+  p.x_bf16 = a.dtype == TFORGE_BF16;
+  p.w_bf16 = a.weight_dtype == TFORGE_BF16;
+  p.out_kind = a.out_dtype;
+  cudaError_t err = launch_rms_norm(p, true, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? TFORGE_OK : cuda_failure(err, "rms_norm launch");
+}
+
+int tforge_rms_norm_backward(const tforge_rms_norm_backward_args *args, void *stream) {
+  if (!args) return TFORGE_ERR_NULL;
+  tforge_rms_norm_backward_args a = *args;
+  if (!is_float(a.dtype) || (a.weight && !is_float(a.weight_dtype))) return TFORGE_ERR_MODE;
+  if (!dims_ok(a.M, a.N)) return TFORGE_ERR_SHAPE;
+  if (!pitch(a.lddy, a.N) || !pitch(a.lds, a.N) || !pitch(a.ldds, a.N) || !pitch(a.lddx, a.N)) return TFORGE_ERR_SHAPE;
+  if (a.N == 0) return TFORGE_OK;
+  if (a.M > 0 && (!a.dy || !a.s || !a.rstd || !a.dx)) return TFORGE_ERR_NULL;
+  const int e = elem_size(a.dtype);
+  const Array ins[] = {{a.dy, a.M, a.N, a.lddy, e}, {a.s, a.M, a.N, a.lds, e},
+                       {a.weight, 1, a.N, a.N, elem_size(a.weight_dtype)}, {a.rstd, 1, a.M, a.M, 4}, {a.ds, a.M, a.N, a.ldds, e}};
+  const Array outs[] = {{a.dx, a.M, a.N, a.lddx, e}, {a.dweight, 1, a.N, a.N, 4}};
+  int rc = check_arrays(ins, outs, 0, 4);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a.M == 0) {
+    cudaError_t err = a.dweight ? cudaMemsetAsync(a.dweight, 0, (size_t)a.N * 4, st) : cudaSuccess;
+    return err == cudaSuccess ? TFORGE_OK : cuda_failure(err, "cudaMemsetAsync(dweight)");
+  }
+  NormBwdArgs p{};
+  p.dy = a.dy;
+  p.s = a.s;
+  p.weight = a.weight;
+  p.ds = a.ds;
+  p.rstd = a.rstd;
+  p.dx = a.dx;
+  p.M = a.M;
+  p.N = a.N;
+  p.lddy = a.lddy;
+  p.lds = a.lds;
+  p.ldds = a.ldds;
+  p.lddx = a.lddx;
+  p.x_bf16 = a.dtype == TFORGE_BF16;
+  p.w_bf16 = a.weight_dtype == TFORGE_BF16;
+  const int parts = rms_norm_bwd_parts(a.M, a.N);
+  Scratch scratch(st);
+  void *part = nullptr;
+  if (a.dweight && parts > 1) {
+    rc = scratch.get(&part, (uint64_t)parts * a.N * 4);
+    if (rc) return rc;
+  }
+  float *sums = a.dweight ? (parts > 1 ? static_cast<float *>(part) : a.dweight) : nullptr;
+  cudaError_t err = launch_rms_norm_bwd(p, sums, parts, st);
+  if (err == cudaSuccess && part) err = launch_column_sum(static_cast<const float *>(part), parts, a.N, a.dweight, st);
+  return err == cudaSuccess ? TFORGE_OK : cuda_failure(err, "rms_norm_backward launch");
+}
+
+int tforge_quantize_e4m3(const void *x, int dtype, uint8_t *q, float *scale, int64_t M, int64_t N, int64_t ldx,
+                         int64_t ldq, void *stream) {
+  if (!is_float(dtype)) return TFORGE_ERR_MODE;
+  if (!dims_ok(M, N) || !pitch(ldx, N) || !pitch(ldq, N)) return TFORGE_ERR_SHAPE;
+  if (M == 0 || N == 0) return TFORGE_OK;
+  if (!x || !q || !scale) return TFORGE_ERR_NULL;
+  const Array ins[] = {{x, M, N, ldx, elem_size(dtype)}};
+  const Array outs[] = {{q, M, N, ldq, 1}, {scale, 1, M, M, 4}};
+  int rc = check_arrays(ins, outs);
+  if (rc) return rc;
+  NormArgs p{};
+  p.x = x;
+  p.out = q;
+  p.scale = scale;
+  p.M = M;
+  p.N = N;
+  p.ldx = ldx;
+  p.ldo = ldq;
+  p.x_bf16 = dtype == TFORGE_BF16;
+  p.out_kind = TFORGE_E4M3;
+  cudaError_t err = launch_rms_norm(p, false, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? TFORGE_OK : cuda_failure(err, "quantize_e4m3 launch");
+}
+
+int tforge_debug_linear_kernel(int kernel, int tile, int splits) {
+  const bool tile_ok = tile == 16 || tile == 32 || tile == 64 || tile == 128 || tile == 256;
+  const bool split_ok = splits == 1 || splits == 2 || splits == 4 || splits == 8;
+  if (kernel < 0 || kernel > 1 || (kernel == 1 && (!tile_ok || !split_ok))) return TFORGE_ERR_MODE;
+  g_force.store(kernel == 1 ? 1u | (uint32_t)tile << 8 | (uint32_t)splits << 24 : (uint32_t)kernel);
+  return TFORGE_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,302 @@
+// tf_linear_slim.cu -- the linear layer on one CTA per tile with the operands exchanged: the
+// weights' columns are the tensor core's 128 rows and BT = 16 .. 256 tokens its columns, so that a
+// few tokens (BT 16: a decoding batch) cost no padding to 128.
+//
+//   out[m, n] = act((sum_k A[m, k] B[k, n]) a_scale[m] b_scale[n] + bias[n]) + residual[m, n]
+//
+// Operands are bf16 or e4m3, 128 bytes of k a stage, each K-major or (bf16) MN-major as it lies in
+// memory, brought by TMA into a ring of 128-B-swizzled tiles; one thread issues the MMAs; the
+// accumulator is BT columns of tensor memory.  With few tiles a cluster of S CTAs shares a tile:
+// CTA z takes the z-th part of k, leaves its f32 sums in its shared memory, and after a cluster
+// barrier each CTA adds 1/S of the tile's values from all S, in order of z (the same bits every
+// time), and finishes them.
+//
+// The output tile is transposed in tensor memory (lane = column n), so a warp's 32 lanes hold 32
+// neighbouring columns of one token: residual reads and output writes are coalesced at any
+// alignment and pitch, without staging.
+//
+// 256 threads: warp 0 TMA producer, warp 1 MMA issuer, then all eight warps the epilogue (two per
+// 32-lane quadrant, taking token chunks in turn).  Every wait is bounded (tf_ptx.cuh).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "tf_epilogue.cuh"
+#include "tf_internal.h"
+#include "tf_ptx.cuh"
+
+namespace tf {
+
+namespace {
+
+template <int BT, int STAGES>
+struct SlimLayout {
+  static constexpr int kThreads = 256;
+  static constexpr int kWBytes = 128 * 128;  // 128 columns n x 128 B of k
+  static constexpr int kTBytes = BT * 128;   // BT tokens x 128 B of k
+  static constexpr int kStageBytes = kWBytes + kTBytes;
+  static constexpr int kRing = STAGES * kStageBytes;
+  static constexpr int kBarOff = kRing;
+  // full[STAGES], empty[STAGES], accf; then the TMEM slot and the abort flag.
+  static constexpr int kSmemBytes = 1024 + kBarOff + 8 * (2 * STAGES + 1) + 16;
+  static constexpr int kTmemCols = BT < 32 ? 32 : BT;
+  static_assert(BT * 512 <= kRing, "the partial sums reuse the ring");
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+
+__device__ __forceinline__ float residual_at(const LinearParams &p, int64_t i) {
+  return p.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.residual)[i])
+                    : static_cast<const float *>(p.residual)[i];
+}
+__device__ __forceinline__ void put(void *base, int bf16, int64_t i, float v) {
+  if (bf16) static_cast<__nv_bfloat16 *>(base)[i] = __float2bfloat16_rn(v);
+  else static_cast<float *>(base)[i] = v;
+}
+
+// Finishes CNT tokens j = j0 .. j0 + CNT - 1 of column n (bias and b_scale: bn, sn).
+template <int CNT>
+__device__ __forceinline__ void finish_column(const LinearParams &p, float (&v)[CNT], int64_t m0, int64_t n, float bn,
+                                              float sn) {
+  float res[CNT];
+#pragma unroll
+  for (int j = 0; j < CNT; ++j) res[j] = p.residual && m0 + j < p.M ? residual_at(p, (m0 + j) * p.ldr + n) : 0.f;
+#pragma unroll
+  for (int j = 0; j < CNT; ++j) {
+    if (p.a_scale && m0 + j < p.M) v[j] = v[j] * __ldg(p.a_scale + m0 + j) * sn;
+    v[j] += bn;
+    if (p.pre && m0 + j < p.M) put(p.pre, p.out_bf16, (m0 + j) * p.ldp + n, v[j]);
+  }
+  with_activation(p.act, [&](auto act) {
+#pragma unroll
+    for (int j = 0; j < CNT; ++j) v[j] = activate<decltype(act)::value>(v[j]);
+  });
+#pragma unroll
+  for (int j = 0; j < CNT; ++j)
+    if (m0 + j < p.M) put(p.out, p.out_bf16, (m0 + j) * p.ldo + n, p.residual ? v[j] + res[j] : v[j]);
+}
+
+// F8: e4m3 operands (both K-major).  WMN / TMN: the weights' / tokens' tile is MN-major (bf16).
+template <bool F8, bool WMN, bool TMN, int BT, int STAGES>
+__global__ void __launch_bounds__(256)
+    linear_slim_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
+                       const LinearParams p) {
+  using L = SlimLayout<BT, STAGES>;
+  static_assert(!F8 || (!WMN && !TMN), "8-bit operands are K-major");
+  static_assert(!TMN || BT % 64 == 0, "MN-major tokens come in blocks of 64");
+  constexpr int kElem = F8 ? 1 : 2, kBK = 128 / kElem;
+  constexpr uint32_t kIdesc = instr_desc_majors(F8 ? 0u : 1u, 128, BT, WMN, TMN);
+  using MN = BTileMN<2>;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBarOff);
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * STAGES, accf = empty0 + 8 * STAGES;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 1);
+  volatile uint32_t *abort_flag = tmem_slot + 1;
+  const WaitCtl wc{abort_flag, p.status, p.limit_ns};
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles_m = (p.M + BT - 1) / BT, tiles_n = (p.N + 127) / 128;
+  int tm, tn;
+  raster_tile((int)blockIdx.x, tiles_m, tiles_n, kRasterGroup, tm, tn);
+  const int m0 = tm * BT, n0 = tn * 128;
+  const int z = (int)blockIdx.z, splits = (int)gridDim.z;
+  const int nkb_all = (p.K + kBK - 1) / kBK;
+  const int kb0 = (int)((int64_t)nkb_all * z / splits), nkb = (int)((int64_t)nkb_all * (z + 1) / splits) - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    mbar_init(accf, 1);
+    *abort_flag = 0u;
+    fence_mbar_init();
+    if (p.K > 0) {  // K = 0: no maps
+      tma_prefetch_desc(&tmT);
+      tma_prefetch_desc(&tmW);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), L::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    grid_dependency_wait();
+    int kb = 0;
+    for (; kb < nkb; ++kb) {
+      const int s = kb % STAGES, round = kb / STAGES;
+      if (round > 0 && !mbar_wait(empty0 + 8 * s, (round - 1) & 1, wc)) break;
+      if (p.debug_skip && kb == 0) continue;  // test hook: this stage never fills
+      const uint32_t slot = sbase + s * L::kStageBytes, bar = full0 + 8 * s;
+      const int kc = (kb0 + kb) * kBK;
+      mbar_arrive_expect_tx(bar, L::kStageBytes);
+      if constexpr (WMN) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) tma_load_2d(slot + j * 8192, &tmW, n0 + 64 * j, kc, bar);
+      } else {
+        tma_load_2d(slot, &tmW, kc, n0, bar);
+      }
+      if constexpr (TMN) {
+#pragma unroll
+        for (int j = 0; j < BT / 64; ++j) tma_load_2d(slot + L::kWBytes + j * 8192, &tmT, m0 + 64 * j, kc, bar);
+      } else {
+        tma_load_2d(slot + L::kWBytes, &tmT, kc, m0, bar);
+      }
+    }
+    if (*abort_flag) {  // no load may be in flight when this CTA leaves
+#pragma unroll 1
+      for (int s = 0; s < STAGES; ++s) {
+        if (kb - 1 < s) continue;
+        const int last = kb - 1 - ((kb - 1 - s) % STAGES);
+        if (p.debug_skip && last == 0) continue;
+        mbar_wait_drain(full0 + 8 * s, (last / STAGES) & 1, p.limit_ns);
+      }
+    }
+  } else if (warp == 1 && lane == 0 && nkb > 0) {
+    const uint64_t w_d0 = WMN ? MN::desc(sbase, 0, false) : smem_desc(sbase, 16, 1024, 2);
+    const uint64_t t_d0 = TMN ? MN::desc(sbase + L::kWBytes, 0, false) : smem_desc(sbase + L::kWBytes, 16, 1024, 2);
+    constexpr uint32_t kWStep = WMN ? MN::step(false) >> 4 : 2u, kTStep = TMN ? MN::step(false) >> 4 : 2u;
+    int s = 0;
+    uint32_t phase = 0;
+    uint64_t so = 0;
+    for (int kb = 0; kb < nkb; ++kb) {
+      if (!mbar_wait(full0 + 8 * s, phase, wc)) break;
+      tc_fence_after();
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        if constexpr (F8) mma_ss_f8(tmem, w_d0 + so + ks * kWStep, t_d0 + so + ks * kTStep, kIdesc, (kb | ks) ? 1u : 0u);
+        else mma_ss<false>(tmem, w_d0 + so + ks * kWStep, t_d0 + so + ks * kTStep, kIdesc, (kb | ks) ? 1u : 0u);
+      }
+      mma_commit(empty0 + 8 * s);
+      so += L::kStageBytes >> 4;
+      if (++s == STAGES) {
+        s = 0;
+        phase ^= 1u;
+        so = 0;
+      }
+    }
+    mma_commit(accf);
+    if (*abort_flag) mbar_wait_drain(accf, 0, p.limit_ns);
+  }
+  __syncwarp();
+
+  // ---------------- epilogue: all warps; warp w reads TMEM lanes 32 (w % 4) .. + 31 ----------------
+  grid_dependency_wait();  // bias, scales, residual: written by the kernel before; outputs: read by it
+  const int q = warp & 3, half = warp >> 2, r = q * 32 + lane, n = n0 + r;
+  const bool ok = nkb == 0 || (mbar_wait(accf, 0, wc) && !*abort_flag);
+  tc_fence_after();
+  const bool col_ok = n < p.N;
+  const float bn = p.bias && col_ok ? __ldg(p.bias + n) : 0.f, sn = p.b_scale && col_ok ? __ldg(p.b_scale + n) : 1.f;
+  const uint32_t tacc = tmem + ((uint32_t)(q * 32) << 16);
+  if (splits == 1) {
+#pragma unroll 1
+    for (int c = half; c < BT / 16; c += 2) {
+      if (m0 + 16 * c >= p.M) break;
+      uint32_t rr[16];
+      float v[16];
+      if (__all_sync(0xFFFFFFFFu, ok && nkb > 0)) {
+        tmem_ld_32x32b_x16(tacc + 16 * c, rr);
+        tmem_ld_wait(rr);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) rr[j] = 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(rr[j]);
+      if (ok && col_ok) finish_column<16>(p, v, m0 + 16 * c, n, bn, sn);
+    }
+  } else {
+    // Partial sums, token by token: value (j, r) at float j * 128 + r of the ring (every load has
+    // been consumed), neighbouring lanes in neighbouring banks.
+    float *part = reinterpret_cast<float *>(smem);
+#pragma unroll 1
+    for (int c = half; c < BT / 16; c += 2) {
+      if (m0 + 16 * c >= p.M) break;
+      uint32_t rr[16];
+      if (__all_sync(0xFFFFFFFFu, ok && nkb > 0)) {
+        tmem_ld_32x32b_x16(tacc + 16 * c, rr);
+        tmem_ld_wait(rr);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) rr[j] = 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) part[(16 * c + j) * 128 + r] = __uint_as_float(rr[j]);
+    }
+    cluster_sync();
+    // CTA z finishes tokens z, z + S, ... of the tile, two at a time by its thread halves.
+    const int live = p.M - m0 < BT ? p.M - m0 : BT;
+    uint32_t src[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) src[s] = s < splits ? map_to_cta(sbase, s) : 0u;
+#pragma unroll 1
+    for (int j = z + splits * half; j < live; j += 2 * splits) {
+      float v[1] = {0.f};
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s < splits) v[0] += ld_cluster_f32(src[s] + (j * 128 + r) * 4);
+      if (ok && col_ok) finish_column<1>(p, v, m0 + j, n, bn, sn);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (splits > 1) cluster_sync();  // no CTA leaves while another may read its sums
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kTmemCols);
+  }
+}
+
+template <bool F8, bool WMN, bool TMN, int BT, int STAGES>
+cudaError_t launch_slim_kern(const CUtensorMap &tmT, const CUtensorMap &tmW, const LinearParams &p, cudaStream_t st) {
+  using L = SlimLayout<BT, STAGES>;
+  auto kern = linear_slim_kernel<F8, WMN, TMN, BT, STAGES>;
+  static unsigned long long configured = 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(__atomic_load_n(&configured, __ATOMIC_ACQUIRE) & bit)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    __atomic_fetch_or(&configured, bit, __ATOMIC_RELEASE);
+  }
+  const int64_t tiles = (int64_t)((p.M + BT - 1) / BT) * ((p.N + 127) / 128);
+  if (tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = (unsigned)p.splits;
+  cudaLaunchConfig_t cfg = {dim3((unsigned)tiles, 1, (unsigned)p.splits), dim3(L::kThreads), (size_t)L::kSmemBytes, st, attr, 1};
+  return cudaLaunchKernelEx(&cfg, kern, tmT, tmW, p);
+}
+
+// Ring depths: two CTAs an SM (about 100 KB each) up to 128 tokens, one with 256.
+template <bool F8, bool WMN, bool TMN>
+cudaError_t launch_slim_bt(int bt, const CUtensorMap &tmT, const CUtensorMap &tmW, const LinearParams &p, cudaStream_t st) {
+  if constexpr (!TMN) {
+    if (bt == 16) return launch_slim_kern<F8, WMN, TMN, 16, 6>(tmT, tmW, p, st);
+    if (bt == 32) return launch_slim_kern<F8, WMN, TMN, 32, 5>(tmT, tmW, p, st);
+  }
+  if (bt == 64) return launch_slim_kern<F8, WMN, TMN, 64, 4>(tmT, tmW, p, st);
+  if (bt == 128) return launch_slim_kern<F8, WMN, TMN, 128, 3>(tmT, tmW, p, st);
+  if (bt == 256) return launch_slim_kern<F8, WMN, TMN, 256, 4>(tmT, tmW, p, st);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t launch_linear_slim(bool f8, bool w_mn, bool t_mn, int bt, const CUtensorMap &tmT, const CUtensorMap &tmW,
+                               const LinearParams &p, cudaStream_t st) {
+  if (f8) return w_mn || t_mn ? cudaErrorInvalidValue : launch_slim_bt<true, false, false>(bt, tmT, tmW, p, st);
+  if (t_mn) return w_mn ? launch_slim_bt<false, true, true>(bt, tmT, tmW, p, st) : cudaErrorInvalidValue;
+  return w_mn ? launch_slim_bt<false, true, false>(bt, tmT, tmW, p, st) : launch_slim_bt<false, false, false>(bt, tmT, tmW, p, st);
+}
+
+}  // namespace tf
