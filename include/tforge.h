@@ -319,7 +319,7 @@ int tforge_debug_skip_load(int on);
 
 /* Test hook: the kernel that tforge_linear's and tforge_linear_backward's products take.  kernel 0:
  * chosen by size; 1: one CTA per 128 columns x `tile` rows (16, 32, 64, 128 or 256), `splits` CTAs
- * (1, 2, 4 or 8) sharing a tile's K.  A forced kernel that cannot take a product gives
+ * (1, 2, 4 or 8) sharing a tile's K; 2: persistent CTA pairs on 256 x 256 tiles.  A forced kernel that cannot take a product gives
  * TFORGE_ERR_UNSUPPORTED. */
 int tforge_debug_linear_kernel(int kernel, int tile, int splits);
 

@@ -24,7 +24,7 @@ LIB = PKG / "libtforge_gpu.so"
 RUNNER = PKG / "tforge-gpu-bench"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 LIB_SOURCES = ["tf_api.cu", "tf_gemm_tc.cu", "tf_gemm_2sm.cu", "tf_simt.cu", "tf_noalloc.cu", "tf_host.cu",
-               "tf_gemm_2sm_persist.cu", "tf_norm.cu", "tf_linear_slim.cu", "tf_layer.cu"]
+               "tf_gemm_2sm_persist.cu", "tf_norm.cu", "tf_linear_slim.cu", "tf_linear_pair.cu", "tf_layer.cu"]
 
 
 def nvcc() -> str:

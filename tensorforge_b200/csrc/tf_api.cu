@@ -596,6 +596,10 @@ int encode_rows_map(CUtensorMap *m, const void *base, int esz, int64_t rows, int
   return TFORGE_OK;
 }
 
+int encode_out_map(CUtensorMap *m, void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld) {
+  return make_tmap(m, base, bf16, rows, cols, ld, 32, 128, bf16 ? SW64 : SW128);
+}
+
 int device_pool(cudaMemPool_t *out) { return scratch_pool(out); }
 int device_status_word(uint32_t **out) { return status_word(out); }
 int cuda_failure(cudaError_t e, const char *what) { return cuda_fail(e, what); }

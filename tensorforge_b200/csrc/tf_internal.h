@@ -191,12 +191,22 @@ struct LinearParams {
   uint64_t limit_ns;              // bounded-wait limit
   int32_t debug_skip;             // test hook: skip the first stage's loads
   int32_t splits;                 // slim kernel: CTAs that share a tile's k (1, 2, 4 or 8)
+  // Pair kernel: out, pre and the residual start their rows on 16-byte boundaries, so that TMA
+  // stores the tiles (and tmO, tmP are set) and the residual is read 16 bytes at a time.
+  int32_t tma_out;
 };
 // One-CTA kernel of 128 columns x bt tokens (16, 32, 64, 128, 256; from 64 with t_mn).  tmT: A as
 // {128 B of k x bt rows} boxes, or with t_mn (A stored k x m) {64 columns x 64 rows}; tmW: B stored
 // n x k as {128 B x 128 rows} boxes, or with w_mn (stored k x n) {64 columns x 64 rows}.
 cudaError_t launch_linear_slim(bool f8, bool w_mn, bool t_mn, int bt, const CUtensorMap &tmT, const CUtensorMap &tmW,
                                const LinearParams &p, cudaStream_t stream);
+
+// Persistent CTA pairs on 256 x 256 tiles, K > 0.  tmA / tmB: as tmT / tmW above with 128 rows a
+// box.  tmO / tmP: maps of out and pre (encode_out_map), read when p.tma_out.
+cudaError_t launch_linear_pair(bool f8, bool a_mn, bool b_mn, const CUtensorMap &tmA, const CUtensorMap &tmB,
+                               const CUtensorMap &tmO, const CUtensorMap &tmP, const LinearParams &p, cudaStream_t stream);
+// Output map: boxes of 32 columns x 128 rows, f32 in the 128-byte or bf16 in the 64-byte swizzle.
+int encode_out_map(CUtensorMap *m, void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld);
 
 // tforge_rms_norm / tforge_quantize_e4m3 with every pitch filled in (tf_norm.cu).
 struct NormArgs {

@@ -1,6 +1,7 @@
 // tf_layer.cu -- C-ABI of the transformer-layer operators (include/tforge.h): argument checks,
 // operand copies where TMA cannot read the caller's rows, the choice of the product's kernel, and
-// the gradient's elementwise pass.  The kernels are in tf_linear_slim.cu and tf_norm.cu.
+// the gradient's elementwise pass.  The kernels are in tf_linear_slim.cu, tf_linear_pair.cu and
+// tf_norm.cu.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -182,6 +183,23 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
   p.debug_skip = debug_skip_load();
   Choice c = choose_slim(M, N, K, t_mn, esz);
   const uint32_t force = g_force.load();
+  const bool pair = (force & 255) == 2;
+  if (pair) {
+    if (K == 0) return TFORGE_ERR_UNSUPPORTED;
+    auto rows16 = [](const void *q, int64_t ld, int e) { return at(q, 16) && ld * e % 16 == 0; };
+    const int eo = p.out_bf16 ? 2 : 4;
+    p.tma_out = rows16(p.out, p.ldo, eo) && (!p.pre || rows16(p.pre, p.ldp, eo)) &&
+                (!p.residual || rows16(p.residual, p.ldr, p.res_bf16 ? 2 : 4));
+    CUtensorMap tmA{}, tmB{}, tmO{}, tmP{};
+    const uint32_t bk = 128 / esz;
+    rc = t_mn ? encode_rows_map(&tmA, rows.p, esz, K, M, rows.ld, 64, 64) : encode_rows_map(&tmA, rows.p, esz, M, K, rows.ld, bk, 128);
+    if (!rc) rc = w_mn ? encode_rows_map(&tmB, cols.p, esz, K, N, cols.ld, 64, 64) : encode_rows_map(&tmB, cols.p, esz, N, K, cols.ld, bk, 128);
+    if (!rc && p.tma_out) rc = encode_out_map(&tmO, p.out, p.out_bf16 != 0, M, N, p.ldo);
+    if (!rc && p.tma_out && p.pre) rc = encode_out_map(&tmP, p.pre, p.out_bf16 != 0, M, N, p.ldp);
+    if (rc) return rc;
+    cudaError_t e = launch_linear_pair(f8, t_mn, w_mn, tmA, tmB, tmO, tmP, p, st);
+    return e == cudaSuccess ? TFORGE_OK : cuda_failure(e, "linear launch");
+  }
   if ((force & 255) == 1) {
     c.tile = (force >> 8) & 0xFFFF;
     c.splits = (int)(force >> 24);
@@ -550,7 +568,7 @@ int tforge_quantize_e4m3(const void *x, int dtype, uint8_t *q, float *scale, int
 int tforge_debug_linear_kernel(int kernel, int tile, int splits) {
   const bool tile_ok = tile == 16 || tile == 32 || tile == 64 || tile == 128 || tile == 256;
   const bool split_ok = splits == 1 || splits == 2 || splits == 4 || splits == 8;
-  if (kernel < 0 || kernel > 1 || (kernel == 1 && (!tile_ok || !split_ok))) return TFORGE_ERR_MODE;
+  if (kernel < 0 || kernel > 2 || (kernel == 1 && (!tile_ok || !split_ok))) return TFORGE_ERR_MODE;
   g_force.store(kernel == 1 ? 1u | (uint32_t)tile << 8 | (uint32_t)splits << 24 : (uint32_t)kernel);
   return TFORGE_OK;
 }

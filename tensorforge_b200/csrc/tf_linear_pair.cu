@@ -1,0 +1,452 @@
+// tf_linear_pair.cu -- the linear layer's large products: persistent CTA pairs on 256 x 256 tiles.
+//
+//   out[m, n] = act((sum_k A[m, k] B[k, n]) a_scale[m] b_scale[n] + bias[n]) + residual[m, n]
+//
+// Each cluster of two CTAs walks over output tiles (grouped raster order) with one ring of TMA
+// stages running across them -- 128 bytes of k of this CTA's 128 rows of A and of its 128 columns
+// of B, each operand K-major or (bf16) MN-major as it lies in memory -- and two accumulators of 256
+// TMEM columns: the pair's MMAs (cta_group::2, 256 x 256, bf16 or e4m3) fill one while the epilogue
+// empties the other.
+//
+// Epilogue: eight warps a CTA in two groups of four, each group every second chunk of 32 columns, so
+// that one group's residual loads and stores overlap the other's arithmetic.  A thread holds 32
+// columns of one row; the row's scale is its own, the columns' bias and scale are a lane's and go
+// round by shuffles.  Outputs whose rows start on 16-byte boundaries leave through swizzled staging
+// boxes and TMA stores, others through the same boxes turned round, a warp storing 32 neighbouring
+// columns of one row at a time.
+//
+// 384 threads: warp 0 TMA producer (both CTAs), warp 1 MMA issuer (leader), warps 4..11 epilogue.
+// Every wait is bounded (tf_ptx.cuh); after an expiry each role stops, the producer and the issuer
+// wait (bounded) for what they have in flight, and both CTAs meet before TMEM is freed.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "tf_epilogue.cuh"
+#include "tf_internal.h"
+#include "tf_ptx.cuh"
+
+namespace tf {
+
+namespace {
+
+constexpr int kPairStages = 6;
+
+struct PairL {
+  static constexpr int kThreads = 384;
+  static constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kBoxOff = kPairStages * kStageBytes;
+  static constexpr int kBoxBytes = 128 * 128;  // a group's: 128 rows x 32 f32, or two of 32 bf16
+  static constexpr int kBarOff = kBoxOff + 2 * kBoxBytes;
+  // full[], empty[], accf[2], acce[2], drain; then the TMEM slot, the abort flag, the groups' go words.
+  static constexpr int kNumBars = 2 * kPairStages + 5;
+  static constexpr int kSmemBytes = 1024 + kBarOff + 8 * kNumBars + 32;
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+
+// Columns col .. col + CNT - 1 of one residual row (16-byte aligned groups), 0 beyond N.
+template <int CNT>
+__device__ __forceinline__ void load_residual(const LinearParams &p, int64_t row, int col, float (&v)[CNT]) {
+  if (p.res_bf16) {
+    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.residual) + row * p.ldr + col;
+#pragma unroll
+    for (int u = 0; u < CNT / 8; ++u) {
+      if (col + 8 * u + 8 <= p.N) {
+        const uint4 q = *reinterpret_cast<const uint4 *>(src + 8 * u);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[8 * u + 2 * i] = __uint_as_float(w[i] << 16);
+          v[8 * u + 2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[8 * u + i] = col + 8 * u + i < p.N ? __bfloat162float(src[8 * u + i]) : 0.f;
+      }
+    }
+  } else {
+    const float *src = static_cast<const float *>(p.residual) + row * p.ldr + col;
+#pragma unroll
+    for (int u = 0; u < CNT / 4; ++u) {
+      if (col + 4 * u + 4 <= p.N) {
+        const float4 q = *reinterpret_cast<const float4 *>(src + 4 * u);
+        v[4 * u] = q.x;
+        v[4 * u + 1] = q.y;
+        v[4 * u + 2] = q.z;
+        v[4 * u + 3] = q.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * u + i] = col + 4 * u + i < p.N ? src[4 * u + i] : 0.f;
+      }
+    }
+  }
+}
+
+// Row r of a staging box: 32 f32 (128-B swizzle) or 32 bf16 (64-B swizzle), as the output maps say.
+__device__ __forceinline__ void stage_row(uint8_t *box, int r, bool bf16, const float (&v)[32]) {
+  if (bf16) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      *reinterpret_cast<uint4 *>(box + r * 64 + ((u ^ ((r >> 1) & 3)) << 4)) =
+          make_uint4(pack_bf16x2(v[8 * u], v[8 * u + 1]), pack_bf16x2(v[8 * u + 2], v[8 * u + 3]),
+                     pack_bf16x2(v[8 * u + 4], v[8 * u + 5]), pack_bf16x2(v[8 * u + 6], v[8 * u + 7]));
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      *reinterpret_cast<float4 *>(box + r * 128 + ((u ^ (r & 7)) << 4)) =
+          make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+  }
+}
+
+// A warp's 32 rows x 32 columns turned round through its own 4 KB (column j of row l at j ^ l) and
+// stored row by row, a lane a column; `res` adds the residual.
+__device__ __forceinline__ void store_turned(const LinearParams &p, float *buf, int lane, int64_t row0, int col0, void *base,
+                                             int64_t ld, bool res, const float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) buf[lane * 32 + (j ^ lane)] = v[j];
+  __syncwarp();
+  const int rows = p.M - row0 < 32 ? (int)(p.M - row0) : 32;
+  if (col0 + lane < p.N) {
+#pragma unroll 4
+    for (int l = 0; l < rows; ++l) {
+      float x = buf[l * 32 + (lane ^ l)];
+      if (res) {
+        const int64_t i = (row0 + l) * p.ldr + col0 + lane;
+        x += p.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.residual)[i])
+                        : static_cast<const float *>(p.residual)[i];
+      }
+      const int64_t o = (row0 + l) * ld + col0 + lane;
+      if (p.out_bf16) static_cast<__nv_bfloat16 *>(base)[o] = __float2bfloat16_rn(x);
+      else static_cast<float *>(base)[o] = x;
+    }
+  }
+  __syncwarp();
+}
+
+// F8: e4m3 operands (both K-major).  AMN / BMN: A / B is MN-major (bf16).
+template <bool F8, bool AMN, bool BMN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                       const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmP,
+                       const LinearParams p) {
+  using L = PairL;
+  constexpr int STAGES = kPairStages;
+  static_assert(!F8 || (!AMN && !BMN), "8-bit operands are K-major");
+  constexpr int kBK = F8 ? 128 : 64;
+  constexpr uint32_t kIdesc = instr_desc_majors(F8 ? 0u : 1u, 256, 256, AMN, BMN);
+  using MN = BTileMN<2>;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBarOff);
+  // full[s] (leader's): both CTAs' bytes of slot s landed; empty[s]: the MMAs reading slot s are done
+  // (both CTAs); accf[b]: accumulator b holds a tile (both CTAs); acce[b] (leader's): both CTAs'
+  // epilogues have read accumulator b; drain: MMAs in flight after an abort.
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * STAGES, accf0 = empty0 + 8 * STAGES, acce0 = accf0 + 16,
+                 drainf = acce0 + 16;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
+  volatile uint32_t *abort_flag = tmem_slot + 1;
+  const WaitCtl wc{abort_flag, p.status, p.limit_ns};
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int tiles_m = (p.M + 255) / 256, tiles_n = (p.N + 255) / 256, tiles = tiles_m * tiles_n;
+  const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
+  const int my_tiles = pair < tiles ? (tiles - 1 - pair) / npairs + 1 : 0;
+  const int nkb = (p.K + kBK - 1) / kBK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(accf0 + 8 * b, 1);
+      mbar_init(acce0 + 8 * b, 16);  // lane 0 of the eight epilogue warps of both CTAs
+    }
+    mbar_init(drainf, 1);
+    *abort_flag = 0u;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    if (p.tma_out) tma_prefetch_desc(&tmO);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the peer's barriers are initialised before any remote arrive or TMA
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    grid_dependency_wait();
+    const uint32_t lead_full0 = map_to_cta(full0, 0);
+    int g = 0;  // k-blocks issued so far
+    bool ok = true;
+    for (int i = 0; i < my_tiles && ok; ++i) {
+      int tm, tn;
+      raster_tile(pair + i * npairs, tiles_m, tiles_n, kRasterGroup, tm, tn);
+      const int m0 = tm * 256 + (int)rank * 128, n0 = tn * 256 + (int)rank * 128;
+      for (int kb = 0; kb < nkb; ++kb, ++g) {
+        const int s = g % STAGES, round = g / STAGES;
+        if (round > 0 && !mbar_wait_cluster(empty0 + 8 * s, (round - 1) & 1, wc)) {
+          ok = false;
+          break;
+        }
+        if (p.debug_skip && g == 0) continue;  // test hook: this stage never fills
+        const int kc = kb * kBK;
+        const uint32_t slot = sbase + s * L::kStageBytes, bar = lead_full0 + 8 * s;
+        if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * L::kStageBytes);
+        if constexpr (AMN) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) tma_load_2d_pair(slot + j * 8192, &tmA, m0 + 64 * j, kc, bar);
+        } else {
+          tma_load_2d_pair(slot, &tmA, kc, m0, bar);
+        }
+        if constexpr (BMN) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) tma_load_2d_pair(slot + L::kABytes + j * 8192, &tmB, n0 + 64 * j, kc, bar);
+        } else {
+          tma_load_2d_pair(slot + L::kABytes, &tmB, kc, n0, bar);
+        }
+      }
+    }
+    if (*abort_flag) {
+      if (rank == 0) {
+#pragma unroll 1
+        for (int s = 0; s < STAGES; ++s) {
+          if (g - 1 < s) continue;
+          const int last = g - 1 - ((g - 1 - s) % STAGES);
+          if (p.debug_skip && last == 0) continue;
+          mbar_wait_drain_cluster(full0 + 8 * s, (last / STAGES) & 1, p.limit_ns);
+        }
+      } else {  // this CTA's loads complete on the leader's barriers
+        const uint64_t t0 = globaltimer();
+        while (globaltimer() - t0 < 200000) __nanosleep(1000);
+      }
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---------------- pair MMA issuer (leader CTA) ----------------
+    bool ok = true;
+    const uint64_t a_d0 = AMN ? MN::desc(sbase, 0, false) : smem_desc(sbase, 16, 1024, 2);
+    const uint64_t b_d0 = BMN ? MN::desc(sbase + L::kABytes, 0, false) : smem_desc(sbase + L::kABytes, 16, 1024, 2);
+    constexpr uint32_t kAStep = AMN ? MN::step(false) >> 4 : 2u, kBStep = BMN ? MN::step(false) >> 4 : 2u;
+    int s = 0;
+    uint32_t phase = 0, bar = full0;
+    uint64_t so = 0;
+    for (int i = 0; i < my_tiles && ok; ++i) {
+      const int b = i & 1;
+      const uint32_t acc = tmem + 256u * b;
+      if (i >= 2 && !mbar_wait_cluster(acce0 + 8 * b, ((i >> 1) - 1) & 1, wc)) break;
+      tc_fence_after();
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (!mbar_wait_cluster(bar, phase, wc)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t ad = a_d0 + so, bd = b_d0 + so;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          if constexpr (F8) mma_ss_pair_f8(acc, ad + ks * kAStep, bd + ks * kBStep, kIdesc, (kb | ks) ? 1u : 0u);
+          else mma_ss_pair<false>(acc, ad + ks * kAStep, bd + ks * kBStep, kIdesc, (kb | ks) ? 1u : 0u);
+        }
+        mma_commit_pair(bar + 8 * STAGES, 0x3);
+        if (++s == STAGES) {
+          s = 0;
+          phase ^= 1u;
+          bar = full0;
+          so = 0;
+        } else {
+          bar += 8;
+          so += L::kStageBytes >> 4;
+        }
+      }
+      if (!ok) break;
+      mma_commit_pair(accf0 + 8 * b, 0x3);
+    }
+    if (*abort_flag) {
+      mma_commit_pair(drainf, 0x1);
+      mbar_wait_drain_cluster(drainf, 0, p.limit_ns);
+    }
+  } else if (warp >= 4) {
+    // ---------------- epilogue (both CTAs): group g = warps 4 + 4 g .. 7 + 4 g ----------------
+    const int g = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
+    const bool first = r == 0;  // the group's thread that waits and stores
+    const uint32_t bar_a = 1 + 2 * g, bar_b = 2 + 2 * g;
+    const uint32_t lead_acce0 = map_to_cta(acce0, 0);
+    uint8_t *box = smem + L::kBoxOff + g * L::kBoxBytes;
+    volatile uint32_t *go = tmem_slot + 2 + 2 * g;  // by the tile's parity: a warp may lag one tile
+    const bool bf16 = p.out_bf16 != 0, pre = p.pre != nullptr, pingpong = bf16 && !pre;
+    uint32_t turn = 0;
+    grid_dependency_wait();
+#pragma unroll 1
+    for (int i = 0; i < my_tiles; ++i) {
+      const int b = i & 1;
+      int tm, tn;
+      raster_tile(pair + i * npairs, tiles_m, tiles_n, kRasterGroup, tm, tn);
+      const int m0 = tm * 256 + (int)rank * 128, n0 = tn * 256;
+      const int64_t row = m0 + r;
+      const bool row_ok = row < p.M;
+      const float sa = p.a_scale && row_ok ? __ldg(p.a_scale + row) : 1.f;
+      // One thread waits (bounded) and publishes the outcome: the group's four warps take the same
+      // branch, and no named barrier below waits for a warp that gave up.
+      if (first) go[b] = mbar_wait_cluster(accf0 + 8 * b, (i >> 1) & 1, wc, 128) ? 1u : 0u;
+      named_barrier(bar_a, 128);
+      if (!go[b]) break;
+      tc_fence_after();
+      const uint32_t tacc = tmem + 256u * b + ((uint32_t)(q * 32) << 16);
+#pragma unroll 1
+      for (int c = g; c < 8; c += 2) {
+        const int col0 = n0 + c * 32;
+        if (m0 >= p.M || col0 >= p.N) break;  // the same for the whole group
+        uint32_t rr[32];
+        tmem_ld_32x32b_x32(tacc + c * 32, rr);
+        const bool lane_col = col0 + lane < p.N;
+        const float bl = p.bias && lane_col ? __ldg(p.bias + col0 + lane) : 0.f;
+        const float sl = p.b_scale && lane_col ? __ldg(p.b_scale + col0 + lane) : 1.f;
+        float res[32];
+        if (p.residual && p.tma_out && row_ok) {
+          load_residual(p, row, col0, res);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) res[j] = 0.f;
+        }
+        tmem_ld_wait(rr);
+        float v[32];
+        if constexpr (F8) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            v[j] = __uint_as_float(rr[j]) * sa * __shfl_sync(0xFFFFFFFFu, sl, j) + __shfl_sync(0xFFFFFFFFu, bl, j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rr[j]) + __shfl_sync(0xFFFFFFFFu, bl, j);
+        }
+        if (!p.tma_out) {
+          float *buf = reinterpret_cast<float *>(box) + q * 1024;
+          const int64_t row0 = m0 + q * 32;
+          if (pre) store_turned(p, buf, lane, row0, col0, p.pre, p.ldp, false, v);
+          with_activation(p.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = activate<decltype(act)::value>(v[j]);
+          });
+          store_turned(p, buf, lane, row0, col0, p.out, p.ldo, p.residual != nullptr, v);
+          continue;
+        }
+        // The boxes are free once the stores issued from them have read them: all but the last one
+        // when the bf16 box has two halves to alternate between.
+        if (first) {
+          if (pingpong) bulk_wait_group_read1();
+          else bulk_wait_group_read0();
+        }
+        named_barrier(bar_a, 128);
+        uint8_t *obox = pingpong ? box + (turn & 1) * 8192 : (bf16 && pre ? box + 8192 : box);
+        ++turn;
+        if (pre) {
+          stage_row(box, r, bf16, v);
+          if (!bf16) {  // f32: the box holds one tile at a time
+            fence_proxy_async_smem();
+            named_barrier(bar_b, 128);
+            if (first) {
+              tma_store_2d(&tmP, smem_u32(box), col0, m0);
+              bulk_commit_group();
+              bulk_wait_group_read0();
+            }
+            named_barrier(bar_a, 128);
+          }
+        }
+        with_activation(p.act, [&](auto act) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = activate<decltype(act)::value>(v[j]);
+        });
+        if (p.residual) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += res[j];
+        }
+        stage_row(obox, r, bf16, v);
+        fence_proxy_async_smem();
+        named_barrier(bar_b, 128);
+        if (first) {
+          if (pre && bf16) tma_store_2d(&tmP, smem_u32(box), col0, m0);
+          tma_store_2d(&tmO, smem_u32(obox), col0, m0);
+          bulk_commit_group();
+        }
+      }
+      // Every tcgen05.ld of accumulator b has completed (tmem_ld_wait): release it.
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(lead_acce0 + 8 * b);
+    }
+    if (first) bulk_wait_group_read0();  // staging stays valid until read
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while the pair MMA may still read its memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// Co-resident clusters of one instantiation on the current device (0 on failure).
+template <bool F8, bool AMN, bool BMN>
+int pair_clusters() {
+  auto kern = linear_pair_kernel<F8, AMN, BMN>;
+  static int cached[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  int *slot = &cached[dev & 63];
+  int v = __atomic_load_n(slot, __ATOMIC_ACQUIRE);
+  if (v > 0) return v;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PairL::kSmemBytes) != cudaSuccess) return 0;
+  int sms = 0;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (sms / 2 > 0 ? sms / 2 : 1), 1, 1);
+  cfg.blockDim = dim3(PairL::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = PairL::kSmemBytes;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return 0;
+  }
+  __atomic_store_n(slot, n, __ATOMIC_RELEASE);
+  return n;
+}
+
+template <bool F8, bool AMN, bool BMN>
+cudaError_t launch_pair(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmO, const CUtensorMap &tmP,
+                        const LinearParams &p, cudaStream_t st) {
+  const int clusters = pair_clusters<F8, AMN, BMN>();
+  if (clusters <= 0) return cudaErrorInvalidConfiguration;
+  const int64_t tiles = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
+  if (tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
+  const int pairs = tiles < clusters ? (int)tiles : clusters;
+  linear_pair_kernel<F8, AMN, BMN><<<2 * pairs, PairL::kThreads, PairL::kSmemBytes, st>>>(tmA, tmB, tmO, tmP, p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_linear_pair(bool f8, bool a_mn, bool b_mn, const CUtensorMap &tmA, const CUtensorMap &tmB,
+                               const CUtensorMap &tmO, const CUtensorMap &tmP, const LinearParams &p, cudaStream_t st) {
+  if (p.K <= 0 || (f8 && (a_mn || b_mn)) || (a_mn && !b_mn)) return cudaErrorInvalidValue;
+  if (f8) return launch_pair<true, false, false>(tmA, tmB, tmO, tmP, p, st);
+  if (a_mn) return launch_pair<false, true, true>(tmA, tmB, tmO, tmP, p, st);
+  return b_mn ? launch_pair<false, false, true>(tmA, tmB, tmO, tmP, p, st)
+              : launch_pair<false, false, false>(tmA, tmB, tmO, tmP, p, st);
+}
+
+}  // namespace tf

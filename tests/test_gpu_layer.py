@@ -230,6 +230,34 @@ def test_linear_one_cta_kernel(tile, splits, dtype, trans_b):
     Linear(9, 140, 70, dtype, "gelu", residual=torch.float32, out=torch.float32, trans_b=trans_b).call().check()
 
 
+@pytest.mark.parametrize("dtype,trans_b", [(torch.bfloat16, True), (torch.bfloat16, False), (torch.float8_e4m3fn, True)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pre", [True, False])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (16, 0), (3, 1)])
+def test_linear_pair_kernel(dtype, trans_b, out, pre, pad, shift):
+    """The 256 x 256 kernel, with tiles that end inside the matrix and fewer stages of k than its ring."""
+    _lib.check(_lib.lib().tforge_debug_linear_kernel(2, 0, 0))
+    Linear(300, 520, 200, dtype, "gelu", residual=out, out=out, pre=pre, trans_b=trans_b, pad=pad, shift=shift).call().check()
+    Linear(5, 40, 1000, dtype, "silu", out=out, pre=pre, trans_b=trans_b, pad=pad, shift=shift).call().check()
+
+
+@pytest.mark.parametrize("dtype,trans_b", [(torch.bfloat16, False), (torch.float8_e4m3fn, True)])
+def test_linear_pair_kernel_walks_tiles(dtype, trans_b):
+    """More tiles than CTA pairs: both accumulators in turn, the ring across tiles."""
+    _lib.check(_lib.lib().tforge_debug_linear_kernel(2, 0, 0))
+    c = Linear(2570, 5200, 136, dtype, "relu", residual=torch.bfloat16, trans_b=trans_b).call()
+    c.check()
+    first = c.out.clone()
+    assert torch.equal(c.call().out, first)
+
+
+@pytest.mark.parametrize("trans_b", [True, False])
+def test_linear_backward_pair_kernel(trans_b):
+    _lib.check(_lib.lib().tforge_debug_linear_kernel(2, 0, 0))
+    check_linear_backward(300, 520, 264, trans_b=trans_b)
+    check_linear_backward(77, 131, 65, trans_b=trans_b, grad=torch.float32)
+
+
 def test_linear_infinities_and_nan():
     """An infinite operand reaches its row as the formula says; the other rows do not see it."""
     c = Linear(20, 96, 64, act="relu", out=torch.float32)
