@@ -64,10 +64,20 @@ struct TcParams {
   int32_t pdl;
 };
 
-// Launch attribute of a programmatic dependent launch (TcParams::pdl).
+// Launch attribute of a programmatic dependent launch (TcParams::pdl; every launch of the
+// transformer-layer kernels, which touch global memory only after griddepcontrol.wait).
 inline void pdl_attr(cudaLaunchAttribute &a) {
   a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   a.val.programmaticStreamSerializationAllowed = 1;
+}
+
+// Launches `kern` as a programmatic dependent of the kernel before it on the stream.
+template <typename... P, typename... A>
+inline cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, dim3 block, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute attr[1];
+  pdl_attr(attr[0]);
+  cudaLaunchConfig_t cfg = {grid, block, 0, stream, attr, 1};
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
 }
 
 struct TcConfig {
@@ -191,9 +201,9 @@ struct LinearParams {
   uint64_t limit_ns;              // bounded-wait limit
   int32_t debug_skip;             // test hook: skip the first stage's loads
   int32_t splits;                 // slim kernel: CTAs that share a tile's k (1, 2, 4 or 8)
-  // Pair kernel: out, pre and the residual start their rows on 16-byte boundaries, so that TMA
-  // stores the tiles (and tmO, tmP are set) and the residual is read 16 bytes at a time.
-  int32_t tma_out;
+  // Every array of the epilogue that is there starts its rows on 16-byte boundaries: the pair kernel
+  // then stores tiles by TMA (tmO, tmP), the slim kernel eight columns at a time.
+  int32_t vec;
 };
 // One-CTA kernel of 128 columns x bt tokens (16, 32, 64, 128, 256; from 64 with t_mn).  tmT: A as
 // {128 B of k x bt rows} boxes, or with t_mn (A stored k x m) {64 columns x 64 rows}; tmW: B stored
@@ -202,7 +212,7 @@ cudaError_t launch_linear_slim(bool f8, bool w_mn, bool t_mn, int bt, const CUte
                                const LinearParams &p, cudaStream_t stream);
 
 // Persistent CTA pairs on 256 x 256 tiles, K > 0.  tmA / tmB: as tmT / tmW above with 128 rows a
-// box.  tmO / tmP: maps of out and pre (encode_out_map), read when p.tma_out.
+// box.  tmO / tmP: maps of out and pre (encode_out_map), read when p.vec.
 cudaError_t launch_linear_pair(bool f8, bool a_mn, bool b_mn, const CUtensorMap &tmA, const CUtensorMap &tmB,
                                const CUtensorMap &tmO, const CUtensorMap &tmP, const LinearParams &p, cudaStream_t stream);
 // Output map: boxes of 32 columns x 128 rows, f32 in the 128-byte or bf16 in the 64-byte swizzle.

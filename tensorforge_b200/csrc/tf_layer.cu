@@ -105,6 +105,8 @@ __device__ __forceinline__ D convert(S v) {
 template <typename S, typename D>
 __global__ void __launch_bounds__(256) copy_rows_kernel(const S *__restrict__ src, int64_t lds, D *__restrict__ dst,
                                                         int64_t ldd, int64_t rows, int64_t cols) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int64_t groups = (cols + 7) / 8, total = rows * groups;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / groups, c = (i - r * groups) * 8;
@@ -135,14 +137,17 @@ int prepare_operand(Operand &o, int dtype, Scratch &scratch, cudaStream_t st) {
   if (rc) return rc;
   int64_t blocks = (o.rows * ((o.cols + 7) / 8) + 255) / 256;
   if (blocks > 148 * 16) blocks = 148 * 16;
-  const unsigned g = (unsigned)blocks;
+  const dim3 g((unsigned)blocks), b(256);
+  cudaError_t e;
   if (dtype == TFORGE_F32)
-    copy_rows_kernel<<<g, 256, 0, st>>>(static_cast<const float *>(o.p), o.ld, static_cast<__nv_bfloat16 *>(q), ldd, o.rows, o.cols);
+    e = launch_dependent(copy_rows_kernel<float, __nv_bfloat16>, g, b, st, static_cast<const float *>(o.p), o.ld,
+                         static_cast<__nv_bfloat16 *>(q), ldd, o.rows, o.cols);
   else if (dtype == TFORGE_BF16)
-    copy_rows_kernel<<<g, 256, 0, st>>>(static_cast<const uint16_t *>(o.p), o.ld, static_cast<uint16_t *>(q), ldd, o.rows, o.cols);
+    e = launch_dependent(copy_rows_kernel<uint16_t, uint16_t>, g, b, st, static_cast<const uint16_t *>(o.p), o.ld,
+                         static_cast<uint16_t *>(q), ldd, o.rows, o.cols);
   else
-    copy_rows_kernel<<<g, 256, 0, st>>>(static_cast<const uint8_t *>(o.p), o.ld, static_cast<uint8_t *>(q), ldd, o.rows, o.cols);
-  cudaError_t e = cudaGetLastError();
+    e = launch_dependent(copy_rows_kernel<uint8_t, uint8_t>, g, b, st, static_cast<const uint8_t *>(o.p), o.ld,
+                         static_cast<uint8_t *>(q), ldd, o.rows, o.cols);
   if (e != cudaSuccess) return cuda_failure(e, "operand copy");
   o.p = q;
   o.ld = ldd;
@@ -181,21 +186,21 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
   if (rc) return rc;
   p.limit_ns = wait_limit_ns();
   p.debug_skip = debug_skip_load();
+  auto rows16 = [](const void *q, int64_t ld, int e) { return !q || (at(q, 16) && ld * e % 16 == 0); };
+  const int eo = p.out_bf16 ? 2 : 4;
+  p.vec = rows16(p.out, p.ldo, eo) && rows16(p.pre, p.ldp, eo) && rows16(p.residual, p.ldr, p.res_bf16 ? 2 : 4) &&
+          at(p.bias, 16) && at(p.b_scale, 16);
   Choice c = choose_slim(M, N, K, t_mn, esz);
   const uint32_t force = g_force.load();
   const bool pair = (force & 255) == 2;
   if (pair) {
     if (K == 0) return TFORGE_ERR_UNSUPPORTED;
-    auto rows16 = [](const void *q, int64_t ld, int e) { return at(q, 16) && ld * e % 16 == 0; };
-    const int eo = p.out_bf16 ? 2 : 4;
-    p.tma_out = rows16(p.out, p.ldo, eo) && (!p.pre || rows16(p.pre, p.ldp, eo)) &&
-                (!p.residual || rows16(p.residual, p.ldr, p.res_bf16 ? 2 : 4));
     CUtensorMap tmA{}, tmB{}, tmO{}, tmP{};
     const uint32_t bk = 128 / esz;
     rc = t_mn ? encode_rows_map(&tmA, rows.p, esz, K, M, rows.ld, 64, 64) : encode_rows_map(&tmA, rows.p, esz, M, K, rows.ld, bk, 128);
     if (!rc) rc = w_mn ? encode_rows_map(&tmB, cols.p, esz, K, N, cols.ld, 64, 64) : encode_rows_map(&tmB, cols.p, esz, N, K, cols.ld, bk, 128);
-    if (!rc && p.tma_out) rc = encode_out_map(&tmO, p.out, p.out_bf16 != 0, M, N, p.ldo);
-    if (!rc && p.tma_out && p.pre) rc = encode_out_map(&tmP, p.pre, p.out_bf16 != 0, M, N, p.ldp);
+    if (!rc && p.vec) rc = encode_out_map(&tmO, p.out, p.out_bf16 != 0, M, N, p.ldo);
+    if (!rc && p.vec && p.pre) rc = encode_out_map(&tmP, p.pre, p.out_bf16 != 0, M, N, p.ldp);
     if (rc) return rc;
     cudaError_t e = launch_linear_pair(f8, t_mn, w_mn, tmA, tmB, tmO, tmP, p, st);
     return e == cudaSuccess ? TFORGE_OK : cuda_failure(e, "linear launch");
@@ -230,6 +235,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     activation_grad_kernel(int act, const T *__restrict__ dout, int64_t lddo, const T *__restrict__ pre, int64_t ldp,
                            __nv_bfloat16 *__restrict__ dz, int64_t ldz, float *__restrict__ part, int64_t M, int64_t N) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   __shared__ float sm[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c0 = (int64_t)blockIdx.x * 256;
@@ -310,9 +317,8 @@ cudaError_t launch_activation_grad(int act, const void *dout, int64_t lddo, cons
                    (act == TFORGE_ACT_NONE || (at(pre, 16) && ldp * e % 16 == 0));
   const dim3 g((unsigned)((N + 255) / 256), (unsigned)row_blocks);
   auto kern = vec ? activation_grad_kernel<T, true> : activation_grad_kernel<T, false>;
-  kern<<<g, 256, 0, st>>>(act, static_cast<const T *>(dout), lddo, static_cast<const T *>(pre), ldp,
+  return launch_dependent(kern, g, dim3(256), st, act, static_cast<const T *>(dout), lddo, static_cast<const T *>(pre), ldp,
                           static_cast<__nv_bfloat16 *>(dz), ldz, part, M, N);
-  return cudaGetLastError();
 }
 
 // Row blocks: about eight blocks an SM in all, each of at least 32 rows.

@@ -170,7 +170,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
-    if (p.tma_out) tma_prefetch_desc(&tmO);
+    if (p.vec) tma_prefetch_desc(&tmO);
   }
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(tmem_slot), 512);
@@ -182,9 +182,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // Nothing of global memory is read or written, and no bounded wait begins, before this.
+  grid_dependency_wait();
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer (both CTAs) ----------------
-    grid_dependency_wait();
+    grid_launch_dependents();
     const uint32_t lead_full0 = map_to_cta(full0, 0);
     int g = 0;  // k-blocks issued so far
     bool ok = true;
@@ -284,7 +286,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
     volatile uint32_t *go = tmem_slot + 2 + 2 * g;  // by the tile's parity: a warp may lag one tile
     const bool bf16 = p.out_bf16 != 0, pre = p.pre != nullptr, pingpong = bf16 && !pre;
     uint32_t turn = 0;
-    grid_dependency_wait();
 #pragma unroll 1
     for (int i = 0; i < my_tiles; ++i) {
       const int b = i & 1;
@@ -311,7 +312,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
         const float bl = p.bias && lane_col ? __ldg(p.bias + col0 + lane) : 0.f;
         const float sl = p.b_scale && lane_col ? __ldg(p.b_scale + col0 + lane) : 1.f;
         float res[32];
-        if (p.residual && p.tma_out && row_ok) {
+        if (p.residual && p.vec && row_ok) {
           load_residual(p, row, col0, res);
         } else {
 #pragma unroll
@@ -327,7 +328,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rr[j]) + __shfl_sync(0xFFFFFFFFu, bl, j);
         }
-        if (!p.tma_out) {
+        if (!p.vec) {
           float *buf = reinterpret_cast<float *>(box) + q * 1024;
           const int64_t row0 = m0 + q * 32;
           if (pre) store_turned(p, buf, lane, row0, col0, p.pre, p.ldp, false, v);
@@ -434,8 +435,10 @@ cudaError_t launch_pair(const CUtensorMap &tmA, const CUtensorMap &tmB, const CU
   const int64_t tiles = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
   if (tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
   const int pairs = tiles < clusters ? (int)tiles : clusters;
-  linear_pair_kernel<F8, AMN, BMN><<<2 * pairs, PairL::kThreads, PairL::kSmemBytes, st>>>(tmA, tmB, tmO, tmP, p);
-  return cudaGetLastError();
+  cudaLaunchAttribute attr[1];
+  pdl_attr(attr[0]);
+  cudaLaunchConfig_t cfg = {dim3(2 * pairs), dim3(PairL::kThreads), (size_t)PairL::kSmemBytes, st, attr, 1};
+  return cudaLaunchKernelEx(&cfg, linear_pair_kernel<F8, AMN, BMN>, tmA, tmB, tmO, tmP, p);
 }
 
 }  // namespace

@@ -6,17 +6,17 @@
 //
 // Operands are bf16 or e4m3, 128 bytes of k a stage, each K-major or (bf16) MN-major as it lies in
 // memory, brought by TMA into a ring of 128-B-swizzled tiles; one thread issues the MMAs; the
-// accumulator is BT columns of tensor memory.  With few tiles a cluster of S CTAs shares a tile:
-// CTA z takes the z-th part of k, leaves its f32 sums in its shared memory, and after a cluster
-// barrier each CTA adds 1/S of the tile's values from all S, in order of z (the same bits every
-// time), and finishes them.
+// accumulator is BT columns of tensor memory.  With few tiles a cluster of S CTAs shares a tile,
+// CTA z taking the z-th part of k.
 //
-// The output tile is transposed in tensor memory (lane = column n), so a warp's 32 lanes hold 32
-// neighbouring columns of one token: residual reads and output writes are coalesced at any
-// alignment and pitch, without staging.
+// Epilogue: the tile is transposed in tensor memory (lane = column n), so it is first left in the
+// ring's shared memory as f32, token by token; after a barrier (of the cluster, if it shares the
+// tile) each CTA takes 1/S of the tile's values in groups of eight neighbouring columns of a token,
+// adds the S CTAs' sums in order of z (the same bits every time) and finishes them: 16-byte
+// accesses where the caller's rows allow, single elements elsewhere.
 //
-// 256 threads: warp 0 TMA producer, warp 1 MMA issuer, then all eight warps the epilogue (two per
-// 32-lane quadrant, taking token chunks in turn).  Every wait is bounded (tf_ptx.cuh).
+// 256 threads: warp 0 TMA producer, warp 1 MMA issuer, then all eight warps the epilogue.  Every
+// wait is bounded (tf_ptx.cuh), and none begins before the kernel that this launch follows is done.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -47,31 +47,73 @@ __device__ __forceinline__ float residual_at(const LinearParams &p, int64_t i) {
   return p.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.residual)[i])
                     : static_cast<const float *>(p.residual)[i];
 }
-__device__ __forceinline__ void put(void *base, int bf16, int64_t i, float v) {
-  if (bf16) static_cast<__nv_bfloat16 *>(base)[i] = __float2bfloat16_rn(v);
-  else static_cast<float *>(base)[i] = v;
+// Eight f32 at a 16-byte boundary.
+__device__ __forceinline__ void read8(const float *src, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4 *>(src)[0], b = reinterpret_cast<const float4 *>(src)[1];
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+// Columns n .. n + 7 of an output row, those below N.
+__device__ __forceinline__ void put8(void *base, bool bf16, bool vec, int64_t i, int live, const float (&v)[8]) {
+  if (bf16) {
+    __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(base) + i;
+    if (vec) {
+      *reinterpret_cast<uint4 *>(o) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                 pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < live) o[j] = __float2bfloat16_rn(v[j]);
+    }
+  } else {
+    float *o = static_cast<float *>(base) + i;
+    if (vec) {
+      reinterpret_cast<float4 *>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4 *>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < live) o[j] = v[j];
+    }
+  }
 }
 
-// Finishes CNT tokens j = j0 .. j0 + CNT - 1 of column n (bias and b_scale: bn, sn).
-template <int CNT>
-__device__ __forceinline__ void finish_column(const LinearParams &p, float (&v)[CNT], int64_t m0, int64_t n, float bn,
-                                              float sn) {
-  float res[CNT];
+// Finishes the accumulated sums v of token m, columns n .. n + 7 (`live` of them below N).  vec: every
+// array of the epilogue has these eight on a 16-byte boundary.
+__device__ __forceinline__ void finish8(const LinearParams &p, float (&v)[8], int64_t m, int n, int live, bool vec,
+                                        const float (&res)[8]) {
+  float c[8];
+  if (p.a_scale) {
+    const float sa = __ldg(p.a_scale + m);
+    if (vec) {
+      read8(p.b_scale + n, c);
+    } else {
 #pragma unroll
-  for (int j = 0; j < CNT; ++j) res[j] = p.residual && m0 + j < p.M ? residual_at(p, (m0 + j) * p.ldr + n) : 0.f;
+      for (int j = 0; j < 8; ++j) c[j] = j < live ? p.b_scale[n + j] : 0.f;
+    }
 #pragma unroll
-  for (int j = 0; j < CNT; ++j) {
-    if (p.a_scale && m0 + j < p.M) v[j] = v[j] * __ldg(p.a_scale + m0 + j) * sn;
-    v[j] += bn;
-    if (p.pre && m0 + j < p.M) put(p.pre, p.out_bf16, (m0 + j) * p.ldp + n, v[j]);
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * sa * c[j];
   }
+  if (p.bias) {
+    if (vec) {
+      read8(p.bias + n, c);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = j < live ? p.bias[n + j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += c[j];
+  }
+  if (p.pre) put8(p.pre, p.out_bf16, vec, m * p.ldp + n, live, v);
   with_activation(p.act, [&](auto act) {
 #pragma unroll
-    for (int j = 0; j < CNT; ++j) v[j] = activate<decltype(act)::value>(v[j]);
+    for (int j = 0; j < 8; ++j) v[j] = activate<decltype(act)::value>(v[j]);
   });
+  if (p.residual) {
 #pragma unroll
-  for (int j = 0; j < CNT; ++j)
-    if (m0 + j < p.M) put(p.out, p.out_bf16, (m0 + j) * p.ldo + n, p.residual ? v[j] + res[j] : v[j]);
+    for (int j = 0; j < 8; ++j) v[j] += res[j];
+  }
+  put8(p.out, p.out_bf16, vec, m * p.ldo + n, live, v);
 }
 
 // F8: e4m3 operands (both K-major).  WMN / TMN: the weights' / tokens' tile is MN-major (bf16).
@@ -126,8 +168,10 @@ __global__ void __launch_bounds__(256)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // Nothing of global memory is read or written, and no bounded wait begins, before this.
+  grid_dependency_wait();
   if (warp == 0 && lane == 0) {
-    grid_dependency_wait();
+    grid_launch_dependents();
     int kb = 0;
     for (; kb < nkb; ++kb) {
       const int s = kb % STAGES, round = kb / STAGES;
@@ -186,63 +230,74 @@ __global__ void __launch_bounds__(256)
   }
   __syncwarp();
 
-  // ---------------- epilogue: all warps; warp w reads TMEM lanes 32 (w % 4) .. + 31 ----------------
-  grid_dependency_wait();  // bias, scales, residual: written by the kernel before; outputs: read by it
-  const int q = warp & 3, half = warp >> 2, r = q * 32 + lane, n = n0 + r;
+  // ---------------- epilogue ----------------
+  // Warp w reads TMEM lanes 32 (w % 4) .. + 31, tokens in chunks of 16 by its half.  Value (token j,
+  // column r) goes to float j * 128 + r of the ring (every load has been consumed).
+  const int q = warp & 3, half = warp >> 2, r = q * 32 + lane;
   const bool ok = nkb == 0 || (mbar_wait(accf, 0, wc) && !*abort_flag);
   tc_fence_after();
-  const bool col_ok = n < p.N;
-  const float bn = p.bias && col_ok ? __ldg(p.bias + n) : 0.f, sn = p.b_scale && col_ok ? __ldg(p.b_scale + n) : 1.f;
+  const int tokens = p.M - m0 < BT ? p.M - m0 : BT;
+  float *part = reinterpret_cast<float *>(smem);
   const uint32_t tacc = tmem + ((uint32_t)(q * 32) << 16);
-  if (splits == 1) {
 #pragma unroll 1
-    for (int c = half; c < BT / 16; c += 2) {
-      if (m0 + 16 * c >= p.M) break;
-      uint32_t rr[16];
-      float v[16];
-      if (__all_sync(0xFFFFFFFFu, ok && nkb > 0)) {
-        tmem_ld_32x32b_x16(tacc + 16 * c, rr);
-        tmem_ld_wait(rr);
+  for (int c = half; 16 * c < tokens; c += 2) {
+    uint32_t rr[16];
+    if (__all_sync(0xFFFFFFFFu, ok && nkb > 0)) {
+      tmem_ld_32x32b_x16(tacc + 16 * c, rr);
+      tmem_ld_wait(rr);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) rr[j] = 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) part[(16 * c + j) * 128 + r] = __uint_as_float(rr[j]);
+  }
+  const bool all_ok = __syncthreads_and(ok);
+  if (splits > 1) cluster_sync();
+  // Group g of eight columns: token g / 16, columns n0 + 8 (g % 16) ..; this CTA's share of them.
+  const int groups = tokens * 16, share = (groups + splits - 1) / splits;
+  const int g1 = (z + 1) * share < groups ? (z + 1) * share : groups;
+#pragma unroll 1
+  for (int g = z * share + (int)threadIdx.x; g < g1; g += L::kThreads) {
+    const int n = n0 + 8 * (g & 15), live = p.N - n;
+    const int64_t m = m0 + (g >> 4);
+    if (live <= 0 || !all_ok) continue;
+    const bool vec = p.vec && live >= 8;
+    float res[8];
+    if (p.residual) {
+      const int64_t i = m * p.ldr + n;
+      if (vec && p.res_bf16) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.residual) + i);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          res[2 * j] = __uint_as_float(w[j] << 16);
+          res[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        }
+      } else if (vec) {
+        read8(static_cast<const float *>(p.residual) + i, res);
       } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) rr[j] = 0u;
+        for (int j = 0; j < 8; ++j) res[j] = j < live ? residual_at(p, i + j) : 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(rr[j]);
-      if (ok && col_ok) finish_column<16>(p, v, m0 + 16 * c, n, bn, sn);
     }
-  } else {
-    // Partial sums, token by token: value (j, r) at float j * 128 + r of the ring (every load has
-    // been consumed), neighbouring lanes in neighbouring banks.
-    float *part = reinterpret_cast<float *>(smem);
-#pragma unroll 1
-    for (int c = half; c < BT / 16; c += 2) {
-      if (m0 + 16 * c >= p.M) break;
-      uint32_t rr[16];
-      if (__all_sync(0xFFFFFFFFu, ok && nkb > 0)) {
-        tmem_ld_32x32b_x16(tacc + 16 * c, rr);
-        tmem_ld_wait(rr);
-      } else {
+    float v[8];
+    if (splits == 1) {
+      read8(part + 8 * g, v);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) rr[j] = 0u;
+      for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        if (s < splits) {
+          const uint32_t src = map_to_cta(sbase + 32 * g, s);
+          const float4 a = ld_cluster_f32x4(src), b = ld_cluster_f32x4(src + 16);
+          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+        }
       }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) part[(16 * c + j) * 128 + r] = __uint_as_float(rr[j]);
     }
-    cluster_sync();
-    // CTA z finishes tokens z, z + S, ... of the tile, two at a time by its thread halves.
-    const int live = p.M - m0 < BT ? p.M - m0 : BT;
-    uint32_t src[8];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) src[s] = s < splits ? map_to_cta(sbase, s) : 0u;
-#pragma unroll 1
-    for (int j = z + splits * half; j < live; j += 2 * splits) {
-      float v[1] = {0.f};
-#pragma unroll
-      for (int s = 0; s < 8; ++s)
-        if (s < splits) v[0] += ld_cluster_f32(src[s] + (j * 128 + r) * 4);
-      if (ok && col_ok) finish_column<1>(p, v, m0 + j, n, bn, sn);
-    }
+    finish8(p, v, m, n, live, vec, res);
   }
   tc_fence_before();
   __syncthreads();
@@ -268,16 +323,19 @@ cudaError_t launch_slim_kern(const CUtensorMap &tmT, const CUtensorMap &tmW, con
   }
   const int64_t tiles = (int64_t)((p.M + BT - 1) / BT) * ((p.N + 127) / 128);
   if (tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = (unsigned)p.splits;
-  cudaLaunchConfig_t cfg = {dim3((unsigned)tiles, 1, (unsigned)p.splits), dim3(L::kThreads), (size_t)L::kSmemBytes, st, attr, 1};
+  cudaLaunchAttribute attr[2];
+  pdl_attr(attr[0]);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = (unsigned)p.splits;
+  cudaLaunchConfig_t cfg = {dim3((unsigned)tiles, 1, (unsigned)p.splits), dim3(L::kThreads), (size_t)L::kSmemBytes, st, attr, 2};
   return cudaLaunchKernelEx(&cfg, kern, tmT, tmW, p);
 }
 
-// Ring depths: two CTAs an SM (about 100 KB each) up to 128 tokens, one with 256.
+// Ring depths: about 100 KB a CTA, so that two share an SM; one with 256 tokens.  (Twice the depth
+// for launches of no more CTAs than SMs measured no faster, and a cluster of eight such CTAs finds
+// fewer places: 64 x 512 x 8192 19.1 us instead of 10.9.)
 template <bool F8, bool WMN, bool TMN>
 cudaError_t launch_slim_bt(int bt, const CUtensorMap &tmT, const CUtensorMap &tmW, const LinearParams &p, cudaStream_t st) {
   if constexpr (!TMN) {
@@ -296,7 +354,8 @@ cudaError_t launch_linear_slim(bool f8, bool w_mn, bool t_mn, int bt, const CUte
                                const LinearParams &p, cudaStream_t st) {
   if (f8) return w_mn || t_mn ? cudaErrorInvalidValue : launch_slim_bt<true, false, false>(bt, tmT, tmW, p, st);
   if (t_mn) return w_mn ? launch_slim_bt<false, true, true>(bt, tmT, tmW, p, st) : cudaErrorInvalidValue;
-  return w_mn ? launch_slim_bt<false, true, false>(bt, tmT, tmW, p, st) : launch_slim_bt<false, false, false>(bt, tmT, tmW, p, st);
+  return w_mn ? launch_slim_bt<false, true, false>(bt, tmT, tmW, p, st)
+              : launch_slim_bt<false, false, false>(bt, tmT, tmW, p, st);
 }
 
 }  // namespace tf

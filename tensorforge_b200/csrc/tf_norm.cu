@@ -149,6 +149,8 @@ __device__ __forceinline__ float finish_row(const NormArgs &p, int64_t m, float 
 // else single elements, T apart.  NORM false: the quantizer (y = x).
 template <typename X, int OUT, bool VEC, int T, int E, bool NORM>
 __global__ void __launch_bounds__(T == 32 ? 256 : T) norm_row_kernel(const NormArgs p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   constexpr int kRows = T == 32 ? 8 : 1;
   __shared__ uint32_t sm[64];
   const int t = T == 32 ? (threadIdx.x & 31) : threadIdx.x;
@@ -262,6 +264,8 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) norm_row_kernel(const NormA
 // The first pass only reads (sum_out may be the residual's or x's own rows), the second writes.
 template <typename X, int OUT, bool NORM>
 __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   __shared__ uint32_t sm[64];
   const int64_t m = blockIdx.x;
   const X *x = static_cast<const X *>(p.x) + m * p.ldx;
@@ -299,6 +303,8 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs p) {
 // part: gridDim.x rows of N f32, this block's column sums (null: no dweight).
 template <typename X, bool VEC, int T, int E>
 __global__ void __launch_bounds__(T == 32 ? 256 : T) norm_bwd_kernel(const NormBwdArgs p, float *__restrict__ part) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   constexpr int kRows = T == 32 ? 8 : 1;
   __shared__ uint32_t sm[2][64];
   __shared__ float comb[kRows > 1 ? kRows * T * E : 1];
@@ -403,6 +409,8 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) norm_bwd_kernel(const NormB
 // row of `part`, each element read and written by one thread.
 template <typename X>
 __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwdArgs p, float *__restrict__ part) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   __shared__ uint32_t sm[2][64];
   NormArgs wa{};
   wa.weight = p.weight;
@@ -436,6 +444,8 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwdArgs p
 // threads share a column's rows.
 __global__ void __launch_bounds__(1024) column_sum_kernel(const float *__restrict__ part, int rows, int64_t N,
                                                           float *__restrict__ out) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   __shared__ float sm[32][33];
   const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
   float v = 0.f;
@@ -457,14 +467,13 @@ bool at16(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 template <typename X, int OUT, bool VEC, bool NORM>
 cudaError_t launch_norm_rows(const NormArgs &p, cudaStream_t st) {
   const unsigned g = (unsigned)p.M;
-  if (p.N <= 256) norm_row_kernel<X, OUT, VEC, 32, 8, NORM><<<(unsigned)((p.M + 7) / 8), 256, 0, st>>>(p);
-  else if (p.N <= 1024) norm_row_kernel<X, OUT, VEC, 128, 8, NORM><<<g, 128, 0, st>>>(p);
-  else if (p.N <= 2048) norm_row_kernel<X, OUT, VEC, 256, 8, NORM><<<g, 256, 0, st>>>(p);
-  else if (p.N <= 4096) norm_row_kernel<X, OUT, VEC, 256, 16, NORM><<<g, 256, 0, st>>>(p);
-  else if (p.N <= 8192) norm_row_kernel<X, OUT, VEC, 512, 16, NORM><<<g, 512, 0, st>>>(p);
-  else if (p.N <= 16384) norm_row_kernel<X, OUT, VEC, 1024, 16, NORM><<<g, 1024, 0, st>>>(p);
-  else norm_long_kernel<X, OUT, NORM><<<g, 1024, 0, st>>>(p);
-  return cudaGetLastError();
+  if (p.N <= 256) return launch_dependent(norm_row_kernel<X, OUT, VEC, 32, 8, NORM>, dim3((unsigned)((p.M + 7) / 8)), dim3(256), st, p);
+  if (p.N <= 1024) return launch_dependent(norm_row_kernel<X, OUT, VEC, 128, 8, NORM>, dim3(g), dim3(128), st, p);
+  if (p.N <= 2048) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 8, NORM>, dim3(g), dim3(256), st, p);
+  if (p.N <= 4096) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 16, NORM>, dim3(g), dim3(256), st, p);
+  if (p.N <= 8192) return launch_dependent(norm_row_kernel<X, OUT, VEC, 512, 16, NORM>, dim3(g), dim3(512), st, p);
+  if (p.N <= 16384) return launch_dependent(norm_row_kernel<X, OUT, VEC, 1024, 16, NORM>, dim3(g), dim3(1024), st, p);
+  return launch_dependent(norm_long_kernel<X, OUT, NORM>, dim3(g), dim3(1024), st, p);
 }
 
 template <typename X, int OUT, bool NORM>
@@ -479,14 +488,13 @@ cudaError_t launch_norm_vec(const NormArgs &p, cudaStream_t st) {
 
 template <typename X, bool VEC>
 cudaError_t launch_bwd_rows(const NormBwdArgs &p, float *part, int grid, cudaStream_t st) {
-  if (p.N <= 256) norm_bwd_kernel<X, VEC, 32, 8><<<grid, 256, 0, st>>>(p, part);
-  else if (p.N <= 1024) norm_bwd_kernel<X, VEC, 128, 8><<<grid, 128, 0, st>>>(p, part);
-  else if (p.N <= 2048) norm_bwd_kernel<X, VEC, 256, 8><<<grid, 256, 0, st>>>(p, part);
-  else if (p.N <= 4096) norm_bwd_kernel<X, VEC, 256, 16><<<grid, 256, 0, st>>>(p, part);
-  else if (p.N <= 8192) norm_bwd_kernel<X, VEC, 512, 16><<<grid, 512, 0, st>>>(p, part);
-  else if (p.N <= 16384) norm_bwd_kernel<X, VEC, 1024, 16><<<grid, 1024, 0, st>>>(p, part);
-  else norm_bwd_long_kernel<X><<<grid, 1024, 0, st>>>(p, part);
-  return cudaGetLastError();
+  if (p.N <= 256) return launch_dependent(norm_bwd_kernel<X, VEC, 32, 8>, dim3(grid), dim3(256), st, p, part);
+  if (p.N <= 1024) return launch_dependent(norm_bwd_kernel<X, VEC, 128, 8>, dim3(grid), dim3(128), st, p, part);
+  if (p.N <= 2048) return launch_dependent(norm_bwd_kernel<X, VEC, 256, 8>, dim3(grid), dim3(256), st, p, part);
+  if (p.N <= 4096) return launch_dependent(norm_bwd_kernel<X, VEC, 256, 16>, dim3(grid), dim3(256), st, p, part);
+  if (p.N <= 8192) return launch_dependent(norm_bwd_kernel<X, VEC, 512, 16>, dim3(grid), dim3(512), st, p, part);
+  if (p.N <= 16384) return launch_dependent(norm_bwd_kernel<X, VEC, 1024, 16>, dim3(grid), dim3(1024), st, p, part);
+  return launch_dependent(norm_bwd_long_kernel<X>, dim3(grid), dim3(1024), st, p, part);
 }
 
 }  // namespace
@@ -522,8 +530,7 @@ cudaError_t launch_rms_norm_bwd(const NormBwdArgs &p, float *part, int grid, cud
 }
 
 cudaError_t launch_column_sum(const float *part, int rows, int64_t N, float *out, cudaStream_t st) {
-  column_sum_kernel<<<(unsigned)((N + 31) / 32), dim3(32, 32), 0, st>>>(part, rows, N, out);
-  return cudaGetLastError();
+  return launch_dependent(column_sum_kernel, dim3((unsigned)((N + 31) / 32)), dim3(32, 32), st, part, rows, N, out);
 }
 
 }  // namespace tf
