@@ -156,21 +156,45 @@ int prepare_operand(Operand &o, int dtype, Scratch &scratch, cudaStream_t st) {
 
 // ---- the products ---------------------------------------------------------------------------------
 
+// The kernel of a product: tile 0 = CTA pairs on 256 x 256 tiles, else the slim kernel's tile rows
+// and the CTAs that share a tile.
 struct Choice {
-  int tile;    // slim kernel: rows per tile
+  int tile;
   int splits;
 };
 
-// Slim kernel: the narrowest tile that holds all rows (an MN-major row operand comes in blocks of
-// 64), then as many CTAs per tile as the SMs hold at once -- two an SM, one of the widest tile --
-// with at least four stages of k each.
-Choice choose_slim(int64_t M, int64_t N, int64_t K, bool t_mn, int esz) {
-  Choice c{t_mn ? 64 : 16, 1};
-  while (c.tile < 256 && c.tile < M) c.tile *= 2;
-  const int64_t tiles = ((M + c.tile - 1) / c.tile) * ((N + 127) / 128);
-  const int64_t slots = c.tile == 256 ? 148 : 296, nkb = (K * esz + 127) / 128;
-  while (c.splits < 8 && tiles * c.splits * 2 <= slots && nkb / (c.splits * 2) >= 4) c.splits *= 2;
-  return c;
+// Least estimated time in us over the pair kernel and the slim kernel's tiles and splits.  The
+// estimates are fits to a sweep of 162 problems (M 1 .. 4096, nine N x K from 128 x 2048 to
+// 16384 x 4096, bf16 and e4m3) by every kernel: the choice is 2.5 % slower than the fastest on
+// average, and at worst 35 % (1024 x 512 x 8192: 27.3 us against 20.2).
+//   memory: operands and output once at the measured copy rate.
+//   pair:   waves of 74 pairs, each 0.367 us a stage of k (at least 7: an epilogue), or 1.68 x memory.
+//   slim:   a stage of k costs a CTA 0.246 us and 0.0005 per row of its tile, two CTAs an SM each
+//           0.65 of that (one with 256 rows); smoothly no less than 1.24 x memory; and per round of
+//           resident CTAs 2.7 us, the epilogue's rows, and what a cluster of S costs to meet.
+Choice choose(int64_t M, int64_t N, int64_t K, bool t_mn, int esz) {
+  const double nkb = (double)((K * esz + 127) / 128);
+  const double memory = ((double)esz * K * (M + N) + 2.0 * M * N) / 6.55e6;
+  const double waves = std::ceil(std::ceil(M / 256.0) * std::ceil(N / 256.0) / 74.0);
+  Choice best{0, 1};
+  double least = 4.28 + std::fmax(waves * std::fmax(0.367 * nkb, 7.0), 1.68 * memory);
+  if (K == 0) least = 1e300;  // the pair kernel needs a k
+  for (int tile = t_mn ? 64 : 16; tile <= 256; tile *= 2) {
+    const double tiles = std::ceil((double)M / tile) * std::ceil(N / 128.0), live = M < tile ? (double)M : tile;
+    for (int s = 1; s <= 8; s *= 2) {
+      const double ctas = tiles * s, deep = std::ceil(ctas / 148.0);
+      const double load = (deep == 1 || tile == 256 ? deep : 0.65 * deep) * std::ceil(nkb / s) * (0.246 + 0.000535 * tile);
+      const double l2 = load * load, m2 = 1.24 * 1.24 * memory * memory;
+      const double rounds = std::ceil(ctas / (tile == 256 ? 148.0 : 296.0));
+      const double t = std::sqrt(std::sqrt(l2 * l2 + m2 * m2)) + rounds * (2.7 + 0.0375 * live + (s > 1 ? 0.245 + 0.357 * s : 0.0));
+      if (t < least) {
+        least = t;
+        best = Choice{tile, s};
+      }
+    }
+    if (tile >= M) break;  // a wider tile would only add empty rows
+  }
+  return best;
 }
 
 // out (M x N) = epilogue(rows . cols).  rows: M x K, or K x M with t_mn; cols: N x K, or K x N
@@ -190,11 +214,12 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
   const int eo = p.out_bf16 ? 2 : 4;
   p.vec = rows16(p.out, p.ldo, eo) && rows16(p.pre, p.ldp, eo) && rows16(p.residual, p.ldr, p.res_bf16 ? 2 : 4) &&
           at(p.bias, 16) && at(p.b_scale, 16);
-  Choice c = choose_slim(M, N, K, t_mn, esz);
+  Choice c = choose(M, N, K, t_mn, esz);
   const uint32_t force = g_force.load();
-  const bool pair = (force & 255) == 2;
-  if (pair) {
-    if (K == 0) return TFORGE_ERR_UNSUPPORTED;
+  if ((force & 255) == 1) c = Choice{(int)((force >> 8) & 0xFFFF), (int)(force >> 24)};
+  else if ((force & 255) == 2) c = Choice{0, 1};
+  if ((c.tile == 0 && K == 0) || (c.tile != 0 && t_mn && c.tile < 64)) return TFORGE_ERR_UNSUPPORTED;
+  if (c.tile == 0) {
     CUtensorMap tmA{}, tmB{}, tmO{}, tmP{};
     const uint32_t bk = 128 / esz;
     rc = t_mn ? encode_rows_map(&tmA, rows.p, esz, K, M, rows.ld, 64, 64) : encode_rows_map(&tmA, rows.p, esz, M, K, rows.ld, bk, 128);
@@ -204,11 +229,6 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
     if (rc) return rc;
     cudaError_t e = launch_linear_pair(f8, t_mn, w_mn, tmA, tmB, tmO, tmP, p, st);
     return e == cudaSuccess ? TFORGE_OK : cuda_failure(e, "linear launch");
-  }
-  if ((force & 255) == 1) {
-    c.tile = (force >> 8) & 0xFFFF;
-    c.splits = (int)(force >> 24);
-    if (t_mn && c.tile < 64) return TFORGE_ERR_UNSUPPORTED;
   }
   p.splits = c.splits;
   CUtensorMap tmT{}, tmW{};
