@@ -98,29 +98,47 @@ __device__ __forceinline__ void stage_row(uint8_t *box, int r, bool bf16, const 
   }
 }
 
+// The residual of a warp's 32 rows x 32 columns, a lane a column: v[l] of row row0 + l.  One load an
+// element, any alignment, all in flight together.
+__device__ __forceinline__ void load_turned(const LinearParams &p, int lane, int64_t row0, int col0, float (&v)[32]) {
+  const int rows = col0 + lane < p.N ? (int)(p.M - row0 < 32 ? p.M - row0 : 32) : 0;
+  const int64_t i = row0 * p.ldr + col0 + lane;
+  if (p.res_bf16) {
+    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.residual) + i;
+#pragma unroll
+    for (int l = 0; l < 32; ++l) v[l] = l < rows ? __bfloat162float(src[l * p.ldr]) : 0.f;
+  } else {
+    const float *src = static_cast<const float *>(p.residual) + i;
+#pragma unroll
+    for (int l = 0; l < 32; ++l) v[l] = l < rows ? src[l * p.ldr] : 0.f;
+  }
+}
+
 // A warp's 32 rows x 32 columns turned round through its own 4 KB (column j of row l at j ^ l) and
-// stored row by row, a lane a column; `res` adds the residual.
-__device__ __forceinline__ void store_turned(const LinearParams &p, float *buf, int lane, int64_t row0, int col0, void *base,
-                                             int64_t ld, bool res, const float (&v)[32]) {
+// stored row by row, a lane a column, res[l] added to row l's.
+template <typename T>
+__device__ __forceinline__ void store_turned(float *buf, int lane, int rows, T *dst, int64_t ld, const float (&v)[32],
+                                             const float (&res)[32], bool add) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) buf[lane * 32 + (j ^ lane)] = v[j];
   __syncwarp();
-  const int rows = p.M - row0 < 32 ? (int)(p.M - row0) : 32;
-  if (col0 + lane < p.N) {
-#pragma unroll 4
-    for (int l = 0; l < rows; ++l) {
+#pragma unroll
+  for (int l = 0; l < 32; ++l) {
+    if (l < rows) {
       float x = buf[l * 32 + (lane ^ l)];
-      if (res) {
-        const int64_t i = (row0 + l) * p.ldr + col0 + lane;
-        x += p.res_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.residual)[i])
-                        : static_cast<const float *>(p.residual)[i];
-      }
-      const int64_t o = (row0 + l) * ld + col0 + lane;
-      if (p.out_bf16) static_cast<__nv_bfloat16 *>(base)[o] = __float2bfloat16_rn(x);
-      else static_cast<float *>(base)[o] = x;
+      if (add) x += res[l];
+      if constexpr (sizeof(T) == 2) dst[l * ld] = __float2bfloat16_rn(x);
+      else dst[l * ld] = x;
     }
   }
   __syncwarp();
+}
+__device__ __forceinline__ void store_turned(const LinearParams &p, float *buf, int lane, int64_t row0, int col0, void *base,
+                                             int64_t ld, const float (&v)[32], const float (&res)[32], bool add) {
+  const int rows = col0 + lane < p.N ? (int)(p.M - row0 < 32 ? p.M - row0 : 32) : 0;
+  const int64_t o = row0 * ld + col0 + lane;
+  if (p.out_bf16) store_turned(buf, lane, rows, static_cast<__nv_bfloat16 *>(base) + o, ld, v, res, add);
+  else store_turned(buf, lane, rows, static_cast<float *>(base) + o, ld, v, res, add);
 }
 
 // F8: e4m3 operands (both K-major).  AMN / BMN: A / B is MN-major (bf16).
@@ -314,6 +332,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
         float res[32];
         if (p.residual && p.vec && row_ok) {
           load_residual(p, row, col0, res);
+        } else if (p.residual && !p.vec) {
+          load_turned(p, lane, m0 + q * 32, col0, res);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) res[j] = 0.f;
@@ -331,12 +351,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
         if (!p.vec) {
           float *buf = reinterpret_cast<float *>(box) + q * 1024;
           const int64_t row0 = m0 + q * 32;
-          if (pre) store_turned(p, buf, lane, row0, col0, p.pre, p.ldp, false, v);
+          if (pre) store_turned(p, buf, lane, row0, col0, p.pre, p.ldp, v, res, false);
           with_activation(p.act, [&](auto act) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = activate<decltype(act)::value>(v[j]);
           });
-          store_turned(p, buf, lane, row0, col0, p.out, p.ldo, p.residual != nullptr, v);
+          store_turned(p, buf, lane, row0, col0, p.out, p.ldo, v, res, p.residual != nullptr);
           continue;
         }
         // The boxes are free once the stores issued from them have read them: all but the last one
