@@ -136,11 +136,21 @@ int status_word(uint32_t **out) {
   if (dev < 0 || dev >= kMaxDev) return TFORGE_ERR_UNSUPPORTED;
   std::lock_guard<std::mutex> lk(g_status_mu);
   if (!g_status[dev]) {
+    // The first call may come while a stream is being captured: allocate outside any capture
+    // (relaxed mode for this thread) and clear on a stream of its own.
     void *p = nullptr;
+    cudaStream_t own = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaThreadExchangeStreamCaptureMode");
     e = cudaMalloc(&p, 256);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMalloc(status)");
-    e = cudaMemset(p, 0, 256);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMemset(status)");
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, 256, own);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+    if (own) cudaStreamDestroy(own);
+    if (e != cudaSuccess && p) cudaFree(p);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return cuda_fail(e, "status word");
     g_status[dev] = static_cast<uint32_t *>(p);
   }
   *out = g_status[dev];

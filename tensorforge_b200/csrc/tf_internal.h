@@ -224,7 +224,7 @@ struct NormArgs {
   void *sum_out, *out;
   float *scale, *rstd;
   int64_t M, N, ldx, ldr, lds, ldo;
-  float eps;
+  float eps, inv_n;  // inv_n = 1 / N
   int32_t x_bf16, w_bf16;
   int32_t out_kind;  // 0 f32, 1 bf16, 2 e4m3
 };
@@ -233,12 +233,13 @@ struct NormBwdArgs {
   const float *rstd;
   void *dx;
   int64_t M, N, lddy, lds, ldds, lddx;
+  float inv_n;  // 1 / N
   int32_t x_bf16, w_bf16;
 };
 // norm false: the row quantizer (out_kind 2).
 cudaError_t launch_rms_norm(const NormArgs &p, bool norm, cudaStream_t stream);
 // Blocks of the gradient kernel, and so rows of its scratch `part` (rows x N f32; null: no dweight).
-int rms_norm_bwd_parts(int64_t M, int64_t N);
+int rms_norm_bwd_blocks(const NormBwdArgs &p);
 cudaError_t launch_rms_norm_bwd(const NormBwdArgs &p, float *part, int grid, cudaStream_t stream);
 // out[n] = sum over r < rows, in a fixed order, of part[r * N + n].
 cudaError_t launch_column_sum(const float *part, int rows, int64_t N, float *out, cudaStream_t stream);

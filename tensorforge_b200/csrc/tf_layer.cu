@@ -513,6 +513,7 @@ int tforge_rms_norm(const tforge_rms_norm_args *args, void *stream) {
   p.lds = a.lds;
   p.ldo = a.ldo;
   p.eps = a.eps;
+  p.inv_n = 1.0f / (float)a.N;
   p.x_bf16 = a.dtype == TFORGE_BF16;
   p.w_bf16 = a.weight_dtype == TFORGE_BF16;
   p.out_kind = a.out_dtype;
@@ -552,9 +553,10 @@ int tforge_rms_norm_backward(const tforge_rms_norm_backward_args *args, void *st
   p.lds = a.lds;
   p.ldds = a.ldds;
   p.lddx = a.lddx;
+  p.inv_n = 1.0f / (float)a.N;
   p.x_bf16 = a.dtype == TFORGE_BF16;
   p.w_bf16 = a.weight_dtype == TFORGE_BF16;
-  const int parts = rms_norm_bwd_parts(a.M, a.N);
+  const int parts = rms_norm_bwd_blocks(p);
   Scratch scratch(st);
   void *part = nullptr;
   if (a.dweight && parts > 1) {

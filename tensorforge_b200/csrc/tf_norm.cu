@@ -19,6 +19,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "tf_internal.h"
 #include "tf_ptx.cuh"
 
@@ -68,29 +70,55 @@ __device__ __forceinline__ uint32_t pack_e4m3x2(float lo, float hi) {
   return d;
 }
 
-// Sum of `a` and maximum of `b` over the T threads of one row.  `sm`: 2 x 32 words of shared memory
-// of the row's own (T > 32).  Every thread gets the same bits.
-template <int T>
+// Sum of `a` and, with MAX, maximum of `b` over the T threads of one row (T a power of two: below
+// 32 a part of a warp, above it the whole block).  `sm`: 64 words of shared memory for T > 32, not
+// written again before the next reduction's barrier but one.  Every thread of the row gets the
+// same bits.
+template <int T, bool MAX>
 __device__ __forceinline__ void row_reduce(float &a, uint32_t &b, uint32_t *sm) {
+  constexpr int W = T < 32 ? T : 32, N = T / 32;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
+  for (int o = W / 2; o; o >>= 1) {
     a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
-    b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
+    if constexpr (MAX) b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
   }
   if constexpr (T > 32) {
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) {
+    const int w = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) {
       sm[w] = __float_as_uint(a);
-      sm[32 + w] = b;
+      if constexpr (MAX) sm[32 + w] = b;
     }
     __syncthreads();
-    constexpr int W = T / 32;
-    a = lane < W ? __uint_as_float(sm[lane]) : 0.f;
-    b = lane < W ? sm[32 + lane] : 0u;
+    // The same sum in every thread: four or eight warps' values by 16-byte reads that a warp shares,
+    // else a read a lane and shuffles.
+    if constexpr (N == 4 || N == 8) {
+      float s[N];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
-      b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
+      for (int i = 0; i < N; i += 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(sm + i);
+        s[i] = v.x; s[i + 1] = v.y; s[i + 2] = v.z; s[i + 3] = v.w;
+      }
+#pragma unroll
+      for (int o = N / 2; o; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; ++i) s[i] += s[i + o];
+      a = s[0];
+      if constexpr (MAX) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(sm + 32 + i);
+          b = max(max(max(v.x, v.y), max(v.z, v.w)), b);
+        }
+      }
+    } else {
+      const int i = threadIdx.x & (N - 1);
+      a = __uint_as_float(sm[i]);
+      if constexpr (MAX) b = sm[32 + i];
+#pragma unroll
+      for (int o = N / 2; o; o >>= 1) {
+        a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+        if constexpr (MAX) b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
+      }
     }
   }
 }
@@ -127,36 +155,45 @@ __device__ __forceinline__ void out1(const NormArgs &p, int64_t m, int64_t c, fl
   else static_cast<uint8_t *>(p.out)[m * p.ldo + c] = (uint8_t)pack_e4m3x2(y, 0.f);
 }
 
-// The factor from t to what the output type holds, and the row's scale and rstd written by one thread.
+// Writes the row's rstd and scale (one thread).  What out holds of t = s weight: t rstd, for 8 bits
+// (t rstd) / scale -- in two steps, since rstd / scale overflows for a row of zeros.
 template <int OUT, bool NORM>
-__device__ __forceinline__ float finish_row(const NormArgs &p, int64_t m, float sumsq, uint32_t amax_bits, bool writer) {
-  float f = 1.f;
-  if constexpr (NORM) {
-    f = __frsqrt_rn(__fadd_rn(__fdiv_rn(sumsq, (float)p.N), p.eps));
-    if (writer && p.rstd) p.rstd[m] = f;
-  }
-  if constexpr (OUT == OUT_E4M3) {
-    float scale = __fdiv_rn(__uint_as_float(amax_bits) * f, kE4m3Max);
-    scale = scale < kTinyScale ? kTinyScale : scale;  // keeps a NaN
-    if (writer) p.scale[m] = scale;
-    return scale;
-  }
-  return f;
-}
+struct RowFactors {
+  float rstd = 1.f, inv = 1.f;
 
-// One row on T threads, E elements a thread in registers; 32-thread rows share a block of eight.
-// VEC: groups of eight consecutive elements (all rows on 16-byte boundaries, N a multiple of 8);
-// else single elements, T apart.  NORM false: the quantizer (y = x).
+  __device__ __forceinline__ RowFactors(const NormArgs &p, int64_t m, float sumsq, uint32_t amax_bits, bool writer) {
+    if constexpr (NORM) {
+      rstd = rsqrtf(fmaf(sumsq, p.inv_n, p.eps));
+      if (writer && p.rstd) p.rstd[m] = rstd;
+    }
+    if constexpr (OUT == OUT_E4M3) {
+      float scale = __fdiv_rn(__uint_as_float(amax_bits) * rstd, kE4m3Max);
+      scale = scale < kTinyScale ? kTinyScale : scale;  // keeps a NaN
+      if (writer) p.scale[m] = scale;
+      inv = __frcp_rn(scale);
+    }
+  }
+  __device__ __forceinline__ float operator()(float t) const {
+    if constexpr (NORM) t *= rstd;
+    if constexpr (OUT == OUT_E4M3) t *= inv;
+    return t;
+  }
+};
+
+// One row on T threads, E elements a thread in registers; below 128 threads a block of 256 holds
+// several rows.  VEC: groups of eight consecutive elements (all rows on 16-byte boundaries, N a
+// multiple of 8); else single elements, T apart.  NORM false: the quantizer (y = x).
 template <typename X, int OUT, bool VEC, int T, int E, bool NORM>
-__global__ void __launch_bounds__(T == 32 ? 256 : T) norm_row_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(T <= 32 ? 256 : T) norm_row_kernel(const NormArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  constexpr int kRows = T == 32 ? 8 : 1;
-  __shared__ uint32_t sm[64];
-  const int t = T == 32 ? (threadIdx.x & 31) : threadIdx.x;
-  const int64_t m = (int64_t)blockIdx.x * kRows + (T == 32 ? threadIdx.x >> 5 : 0);
-  if (kRows > 1 && m >= p.M) return;  // whole warps: nothing below waits for them
-  const int N = (int)p.N;
+  constexpr int kRows = T <= 32 ? 256 / T : 1;
+  __shared__ __align__(16) uint32_t sm[64];
+  const int t = threadIdx.x & (T - 1);
+  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / T;
+  const bool live = row < p.M;  // a part of a warp without a row goes along with no columns
+  const int64_t m = live ? row : 0;
+  const int N = live ? (int)p.N : 0;
   const X *x = static_cast<const X *>(p.x) + m * p.ldx;
   const X *r = p.residual ? static_cast<const X *>(p.residual) + m * p.ldr : nullptr;
   X *so = p.sum_out ? static_cast<X *>(p.sum_out) + m * p.lds : nullptr;
@@ -234,12 +271,8 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) norm_row_kernel(const NormA
       }
     }
   }
-  row_reduce<T>(sumsq, amax, sm);
-  const float f = finish_row<OUT, NORM>(p, m, sumsq, amax, t == 0);
-  // 8 bits: y / scale with y = t rstd, as y times the scale's inverse.
-  const float rs = OUT == OUT_E4M3 && NORM ? __frsqrt_rn(__fadd_rn(__fdiv_rn(sumsq, (float)p.N), p.eps)) : 1.f;
-  const float inv = OUT == OUT_E4M3 ? __frcp_rn(f) : f;
-  auto value = [&](float a) { return OUT == OUT_E4M3 && NORM ? (a * rs) * inv : a * inv; };
+  row_reduce<T, OUT == OUT_E4M3>(sumsq, amax, sm);
+  const RowFactors<OUT, NORM> f(p, m, sumsq, amax, t == 0 && live);
   if constexpr (VEC) {
 #pragma unroll
     for (int i = 0; i < E / 8; ++i) {
@@ -247,7 +280,7 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) norm_row_kernel(const NormA
       if (c < N) {
         float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = value(v[8 * i + j]);
+        for (int j = 0; j < 8; ++j) y[j] = f(v[8 * i + j]);
         out8<OUT>(p, m, c, y);
       }
     }
@@ -255,7 +288,7 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) norm_row_kernel(const NormA
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int c = i * T + t;
-      if (c < N) out1<OUT>(p, m, c, value(v[i]));
+      if (c < N) out1<OUT>(p, m, c, f(v[i]));
     }
   }
 }
@@ -266,7 +299,7 @@ template <typename X, int OUT, bool NORM>
 __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  __shared__ uint32_t sm[64];
+  __shared__ __align__(16) uint32_t sm[64];
   const int64_t m = blockIdx.x;
   const X *x = static_cast<const X *>(p.x) + m * p.ldx;
   const X *r = p.residual ? static_cast<const X *>(p.residual) + m * p.ldr : nullptr;
@@ -283,125 +316,159 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs p) {
     }
     if constexpr (OUT == OUT_E4M3) amax = max(amax, __float_as_uint(s) & 0x7FFFFFFFu);
   }
-  row_reduce<1024>(sumsq, amax, sm);
-  const float f = finish_row<OUT, NORM>(p, m, sumsq, amax, threadIdx.x == 0);
-  const float rs = OUT == OUT_E4M3 && NORM ? __frsqrt_rn(__fadd_rn(__fdiv_rn(sumsq, (float)p.N), p.eps)) : 1.f;
-  const float inv = OUT == OUT_E4M3 ? __frcp_rn(f) : f;
+  row_reduce<1024, OUT == OUT_E4M3>(sumsq, amax, sm);
+  const RowFactors<OUT, NORM> f(p, m, sumsq, amax, threadIdx.x == 0);
 #pragma unroll 4
   for (int64_t c = threadIdx.x; c < p.N; c += 1024) {
     float s = to_f32(x[c]);
     if (r) s = __fadd_rn(s, to_f32(r[c]));
     if (so) store1(so + c, s);
     if constexpr (NORM) s *= weight_at(p, c);
-    out1<OUT>(p, m, c, OUT == OUT_E4M3 && NORM ? (s * rs) * inv : s * inv);
+    out1<OUT>(p, m, c, f(s));
   }
 }
 
 // ---- gradient ------------------------------------------------------------------------------------
 
-// Blocks of kRows rows at a time (kRows = 8 for 32-thread rows); row group b, b + gridDim.x, ...
-// part: gridDim.x rows of N f32, this block's column sums (null: no dweight).
-template <typename X, bool VEC, int T, int E>
-__global__ void __launch_bounds__(T == 32 ? 256 : T) norm_bwd_kernel(const NormBwdArgs p, float *__restrict__ part) {
+// E elements of a row as they are loaded: 16-byte pieces (VEC), or single elements.
+template <typename X, bool VEC, int E>
+struct RawRow {
+  using Piece = std::conditional_t<VEC, uint4, X>;
+  static constexpr int kPer = VEC ? 16 / (int)sizeof(X) : 1, kPieces = E / kPer;
+  Piece v[kPieces];
+
+  // Columns of element e of thread t: groups of eight with VEC, else single ones T apart.
+  template <int T>
+  __device__ __forceinline__ static int col(int e, int t) { return VEC ? ((e / 8) * T + t) * 8 + e % 8 : e * T + t; }
+  // Columns below n (a multiple of 8 with VEC); the others are zeros.
+  template <int T>
+  __device__ __forceinline__ void load(const X *row, int t, int n) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int c = col<T>(i * kPer, t);
+      if (c < n) v[i] = *reinterpret_cast<const Piece *>(row + c);
+      else v[i] = Piece{};
+    }
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (!VEC) {
+      return to_f32(v[e]);
+    } else {
+      const uint4 &u = v[e / kPer];
+      if constexpr (sizeof(X) == 4) {
+        const uint32_t w = e % 4 == 0 ? u.x : e % 4 == 1 ? u.y : e % 4 == 2 ? u.z : u.w;
+        return __uint_as_float(w);
+      } else {
+        const uint32_t w = e % 8 / 2 == 0 ? u.x : e % 8 / 2 == 1 ? u.y : e % 8 / 2 == 2 ? u.z : u.w;
+        return __uint_as_float(e % 2 ? w & 0xFFFF0000u : w << 16);
+      }
+    }
+  }
+};
+
+// Threads of a block and, up to 32 threads a row, its rows.
+template <int T>
+constexpr int kBwdBlock = T <= 32 ? 256 : T;
+
+// How the gradient kernel holds a row: as it was loaded; the same, with the next row's loads under way
+// while a row is reduced and written; or not at all, reading it again after the reduction.
+enum Hold : int { HOLD_ROW = 0, HOLD_NEXT = 1, HOLD_NONE = 2 };
+
+// Row groups b, b + gridDim.x, ... of block b.  part: gridDim.x rows of N f32, this block's column sums (null: no dweight).
+template <typename X, bool VEC, int T, int E, int HOLD>
+__global__ void __launch_bounds__(kBwdBlock<T>) norm_bwd_kernel(const NormBwdArgs p, float *__restrict__ part) {
   grid_dependency_wait();
   grid_launch_dependents();
-  constexpr int kRows = T == 32 ? 8 : 1;
-  __shared__ uint32_t sm[2][64];
+  using Raw = RawRow<X, VEC, E>;
+  constexpr int kRows = kBwdBlock<T> / T;
+  __shared__ __align__(16) uint32_t sm[2][64];
   __shared__ float comb[kRows > 1 ? kRows * T * E : 1];
-  const int t = T == 32 ? (threadIdx.x & 31) : threadIdx.x, sub = T == 32 ? threadIdx.x >> 5 : 0;
-  const int N = (int)p.N;
-  auto col = [&](int e) { return VEC ? ((e / 8) * T + t) * 8 + e % 8 : e * T + t; };
+  const int t = threadIdx.x & (T - 1), sub = threadIdx.x / T;
   NormArgs wa{};
   wa.weight = p.weight;
   wa.w_bf16 = p.w_bf16;
   float w[E], acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    w[e] = col(e) < N ? weight_at(wa, col(e)) : 0.f;
+    const int c = Raw::template col<T>(e, t);
+    w[e] = c < p.N ? weight_at(wa, c) : 0.f;
     acc[e] = 0.f;
   }
+  struct Rows {
+    Raw y, s, d;
+    float rstd;
+  };
+  Rows next;
+  auto fetch = [&](int64_t m0, bool first) {
+    const bool live = m0 + sub < p.M;  // a part of a warp without a row goes along with no columns
+    const int64_t m = live ? m0 + sub : 0;
+    const int n = live ? (int)p.N : 0;
+    next.y.template load<T>(static_cast<const X *>(p.dy) + m * p.lddy, t, n);
+    next.s.template load<T>(static_cast<const X *>(p.s) + m * p.lds, t, n);
+    if (p.ds && !(HOLD == HOLD_NONE && first)) next.d.template load<T>(static_cast<const X *>(p.ds) + m * p.ldds, t, n);
+    next.rstd = __ldg(p.rstd + m);
+  };
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t m0 = (int64_t)blockIdx.x * kRows;
+  if (HOLD == HOLD_NEXT && m0 < p.M) fetch(m0, true);
   int par = 0;
-  for (int64_t m = (int64_t)blockIdx.x * kRows + sub; m < p.M; m += (int64_t)gridDim.x * kRows, par ^= 1) {
-    const X *dy = static_cast<const X *>(p.dy) + m * p.lddy;
-    const X *s = static_cast<const X *>(p.s) + m * p.lds;
-    const X *ds = p.ds ? static_cast<const X *>(p.ds) + m * p.ldds : nullptr;
-    X *dx = static_cast<X *>(p.dx) + m * p.lddx;
-    const float rstd = __ldg(p.rstd + m);
-    float g[E], h[E], d[E];
-    if constexpr (VEC) {
-#pragma unroll
-      for (int i = 0; i < E / 8; ++i) {
-        float (&gg)[8] = *reinterpret_cast<float (*)[8]>(&g[8 * i]);
-        float (&hh)[8] = *reinterpret_cast<float (*)[8]>(&h[8 * i]);
-        float (&dd)[8] = *reinterpret_cast<float (*)[8]>(&d[8 * i]);
-        const int c = (i * T + t) * 8;
-        if (c < N) {
-          load8(dy + c, gg);
-          load8(s + c, hh);
-          if (ds) load8(ds + c, dd);
-        }
-        if (c >= N || !ds) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) dd[j] = 0.f;
-        }
-        if (c >= N) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) gg[j] = hh[j] = 0.f;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int c = e * T + t;
-        g[e] = c < N ? to_f32(dy[c]) : 0.f;
-        h[e] = c < N ? to_f32(s[c]) : 0.f;
-        d[e] = c < N && ds ? to_f32(ds[c]) : 0.f;
-      }
-    }
+  for (; m0 < p.M; m0 += step, par ^= 1) {
+    // The row is kept as it was loaded, and unpacked before and after the reduction: fewer registers.
+    if constexpr (HOLD != HOLD_NEXT) fetch(m0, true);
+    Rows row = next;
     float dot = 0.f;
-    uint32_t none = 0u;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      h[e] *= rstd;
-      acc[e] = fmaf(g[e], h[e], acc[e]);
-      g[e] *= w[e];
-      dot = fmaf(g[e], h[e], dot);
+      const float y = row.y.get(e), h = row.s.get(e) * row.rstd;
+      acc[e] = fmaf(y, h, acc[e]);
+      dot = fmaf(y * w[e], h, dot);
     }
-    row_reduce<T>(dot, none, sm[par]);  // two buffers: the next row's may be written while this one is read
-    const float c1 = __fdiv_rn(dot, (float)N);
+    if (HOLD == HOLD_NEXT && m0 + step < p.M) fetch(m0 + step, true);
+    uint32_t none = 0u;
+    row_reduce<T, false>(dot, none, sm[par]);
+    const float c1 = dot * p.inv_n;
+    if constexpr (HOLD == HOLD_NONE) {
+      fetch(m0, false);
+      row = next;
+    }
+    float g[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) g[e] = fmaf(rstd, fmaf(-h[e], c1, g[e]), d[e]);
+    for (int e = 0; e < E; ++e)
+      g[e] = fmaf(row.rstd, fmaf(-row.s.get(e) * row.rstd, c1, row.y.get(e) * w[e]), p.ds ? row.d.get(e) : 0.f);
+    const int n = m0 + sub < p.M ? (int)p.N : 0;
+    X *dx = static_cast<X *>(p.dx) + (m0 + sub) * p.lddx;
     if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < E / 8; ++i) {
         const int c = (i * T + t) * 8;
-        if (c < N) store8(dx + c, *reinterpret_cast<const float (*)[8]>(&g[8 * i]));
+        if (c < n) store8(dx + c, *reinterpret_cast<const float (*)[8]>(&g[8 * i]));
       }
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (e * T + t < N) store1(dx + e * T + t, g[e]);
+        if (e * T + t < n) store1(dx + e * T + t, g[e]);
     }
   }
   if (!part) return;
-  float *row = part + (int64_t)blockIdx.x * N;
+  float *row = part + (int64_t)blockIdx.x * p.N;
   if constexpr (kRows > 1) {
 #pragma unroll
     for (int e = 0; e < E; ++e) comb[(sub * E + e) * T + t] = acc[e];
     __syncthreads();
-    if (sub == 0) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float v = acc[e];
-#pragma unroll
-        for (int r = 1; r < kRows; ++r) v += comb[(r * E + e) * T + t];
-        if (col(e) < N) row[col(e)] = v;
-      }
+    // Element e of thread t, summed over the block's rows in order, by thread e T + t.
+    for (int i = threadIdx.x; i < E * T; i += kBwdBlock<T>) {
+      float v = 0.f;
+#pragma unroll 4
+      for (int q = 0; q < kRows; ++q) v += comb[q * E * T + i];
+      const int c = Raw::template col<T>(i / T, i % T);
+      if (c < p.N) row[c] = v;
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (col(e) < N) row[col(e)] = acc[e];
+    for (int e = 0; e < E; ++e) {
+      const int c = Raw::template col<T>(e, t);
+      if (c < p.N) row[c] = acc[e];
+    }
   }
 }
 
@@ -411,7 +478,7 @@ template <typename X>
 __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwdArgs p, float *__restrict__ part) {
   grid_dependency_wait();
   grid_launch_dependents();
-  __shared__ uint32_t sm[2][64];
+  __shared__ __align__(16) uint32_t sm[2][64];
   NormArgs wa{};
   wa.weight = p.weight;
   wa.w_bf16 = p.w_bf16;
@@ -429,8 +496,8 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwdArgs p
 #pragma unroll 4
     for (int64_t c = threadIdx.x; c < p.N; c += 1024)
       dot = fmaf(to_f32(dy[c]) * weight_at(wa, c), to_f32(s[c]) * rstd, dot);
-    row_reduce<1024>(dot, none, sm[par]);
-    const float c1 = __fdiv_rn(dot, (float)p.N);
+    row_reduce<1024, false>(dot, none, sm[par]);
+    const float c1 = dot * p.inv_n;
 #pragma unroll 4
     for (int64_t c = threadIdx.x; c < p.N; c += 1024) {
       const float y = to_f32(dy[c]), h = to_f32(s[c]) * rstd, d = ds ? to_f32(ds[c]) : 0.f;
@@ -466,14 +533,19 @@ bool at16(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 
 template <typename X, int OUT, bool VEC, bool NORM>
 cudaError_t launch_norm_rows(const NormArgs &p, cudaStream_t st) {
-  const unsigned g = (unsigned)p.M;
-  if (p.N <= 256) return launch_dependent(norm_row_kernel<X, OUT, VEC, 32, 8, NORM>, dim3((unsigned)((p.M + 7) / 8)), dim3(256), st, p);
-  if (p.N <= 1024) return launch_dependent(norm_row_kernel<X, OUT, VEC, 128, 8, NORM>, dim3(g), dim3(128), st, p);
-  if (p.N <= 2048) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 8, NORM>, dim3(g), dim3(256), st, p);
-  if (p.N <= 4096) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 16, NORM>, dim3(g), dim3(256), st, p);
-  if (p.N <= 8192) return launch_dependent(norm_row_kernel<X, OUT, VEC, 512, 16, NORM>, dim3(g), dim3(512), st, p);
-  if (p.N <= 16384) return launch_dependent(norm_row_kernel<X, OUT, VEC, 1024, 16, NORM>, dim3(g), dim3(1024), st, p);
-  return launch_dependent(norm_long_kernel<X, OUT, NORM>, dim3(g), dim3(1024), st, p);
+  auto grid = [&](int rows) { return dim3((unsigned)((p.M + rows - 1) / rows)); };
+  if constexpr (VEC) {
+    if (p.N <= 64) return launch_dependent(norm_row_kernel<X, OUT, VEC, 8, 8, NORM>, grid(32), dim3(256), st, p);
+    if (p.N <= 128) return launch_dependent(norm_row_kernel<X, OUT, VEC, 16, 8, NORM>, grid(16), dim3(256), st, p);
+  }
+  if (p.N <= 256) return launch_dependent(norm_row_kernel<X, OUT, VEC, 32, 8, NORM>, grid(8), dim3(256), st, p);
+  if (p.N <= 512) return launch_dependent(norm_row_kernel<X, OUT, VEC, 32, 16, NORM>, grid(8), dim3(256), st, p);
+  if (p.N <= 1024) return launch_dependent(norm_row_kernel<X, OUT, VEC, 128, 8, NORM>, grid(1), dim3(128), st, p);
+  if (p.N <= 2048) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 8, NORM>, grid(1), dim3(256), st, p);
+  if (p.N <= 4096) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 16, NORM>, grid(1), dim3(256), st, p);
+  if (p.N <= 8192) return launch_dependent(norm_row_kernel<X, OUT, VEC, 512, 16, NORM>, grid(1), dim3(512), st, p);
+  if (p.N <= 16384) return launch_dependent(norm_row_kernel<X, OUT, VEC, 512, 32, NORM>, grid(1), dim3(512), st, p);
+  return launch_dependent(norm_long_kernel<X, OUT, NORM>, grid(1), dim3(1024), st, p);
 }
 
 template <typename X, int OUT, bool NORM>
@@ -486,15 +558,38 @@ cudaError_t launch_norm_vec(const NormArgs &p, cudaStream_t st) {
   return vec ? launch_norm_rows<X, OUT, true, NORM>(p, st) : launch_norm_rows<X, OUT, false, NORM>(p, st);
 }
 
+// The gradient kernel of a call: eight elements a thread up to 8192 columns, sixteen up to 16384.
+struct BwdKernel {
+  void (*kern)(const NormBwdArgs, float *);
+  int threads, rows, id;  // of a block; a number of its own
+};
+template <typename X, bool VEC, int T, int E>
+BwdKernel bwd_kernel(int id) {
+  // Two rows' pieces fit the registers for bf16 in 16-byte pieces; elsewhere a thread's loads are
+  // enough by themselves.  Sixteen elements a thread do not fit even once at 1024 threads.
+  constexpr int kHold = E > 8 ? HOLD_NONE : VEC && sizeof(X) == 2 ? HOLD_NEXT : HOLD_ROW;
+  return {norm_bwd_kernel<X, VEC, T, E, kHold>, kBwdBlock<T>, kBwdBlock<T> / T, id};
+}
 template <typename X, bool VEC>
-cudaError_t launch_bwd_rows(const NormBwdArgs &p, float *part, int grid, cudaStream_t st) {
-  if (p.N <= 256) return launch_dependent(norm_bwd_kernel<X, VEC, 32, 8>, dim3(grid), dim3(256), st, p, part);
-  if (p.N <= 1024) return launch_dependent(norm_bwd_kernel<X, VEC, 128, 8>, dim3(grid), dim3(128), st, p, part);
-  if (p.N <= 2048) return launch_dependent(norm_bwd_kernel<X, VEC, 256, 8>, dim3(grid), dim3(256), st, p, part);
-  if (p.N <= 4096) return launch_dependent(norm_bwd_kernel<X, VEC, 256, 16>, dim3(grid), dim3(256), st, p, part);
-  if (p.N <= 8192) return launch_dependent(norm_bwd_kernel<X, VEC, 512, 16>, dim3(grid), dim3(512), st, p, part);
-  if (p.N <= 16384) return launch_dependent(norm_bwd_kernel<X, VEC, 1024, 16>, dim3(grid), dim3(1024), st, p, part);
-  return launch_dependent(norm_bwd_long_kernel<X>, dim3(grid), dim3(1024), st, p, part);
+BwdKernel pick_bwd(int64_t N, int id) {
+  if constexpr (VEC) {
+    if (N <= 64) return bwd_kernel<X, VEC, 8, 8>(id);
+    if (N <= 128) return bwd_kernel<X, VEC, 16, 8>(id + 1);
+  }
+  if (N <= 256) return bwd_kernel<X, VEC, 32, 8>(id + 2);
+  if (N <= 512) return bwd_kernel<X, VEC, 64, 8>(id + 9);
+  if (N <= 1024) return bwd_kernel<X, VEC, 128, 8>(id + 3);
+  if (N <= 2048) return bwd_kernel<X, VEC, 256, 8>(id + 4);
+  if (N <= 4096) return bwd_kernel<X, VEC, 512, 8>(id + 5);
+  if (N <= 8192) return bwd_kernel<X, VEC, 1024, 8>(id + 6);
+  if (N <= 16384) return bwd_kernel<X, VEC, 1024, 16>(id + 7);
+  return {norm_bwd_long_kernel<X>, 1024, 1, id + 8};
+}
+
+bool bwd_vec(const NormBwdArgs &p) {
+  const int e = p.x_bf16 ? 2 : 4;
+  return p.N % 8 == 0 && at16(p.dy) && at16(p.s) && at16(p.ds) && at16(p.dx) && p.lddy * e % 16 == 0 &&
+         p.lds * e % 16 == 0 && p.ldds * e % 16 == 0 && p.lddx * e % 16 == 0;
 }
 
 }  // namespace
@@ -512,21 +607,31 @@ cudaError_t launch_rms_norm(const NormArgs &p, bool norm, cudaStream_t st) {
   return p.x_bf16 ? launch_norm_vec<__nv_bfloat16, OUT_E4M3, false>(p, st) : launch_norm_vec<float, OUT_E4M3, false>(p, st);
 }
 
-int rms_norm_bwd_parts(int64_t M, int64_t N) {
-  // Blocks that fill the SMs (2048 threads each) once; no more than there are row groups.
-  const int64_t threads = N <= 256 ? 256 : (N <= 1024 ? 128 : (N <= 4096 ? 256 : (N <= 8192 ? 512 : 1024)));
-  const int64_t rows = N <= 256 ? 8 : 1;
-  const int64_t groups = (M + rows - 1) / rows, most = 148 * (1024 / threads);
+static BwdKernel pick_bwd(const NormBwdArgs &p) {
+  const bool vec = bwd_vec(p);
+  if (p.x_bf16) return vec ? pick_bwd<__nv_bfloat16, true>(p.N, 0) : pick_bwd<__nv_bfloat16, false>(p.N, 10);
+  return vec ? pick_bwd<float, true>(p.N, 20) : pick_bwd<float, false>(p.N, 30);
+}
+
+int rms_norm_bwd_blocks(const NormBwdArgs &p) {
+  // As many blocks as the SMs hold at once, no more than there are row groups.
+  const BwdKernel k = pick_bwd(p);
+  static std::atomic<int> resident[40];
+  int n = resident[k.id].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k.kern, k.threads, 0) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = 1;
+    }
+    resident[k.id].store(n, std::memory_order_relaxed);
+  }
+  const int64_t groups = (p.M + k.rows - 1) / k.rows, most = 148LL * n;
   return (int)(groups < most ? groups : most);
 }
 
 cudaError_t launch_rms_norm_bwd(const NormBwdArgs &p, float *part, int grid, cudaStream_t st) {
-  const int e = p.x_bf16 ? 2 : 4;
-  const bool vec = p.N % 8 == 0 && at16(p.dy) && at16(p.s) && at16(p.ds) && at16(p.dx) && p.lddy * e % 16 == 0 &&
-                   p.lds * e % 16 == 0 && p.ldds * e % 16 == 0 && p.lddx * e % 16 == 0;
-  if (p.x_bf16)
-    return vec ? launch_bwd_rows<__nv_bfloat16, true>(p, part, grid, st) : launch_bwd_rows<__nv_bfloat16, false>(p, part, grid, st);
-  return vec ? launch_bwd_rows<float, true>(p, part, grid, st) : launch_bwd_rows<float, false>(p, part, grid, st);
+  const BwdKernel k = pick_bwd(p);
+  return launch_dependent(k.kern, dim3((unsigned)grid), dim3((unsigned)k.threads), st, p, part);
 }
 
 cudaError_t launch_column_sum(const float *part, int rows, int64_t N, float *out, cudaStream_t st) {

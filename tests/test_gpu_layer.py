@@ -466,6 +466,72 @@ def test_rms_norm_rows(m):
     check_rms_norm(m, 1024)
 
 
+# Several rows a block of the gradient at every width class, the last round only partly filled.
+MANY = [(19000, 264), (19003, 300), (20001, 511), (5000, 1024), (5003, 1111), (5000, 2048), (2400, 4096), (2401, 4099),
+        (1200, 5001), (1300, 8192), (700, 10007), (600, 16384)]
+
+
+@pytest.mark.parametrize("m,n", MANY)
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float8_e4m3fn),
+                                       (torch.float32, torch.float32)])
+def test_rms_norm_many_rows(m, n, dtype, out):
+    check_rms_norm(m, n, dtype, out)
+    check_rms_norm(m, n, dtype, out, residual=False, pad=3, shift=1)
+
+
+@pytest.mark.parametrize("pad,shift", [(8, 8), (1, 0), (0, 1), (7, 5), (2, 4)])
+@pytest.mark.parametrize("m,n", [(19003, 300), (5003, 1111)])
+def test_rms_norm_many_rows_pitches(m, n, pad, shift):
+    for where in ("", "x", "residual"):
+        check_rms_norm(m, n, torch.bfloat16, torch.float8_e4m3fn, pad=pad, shift=shift, in_place=where)
+    check_rms_norm_backward(m, n, pad=pad, shift=shift)
+    check_rms_norm_backward(m, n, pad=pad, shift=shift, in_place=True)
+
+
+@pytest.mark.parametrize("m,n", MANY)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rms_norm_backward_many_rows(m, n, dtype):
+    check_rms_norm_backward(m, n, dtype)
+    check_rms_norm_backward(m, n, dtype, ds=False, dweight=False, pad=3, shift=1)
+
+
+@pytest.mark.parametrize("m,n", [(70, 16), (33, 64), (100, 72), (17, 128), (4099, 40)])
+def test_rms_norm_narrow_rows(m, n):
+    """Several rows a warp, the last warp only partly filled."""
+    check_rms_norm(m, n, out=torch.float8_e4m3fn)
+    check_rms_norm(m, n, torch.float32, torch.float32)
+    check_rms_norm_backward(m, n)
+    check_rms_norm_backward(m, n, torch.float32)
+
+
+def test_quantize_many_rows():
+    for m, n, dtype in ((19003, 300, torch.bfloat16), (2401, 4096, torch.float32)):
+        x = rand(m, n, dtype=dtype)
+        q, sc = torch.empty(m, n, device="cuda", dtype=torch.float8_e4m3fn), torch.empty(m, device="cuda")
+        _lib.quantize_e4m3(ptr(x), ptr(q), ptr(sc), m, n, CODE[dtype], stream=torch.cuda.current_stream().cuda_stream)
+        v, s64 = quantize64(x.double())
+        assert_within(sc, s64, 2.0 ** -24 * s64)
+        assert_within(q.float(), v, v.abs() * (2.0 ** -21) + torch.clamp(v.abs() * 2.0 ** -4, min=2.0 ** -10))
+
+
+def test_linear_waits_are_bounded():
+    L, s = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    L.tforge_set_wait_limit_ns(20_000_000)
+    try:
+        for force in ((1, 16, 1), (1, 64, 4), (2, 0, 0)):
+            for dtype, trans_b in ((torch.bfloat16, False), (torch.float8_e4m3fn, True)):
+                _lib.check(L.tforge_debug_linear_kernel(*force))
+                c = Linear(300, 520, 640, dtype, "gelu", trans_b=trans_b)
+                L.tforge_debug_skip_load(1)
+                c.call()
+                assert _lib.device_status(s) == _lib.ERR_TIMEOUT
+                L.tforge_debug_skip_load(0)
+                c.call().check()
+    finally:
+        L.tforge_debug_skip_load(0)
+        L.tforge_set_wait_limit_ns(0)
+
+
 @pytest.mark.parametrize("scale", [1e-12, 1e-4, 1e4, 1e12])
 def test_rms_norm_magnitudes(scale):
     check_rms_norm(5, 520, torch.float32, torch.float32, scale=scale)
