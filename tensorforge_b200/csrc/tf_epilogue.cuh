@@ -11,24 +11,47 @@
 
 namespace tf {
 
-// z / (1 + exp(-u)), the logistic gate: silu with u = z, the tanh form of gelu with
-// u = 2 sqrt(2/pi) (z + 0.044715 z^3), since (1 + tanh a) / 2 = 1 / (1 + exp(-2 a)).  Where exp
-// overflows the gate is 0, and __fdividef by a divisor above 2^126 gives that 0.  As in the formula,
-// z = -inf gives NaN.
-__device__ __forceinline__ float gated(float z, float u) { return __fdividef(z, 1.0f + __expf(-u)); }
+__device__ __forceinline__ float ex2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The logistic gate 1 / (1 + exp(-u)), u = -w / log2 e: silu is z gate(z), the tanh form of gelu
+// z gate(2 sqrt(2/pi) (z + 0.044715 z^3)), since (1 + tanh a) / 2 = 1 / (1 + exp(-2 a)).  The factor
+// -log2 e is folded into the polynomials.  Where 2^w overflows the gate is 0.
+__device__ __forceinline__ float gate(float w) { return rcp_approx(1.0f + ex2_approx(w)); }
 constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluC3 = 0.044715f * kGeluC;
 
-// z Phi(z), Phi(z) = (1 + erf(z / sqrt 2)) / 2: the sum cancels below z = -3, where the result's
-// absolute error stays under 2^-24 |z|.
-__device__ __forceinline__ float normal_cdf(float z) { return fmaf(0.5f, erff(z * 0.70710678118654752f), 0.5f); }
+// The normal distribution's Phi, by the rational approximation 7.1.26 of Abramowitz and Stegun's
+// Handbook of Mathematical Functions to erfc(|z| / sqrt 2) (absolute error of erf 1.5e-7), whose
+// exp(-z^2 / 2) is also the density's: `e`.  The lower tail comes without cancellation.
+__device__ __forceinline__ float normal_cdf(float z, float &e) {
+  const float t = rcp_approx(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
+  float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+  q = fmaf(q, t, 0.5f * 1.421413741f);
+  q = fmaf(q, t, 0.5f * -0.284496736f);
+  q = fmaf(q, t, 0.5f * 0.254829592f);
+  e = ex2_approx(z * z * (-0.5f * kLog2e));
+  const float tail = q * t * e;  // Phi(-|z|)
+  return z > 0.0f ? 1.0f - tail : tail;
+}
 
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == TFORGE_ACT_RELU) return relu_ieee(z);
-  else if constexpr (ACT == TFORGE_ACT_GELU) return z * normal_cdf(z);
-  else if constexpr (ACT == TFORGE_ACT_GELU_TANH) return gated(z, z * fmaf(kGeluC3, z * z, kGeluC));
-  else if constexpr (ACT == TFORGE_ACT_SILU) return gated(z, z);
+  else if constexpr (ACT == TFORGE_ACT_GELU) {
+    float e;
+    return z * normal_cdf(z, e);
+  } else if constexpr (ACT == TFORGE_ACT_GELU_TANH) return z * gate(z * fmaf(-kLog2e * kGeluC3, z * z, -kLog2e * kGeluC));
+  else if constexpr (ACT == TFORGE_ACT_SILU) return z * gate(-kLog2e * z);
   else return z;
 }
 
@@ -36,17 +59,19 @@ __device__ __forceinline__ float activate(float z) {
 template <int ACT>
 __device__ __forceinline__ float activate_slope(float z) {
   if constexpr (ACT == TFORGE_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
-  else if constexpr (ACT == TFORGE_ACT_GELU)
-    return fmaf(z, 0.3989422804014327f * __expf(-0.5f * z * z), normal_cdf(z));
-  else if constexpr (ACT == TFORGE_ACT_GELU_TANH || ACT == TFORGE_ACT_SILU) {
-    // s = 1 / (1 + exp(-u)): d(z s)/dz = s + z u' s (1 - s).
+  else if constexpr (ACT == TFORGE_ACT_GELU) {
+    float e;
+    const float p = normal_cdf(z, e);
+    return fmaf(z * 0.3989422804014327f, e, p);
+  } else if constexpr (ACT == TFORGE_ACT_GELU_TANH || ACT == TFORGE_ACT_SILU) {
+    // s = gate(u): d(z s)/dz = s + z u' s (1 - s).
     constexpr bool kTanh = ACT == TFORGE_ACT_GELU_TANH;
     const float z2 = z * z;
-    const float u = kTanh ? z * fmaf(kGeluC3, z2, kGeluC) : z;
-    const float du = kTanh ? fmaf(3.0f * kGeluC3, z2, kGeluC) : 1.0f;
-    const float s = __fdividef(1.0f, 1.0f + __expf(-u));
-    const float v = s * (1.0f - s);
-    return v == 0.0f ? s : fmaf(z * du, v, s);  // the gate is 0 or 1: z u' may have overflowed
+    const float w = kTanh ? z * fmaf(-kLog2e * kGeluC3, z2, -kLog2e * kGeluC) : -kLog2e * z;
+    const float zdu = kTanh ? z * fmaf(3.0f * kGeluC3, z2, kGeluC) : z;
+    const float s = gate(w);
+    const float v = fmaf(-s, s, s);
+    return v == 0.0f ? s : fmaf(zdu, v, s);  // the gate is 0 or 1: z u' may have overflowed
   } else return 1.0f;
 }
 

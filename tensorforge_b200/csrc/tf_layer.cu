@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 
@@ -67,56 +68,81 @@ bool pitch(int64_t &ld, int64_t cols) {
   return ld >= cols && ld <= (int64_t)1 << 31;
 }
 
-// Stream-ordered scratch of one call, released (in stream order) when the call returns.
+// Stream-ordered scratch of one call: parts are asked for, then taken in one allocation, released (in
+// stream order) when the call returns.
 class Scratch {
  public:
   explicit Scratch(cudaStream_t st) : st_(st) {}
   Scratch(const Scratch &) = delete;
   ~Scratch() {
-    for (int i = 0; i < n_; ++i) cudaFreeAsync(p_[i], st_);
+    if (base_) cudaFreeAsync(base_, st_);
   }
-  int get(void **out, uint64_t bytes) {
+  // Offset of `bytes` more, on a 256-byte boundary.
+  uint64_t want(uint64_t bytes) {
+    const uint64_t at = size_;
+    size_ += (bytes + 255) & ~uint64_t(255);
+    return at;
+  }
+  int take() {
+    if (!size_) return TFORGE_OK;
     cudaMemPool_t pool = nullptr;
     int rc = device_pool(&pool);
     if (rc) return rc;
-    cudaError_t e = cudaMallocFromPoolAsync(out, bytes, pool, st_);
+    void *p = nullptr;
+    cudaError_t e = cudaMallocFromPoolAsync(&p, size_, pool, st_);
     if (e != cudaSuccess) return cuda_failure(e, "cudaMallocFromPoolAsync(layer scratch)");
-    p_[n_++] = *out;
+    base_ = static_cast<char *>(p);
     return TFORGE_OK;
   }
+  char *at(uint64_t offset) const { return base_ + offset; }
 
  private:
   cudaStream_t st_;
-  void *p_[8];
-  int n_ = 0;
+  char *base_ = nullptr;
+  uint64_t size_ = 0;
 };
 
 // ---- operand copies -------------------------------------------------------------------------------
 
-template <typename S, typename D>
-__device__ __forceinline__ D convert(S v) {
-  if constexpr (std::is_same<S, float>::value) return __float2bfloat16_rn(v);
-  else return v;
-}
+// dst[r * ldd + c] = src[r * lds + c]; dtype is src's: f32 is rounded to bf16.
+struct RowCopy {
+  const void *src;
+  void *dst;
+  int64_t rows, cols, lds, ldd;
+  int32_t dtype;
+};
 
-// dst[r * ldd + c] = src[r * lds + c], f32 rounded to bf16; rows of any alignment into rows on
-// 16-byte boundaries.  Eight elements a thread: single loads, one 16-byte (or 8-byte) store; what
-// lies beyond a row's end within the last group is written as 0.
+// Eight elements of a row that may start anywhere, into rows on 16-byte boundaries: single loads, one
+// store; what lies beyond a row's end within the last group is written as 0.
 template <typename S, typename D>
-__global__ void __launch_bounds__(256) copy_rows_kernel(const S *__restrict__ src, int64_t lds, D *__restrict__ dst,
-                                                        int64_t ldd, int64_t rows, int64_t cols) {
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const int64_t groups = (cols + 7) / 8, total = rows * groups;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+__device__ __forceinline__ void copy_groups(const RowCopy &j, int64_t first, int64_t step) {
+  const int64_t groups = (j.cols + 7) / 8, total = j.rows * groups;
+  for (int64_t i = first; i < total; i += step) {
     const int64_t r = i / groups, c = (i - r * groups) * 8;
-    const S *s = src + r * lds + c;
+    const S *s = static_cast<const S *>(j.src) + r * j.lds + c;
     __align__(16) D v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? convert<S, D>(s[j]) : D{};
-    if constexpr (sizeof(D) == 2) *reinterpret_cast<uint4 *>(dst + r * ldd + c) = *reinterpret_cast<const uint4 *>(v);
-    else *reinterpret_cast<uint2 *>(dst + r * ldd + c) = *reinterpret_cast<const uint2 *>(v);
+    for (int k = 0; k < 8; ++k) {
+      if constexpr (std::is_same<S, float>::value) v[k] = __float2bfloat16_rn(c + k < j.cols ? s[k] : 0.f);
+      else v[k] = c + k < j.cols ? s[k] : D{};
+    }
+    D *d = static_cast<D *>(j.dst) + r * j.ldd + c;
+    if constexpr (sizeof(D) == 2) *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(v);
+    else *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<const uint2 *>(v);
   }
+}
+
+// One or two operands' copies in one launch: blocks below `split` the first's, the others the second's.
+__global__ void __launch_bounds__(256) copy_rows_kernel(const RowCopy a, const RowCopy b, int split) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const bool second = (int)blockIdx.x >= split;
+  const RowCopy &j = second ? b : a;
+  const int64_t block = second ? blockIdx.x - split : blockIdx.x, blocks = second ? gridDim.x - split : split;
+  const int64_t first = block * 256 + threadIdx.x, step = blocks * 256;
+  if (j.dtype == TFORGE_F32) copy_groups<float, __nv_bfloat16>(j, first, step);
+  else if (j.dtype == TFORGE_BF16) copy_groups<uint16_t, uint16_t>(j, first, step);
+  else copy_groups<uint8_t, uint8_t>(j, first, step);
 }
 
 int64_t padded(int64_t cols, int esz) { return (cols * esz + 15) / 16 * 16 / esz; }
@@ -127,32 +153,46 @@ struct Operand {
   int64_t rows, cols, ld;  // as stored
 };
 
-int prepare_operand(Operand &o, int dtype, Scratch &scratch, cudaStream_t st) {
-  const int esz = dtype == TFORGE_E4M3 ? 1 : 2;
-  if (o.rows == 0 || o.cols == 0) return TFORGE_OK;
-  if (dtype != TFORGE_F32 && at(o.p, 16) && o.ld * esz % 16 == 0) return TFORGE_OK;
-  const int64_t ldd = padded(o.cols, esz);
-  void *q = nullptr;
-  int rc = scratch.get(&q, (uint64_t)o.rows * ldd * esz);
-  if (rc) return rc;
-  int64_t blocks = (o.rows * ((o.cols + 7) / 8) + 255) / 256;
-  if (blocks > 148 * 16) blocks = 148 * 16;
-  const dim3 g((unsigned)blocks), b(256);
-  cudaError_t e;
-  if (dtype == TFORGE_F32)
-    e = launch_dependent(copy_rows_kernel<float, __nv_bfloat16>, g, b, st, static_cast<const float *>(o.p), o.ld,
-                         static_cast<__nv_bfloat16 *>(q), ldd, o.rows, o.cols);
-  else if (dtype == TFORGE_BF16)
-    e = launch_dependent(copy_rows_kernel<uint16_t, uint16_t>, g, b, st, static_cast<const uint16_t *>(o.p), o.ld,
-                         static_cast<uint16_t *>(q), ldd, o.rows, o.cols);
-  else
-    e = launch_dependent(copy_rows_kernel<uint8_t, uint8_t>, g, b, st, static_cast<const uint8_t *>(o.p), o.ld,
-                         static_cast<uint8_t *>(q), ldd, o.rows, o.cols);
-  if (e != cudaSuccess) return cuda_failure(e, "operand copy");
-  o.p = q;
-  o.ld = ldd;
-  return TFORGE_OK;
-}
+// The operand copies of one call (at most two).
+class Copies {
+ public:
+  // Notes the copy that `o` needs, if any, and asks for its place.
+  void add(Operand &o, int dtype, Scratch &scratch) {
+    const int esz = dtype == TFORGE_E4M3 ? 1 : 2;
+    if (o.rows == 0 || o.cols == 0) return;
+    if (dtype != TFORGE_F32 && at(o.p, 16) && o.ld * esz % 16 == 0) return;
+    const int64_t ldd = padded(o.cols, esz);
+    offset_[n_] = scratch.want((uint64_t)o.rows * ldd * esz);
+    job_[n_] = {o.p, nullptr, o.rows, o.cols, o.ld, ldd, dtype};
+    operand_[n_++] = &o;
+  }
+  // After scratch.take(): launches the copies and points the operands at them.
+  int run(const Scratch &scratch, cudaStream_t st) {
+    if (!n_) return TFORGE_OK;
+    int64_t blocks[2] = {0, 0};
+    for (int i = 0; i < n_; ++i) {
+      job_[i].dst = scratch.at(offset_[i]);
+      operand_[i]->p = job_[i].dst;
+      operand_[i]->ld = job_[i].ldd;
+      blocks[i] = (job_[i].rows * ((job_[i].cols + 7) / 8) + 255) / 256;
+    }
+    // Up to 16 blocks an SM, shared by the groups that each operand has.
+    const int64_t most = 148 * 16, total = blocks[0] + blocks[1];
+    if (total > most) {
+      blocks[0] = std::max<int64_t>(1, most * blocks[0] / total);
+      if (blocks[1]) blocks[1] = std::max<int64_t>(1, most - blocks[0]);
+    }
+    cudaError_t e = launch_dependent(copy_rows_kernel, dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), st, job_[0],
+                                     job_[n_ - 1], (int)blocks[0]);
+    return e == cudaSuccess ? TFORGE_OK : cuda_failure(e, "operand copy");
+  }
+
+ private:
+  int n_ = 0;
+  uint64_t offset_[2];
+  RowCopy job_[2];
+  Operand *operand_[2];
+};
 
 // ---- the products ---------------------------------------------------------------------------------
 
@@ -248,63 +288,61 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
 // ---- the gradient's elementwise pass ---------------------------------------------------------------
 
 // dz = dout * act'(pre) rounded to bf16 (dz null: not written), and part[b, n] = the f32 sum of the
-// unrounded dz over row block b (part null: not wanted).  A block takes 256 columns (a lane eight:
-// neighbouring ones with VEC, else 32 apart) and its 8 warps every 8th row of row block blockIdx.y.
-// Bound by HBM: reads 2 and writes 1 value an element.
+// unrounded dz over row block b (part null: not wanted).  A warp takes 256 columns (a lane eight:
+// neighbouring ones with VEC, else 32 apart); `across` of a block's eight warps lie side by side, so
+// that wide rows are read 4 KB at a time, and the others take every (8 / across)-th row of row
+// block blockIdx.y.  Bound by HBM (reads two values and writes one an element) and the slope's
+// arithmetic: 8192 x 16384 bf16.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-    activation_grad_kernel(int act, const T *__restrict__ dout, int64_t lddo, const T *__restrict__ pre, int64_t ldp,
-                           __nv_bfloat16 *__restrict__ dz, int64_t ldz, float *__restrict__ part, int64_t M, int64_t N) {
+    activation_grad_kernel(int act, int across, const T *__restrict__ dout, int64_t lddo, const T *__restrict__ pre,
+                           int64_t ldp, __nv_bfloat16 *__restrict__ dz, int64_t ldz, float *__restrict__ part, int64_t M,
+                           int64_t N) {
   grid_dependency_wait();
   grid_launch_dependents();
   __shared__ float sm[8][256];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c0 = (int64_t)blockIdx.x * 256;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, deep = 8 / across;
+  const int64_t c0 = ((int64_t)blockIdx.x * across + warp % across) * 256;
   const int64_t per = (M + gridDim.y - 1) / gridDim.y, r0 = per * blockIdx.y, r1 = r0 + per < M ? r0 + per : M;
   auto off = [&](int j) { return VEC ? lane * 8 + j : j * 32 + lane; };
   float sum[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) sum[j] = 0.f;
-  auto read = [&](const T *row, float (&v)[8]) {
+  struct Raw {
+    std::conditional_t<VEC, uint4, T> v[VEC ? (int)sizeof(T) / 2 : 8];
+  };
+  auto read = [&](const T *row, Raw &q) {
     if constexpr (VEC) {
-      const bool in = c0 + lane * 8 < N;
-      if constexpr (sizeof(T) == 2) {
-        const uint4 u = in ? __ldg(reinterpret_cast<const uint4 *>(row + c0 + lane * 8)) : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[2 * j] = __uint_as_float(w[j] << 16);
-          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 f = in ? __ldg(reinterpret_cast<const float4 *>(row + c0 + lane * 8) + h) : make_float4(0, 0, 0, 0);
-          v[4 * h] = f.x;
-          v[4 * h + 1] = f.y;
-          v[4 * h + 2] = f.z;
-          v[4 * h + 3] = f.w;
-        }
-      }
+      for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+        q.v[h] = c0 + lane * 8 < N ? __ldg(reinterpret_cast<const uint4 *>(row + c0 + lane * 8) + h) : make_uint4(0, 0, 0, 0);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c0 + off(j) < N ? (float)row[c0 + off(j)] : 0.f;
+      for (int j = 0; j < 8; ++j) q.v[j] = c0 + off(j) < N ? row[c0 + off(j)] : T(0.f);
+    }
+  };
+  auto value = [&](const Raw &q, int j) -> float {
+    if constexpr (!VEC) {
+      return (float)q.v[j];
+    } else {
+      constexpr int per16 = 16 / (int)sizeof(T);
+      const uint4 &u = q.v[j / per16];
+      const int k = j % per16 * (int)sizeof(T) / 4;
+      const uint32_t w = k == 0 ? u.x : k == 1 ? u.y : k == 2 ? u.z : u.w;
+      if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+      else return __uint_as_float(j % 2 ? w & 0xFFFF0000u : w << 16);
     }
   };
   with_activation(act, [&](auto a) {
     constexpr int ACT = decltype(a)::value;
-#pragma unroll 2
-    for (int64_t m = r0 + warp; m < r1; m += 8) {
+    auto finish = [&](int64_t m, const Raw &d, const Raw &z) {
       float g[8];
-      read(dout + m * lddo, g);
-      if constexpr (ACT != TFORGE_ACT_NONE) {
-        float z[8];
-        read(pre + m * ldp, z);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] *= activate_slope<ACT>(z[j]);
+      for (int j = 0; j < 8; ++j) {
+        g[j] = value(d, j);
+        if constexpr (ACT != TFORGE_ACT_NONE) g[j] *= activate_slope<ACT>(value(z, j));
+        sum[j] += g[j];
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum[j] += g[j];
       if (dz) {
         if constexpr (VEC) {
           if (c0 + lane * 8 < N)
@@ -316,37 +354,74 @@ __global__ void __launch_bounds__(256)
             if (c0 + off(j) < N) dz[m * ldz + c0 + off(j)] = __float2bfloat16_rn(g[j]);
         }
       }
+    };
+    // Two rows' loads in flight.
+    int64_t m = r0 + warp / across;
+    for (; m + deep < r1; m += 2 * deep) {
+      Raw d[2], z[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        read(dout + (m + i * deep) * lddo, d[i]);
+        if constexpr (ACT != TFORGE_ACT_NONE) read(pre + (m + i * deep) * ldp, z[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) finish(m + i * deep, d[i], z[i]);
+    }
+    if (m < r1) {
+      Raw d, z;
+      read(dout + m * lddo, d);
+      if constexpr (ACT != TFORGE_ACT_NONE) read(pre + m * ldp, z);
+      finish(m, d, z);
     }
   });
   if (!part) return;
+  float *row = part + (int64_t)blockIdx.y * N;
+  if (deep == 1) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c0 + off(j) < N) row[c0 + off(j)] = sum[j];
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) sm[warp][off(j)] = sum[j];
   __syncthreads();
-  float v = 0.f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) v += sm[w][threadIdx.x];
-  const int64_t c = c0 + threadIdx.x;
-  if (c < N) part[(int64_t)blockIdx.y * N + c] = v;
+  for (int i = threadIdx.x; i < across * 256; i += 256) {
+    float v = 0.f;
+    for (int w = 0; w < deep; ++w) v += sm[w * across + i / 256][i % 256];
+    const int64_t c = (int64_t)blockIdx.x * across * 256 + i;
+    if (c < N) row[c] = v;
+  }
+}
+
+// Warps side by side: as many of eight as the columns fill.
+int grad_across(int64_t N) {
+  int a = 1;
+  while (a < 8 && a * 256 < N) a *= 2;
+  return a;
+}
+// Row blocks: up to 16 blocks an SM in all (several rounds of resident ones, so that the last is a
+// small part), each of at least 32 rows, so that the block sums are a few percent of what is read --
+// or fewer rows while there are fewer blocks than would fill the SMs once, down to 8.
+int grad_row_blocks(int64_t M, int64_t N) {
+  const int across = grad_across(N);
+  const int64_t cols = (N + 256 * across - 1) / (256 * across);
+  int64_t rows = 32;
+  while (rows > 8 && (M + rows - 1) / rows * cols < 148 * 4) rows /= 2;
+  int64_t r = 148 * 16 / cols;
+  if (r > (M + rows - 1) / rows) r = (M + rows - 1) / rows;
+  return r < 1 ? 1 : (int)r;
 }
 
 template <typename T>
 cudaError_t launch_activation_grad(int act, const void *dout, int64_t lddo, const void *pre, int64_t ldp, void *dz,
                                    int64_t ldz, float *part, int row_blocks, int64_t M, int64_t N, cudaStream_t st) {
-  const int e = sizeof(T);
+  const int e = sizeof(T), across = grad_across(N);
   const bool vec = N % 8 == 0 && at(dout, 16) && lddo * e % 16 == 0 &&
                    (act == TFORGE_ACT_NONE || (at(pre, 16) && ldp * e % 16 == 0));
-  const dim3 g((unsigned)((N + 255) / 256), (unsigned)row_blocks);
+  const dim3 g((unsigned)((N + 256 * across - 1) / (256 * across)), (unsigned)row_blocks);
   auto kern = vec ? activation_grad_kernel<T, true> : activation_grad_kernel<T, false>;
-  return launch_dependent(kern, g, dim3(256), st, act, static_cast<const T *>(dout), lddo, static_cast<const T *>(pre), ldp,
-                          static_cast<__nv_bfloat16 *>(dz), ldz, part, M, N);
-}
-
-// Row blocks: about eight blocks an SM in all, each of at least 32 rows.
-int grad_row_blocks(int64_t M, int64_t N) {
-  const int64_t cols = (N + 255) / 256;
-  int64_t r = 148 * 8 / cols;
-  if (r > (M + 31) / 32) r = (M + 31) / 32;
-  return r < 1 ? 1 : (int)r;
+  return launch_dependent(kern, g, dim3(256), st, act, across, static_cast<const T *>(dout), lddo, static_cast<const T *>(pre),
+                          ldp, static_cast<__nv_bfloat16 *>(dz), ldz, part, M, N);
 }
 
 int check_linear_types(int act, int trans_b, int a_dtype, int b_dtype) {
@@ -384,8 +459,11 @@ int tforge_linear(const tforge_linear_args *args, void *stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Scratch scratch(st);
   Operand A{a.A, a.M, a.K, a.lda}, B{a.B, brows, bcols, a.ldb};
-  rc = prepare_operand(A, a.a_dtype, scratch, st);
-  if (!rc) rc = prepare_operand(B, a.b_dtype, scratch, st);
+  Copies copies;
+  copies.add(A, a.a_dtype, scratch);
+  copies.add(B, a.b_dtype, scratch);
+  rc = scratch.take();
+  if (!rc) rc = copies.run(scratch, st);
   if (rc) return rc;
   LinearParams p{};
   p.bias = a.bias;
@@ -430,27 +508,30 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Scratch scratch(st);
   // dz and the column sums, unless dout serves as it is.
-  Operand dz{a.dout, a.M, a.N, a.lddo};
+  Operand dz{a.dout, a.M, a.N, a.lddo}, A{a.A, a.M, a.K, a.lda}, B{a.B, brows, bcols, a.ldb};
   const bool need_dz = some && (want_a || want_b) &&
                        (a.activation != TFORGE_ACT_NONE || a.dtype == TFORGE_F32 || !at(a.dout, 16) || a.lddo % 8);
+  const int rb = some ? grad_row_blocks(a.M, a.N) : 1;
+  Copies copies;
+  if (some && want_a) copies.add(B, a.b_dtype, scratch);
+  if (some && want_b) copies.add(A, a.a_dtype, scratch);
+  const uint64_t z_at = need_dz ? scratch.want((uint64_t)a.M * padded(a.N, 2) * 2) : 0;
+  const uint64_t part_at = some && want_bias && rb > 1 ? scratch.want((uint64_t)rb * a.N * 4) : 0;
+  rc = scratch.take();
+  if (!rc) rc = copies.run(scratch, st);
+  if (rc) return rc;
+  if (need_dz) {
+    dz.p = scratch.at(z_at);
+    dz.ld = padded(a.N, 2);
+  }
   if (some && (need_dz || want_bias)) {
-    void *z = nullptr, *part = nullptr;
-    const int rb = grad_row_blocks(a.M, a.N);
-    if (need_dz) {
-      dz.ld = padded(a.N, 2);
-      rc = scratch.get(&z, (uint64_t)a.M * dz.ld * 2);
-      if (rc) return rc;
-      dz.p = z;
-    }
-    if (want_bias && rb > 1) {
-      rc = scratch.get(&part, (uint64_t)rb * a.N * 4);
-      if (rc) return rc;
-    }
-    float *sums = want_bias ? (rb > 1 ? static_cast<float *>(part) : a.dbias) : nullptr;
+    void *z = need_dz ? const_cast<void *>(dz.p) : nullptr;
+    float *part = want_bias && rb > 1 ? reinterpret_cast<float *>(scratch.at(part_at)) : nullptr;
+    float *sums = part ? part : (want_bias ? a.dbias : nullptr);
     cudaError_t e = a.dtype == TFORGE_BF16
                         ? launch_activation_grad<__nv_bfloat16>(a.activation, a.dout, a.lddo, a.pre, a.ldp, z, dz.ld, sums, rb, a.M, a.N, st)
                         : launch_activation_grad<float>(a.activation, a.dout, a.lddo, a.pre, a.ldp, z, dz.ld, sums, rb, a.M, a.N, st);
-    if (e == cudaSuccess && part) e = launch_column_sum(static_cast<const float *>(part), rb, a.N, a.dbias, st);
+    if (e == cudaSuccess && part) e = launch_column_sum(part, rb, a.N, a.dbias, st);
     if (e != cudaSuccess) return cuda_failure(e, "activation gradient");
   } else if (want_bias) {
     cudaError_t e = cudaMemsetAsync(a.dbias, 0, (size_t)a.N * 4, st);
@@ -460,18 +541,12 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
   p.act = TFORGE_ACT_NONE;
   p.out_bf16 = a.grad_dtype == TFORGE_BF16;
   if (want_a) {
-    Operand B{a.B, brows, bcols, a.ldb};
-    if (some) rc = prepare_operand(B, a.b_dtype, scratch, st);
-    if (rc) return rc;
     p.out = a.dA;
     p.ldo = a.ldda;
     rc = product(dz, false, B, a.trans_b != 0, false, a.M, a.K, a.N, p, st);
     if (rc) return rc;
   }
   if (want_b) {
-    Operand A{a.A, a.M, a.K, a.lda};
-    if (some) rc = prepare_operand(A, a.a_dtype, scratch, st);
-    if (rc) return rc;
     p.out = a.dB;
     p.ldo = a.lddb;
     rc = a.trans_b ? product(dz, true, A, true, false, a.N, a.K, a.M, p, st)
@@ -558,14 +633,14 @@ int tforge_rms_norm_backward(const tforge_rms_norm_backward_args *args, void *st
   p.w_bf16 = a.weight_dtype == TFORGE_BF16;
   const int parts = rms_norm_bwd_blocks(p);
   Scratch scratch(st);
-  void *part = nullptr;
-  if (a.dweight && parts > 1) {
-    rc = scratch.get(&part, (uint64_t)parts * a.N * 4);
-    if (rc) return rc;
-  }
-  float *sums = a.dweight ? (parts > 1 ? static_cast<float *>(part) : a.dweight) : nullptr;
+  const bool join = a.dweight && parts > 1;
+  const uint64_t part_at = join ? scratch.want((uint64_t)parts * a.N * 4) : 0;
+  rc = scratch.take();
+  if (rc) return rc;
+  float *part = join ? reinterpret_cast<float *>(scratch.at(part_at)) : nullptr;
+  float *sums = part ? part : a.dweight;
   cudaError_t err = launch_rms_norm_bwd(p, sums, parts, st);
-  if (err == cudaSuccess && part) err = launch_column_sum(static_cast<const float *>(part), parts, a.N, a.dweight, st);
+  if (err == cudaSuccess && part) err = launch_column_sum(part, parts, a.N, a.dweight, st);
   return err == cudaSuccess ? TFORGE_OK : cuda_failure(err, "rms_norm_backward launch");
 }
 
