@@ -606,8 +606,8 @@ int encode_rows_map(CUtensorMap *m, const void *base, int esz, int64_t rows, int
   return TFORGE_OK;
 }
 
-int encode_out_map(CUtensorMap *m, void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld) {
-  return make_tmap(m, base, bf16, rows, cols, ld, 32, 128, bf16 ? SW64 : SW128);
+int encode_out_map(CUtensorMap *m, const void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld) {
+  return make_tmap(m, base, bf16, rows, cols, ld, 32, 32, bf16 ? SW64 : SW128);
 }
 
 int device_pool(cudaMemPool_t *out) { return scratch_pool(out); }

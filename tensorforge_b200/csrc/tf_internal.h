@@ -212,11 +212,12 @@ cudaError_t launch_linear_slim(bool f8, bool w_mn, bool t_mn, int bt, const CUte
                                const LinearParams &p, cudaStream_t stream);
 
 // Persistent CTA pairs on 256 x 256 tiles, K > 0.  tmA / tmB: as tmT / tmW above with 128 rows a
-// box.  tmO / tmP: maps of out and pre (encode_out_map), read when p.vec.
+// box.  tmO / tmP / tmR: maps of out, pre and the residual (encode_out_map), read when p.vec.
 cudaError_t launch_linear_pair(bool f8, bool a_mn, bool b_mn, const CUtensorMap &tmA, const CUtensorMap &tmB,
-                               const CUtensorMap &tmO, const CUtensorMap &tmP, const LinearParams &p, cudaStream_t stream);
-// Output map: boxes of 32 columns x 128 rows, f32 in the 128-byte or bf16 in the 64-byte swizzle.
-int encode_out_map(CUtensorMap *m, void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld);
+                               const CUtensorMap &tmO, const CUtensorMap &tmP, const CUtensorMap &tmR, const LinearParams &p,
+                               cudaStream_t stream);
+// Output map: boxes of 32 columns x 32 rows, f32 in the 128-byte or bf16 in the 64-byte swizzle.
+int encode_out_map(CUtensorMap *m, const void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld);
 
 // tforge_rms_norm / tforge_quantize_e4m3 with every pitch filled in (tf_norm.cu).
 struct NormArgs {

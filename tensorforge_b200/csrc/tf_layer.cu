@@ -260,14 +260,15 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
   else if ((force & 255) == 2) c = Choice{0, 1};
   if ((c.tile == 0 && K == 0) || (c.tile != 0 && t_mn && c.tile < 64)) return TFORGE_ERR_UNSUPPORTED;
   if (c.tile == 0) {
-    CUtensorMap tmA{}, tmB{}, tmO{}, tmP{};
+    CUtensorMap tmA{}, tmB{}, tmO{}, tmP{}, tmR{};
     const uint32_t bk = 128 / esz;
     rc = t_mn ? encode_rows_map(&tmA, rows.p, esz, K, M, rows.ld, 64, 64) : encode_rows_map(&tmA, rows.p, esz, M, K, rows.ld, bk, 128);
     if (!rc) rc = w_mn ? encode_rows_map(&tmB, cols.p, esz, K, N, cols.ld, 64, 64) : encode_rows_map(&tmB, cols.p, esz, N, K, cols.ld, bk, 128);
     if (!rc && p.vec) rc = encode_out_map(&tmO, p.out, p.out_bf16 != 0, M, N, p.ldo);
     if (!rc && p.vec && p.pre) rc = encode_out_map(&tmP, p.pre, p.out_bf16 != 0, M, N, p.ldp);
+    if (!rc && p.vec && p.residual) rc = encode_out_map(&tmR, p.residual, p.res_bf16 != 0, M, N, p.ldr);
     if (rc) return rc;
-    cudaError_t e = launch_linear_pair(f8, t_mn, w_mn, tmA, tmB, tmO, tmP, p, st);
+    cudaError_t e = launch_linear_pair(f8, t_mn, w_mn, tmA, tmB, tmO, tmP, tmR, p, st);
     return e == cudaSuccess ? TFORGE_OK : cuda_failure(e, "linear launch");
   }
   p.splits = c.splits;

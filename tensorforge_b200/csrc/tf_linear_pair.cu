@@ -8,16 +8,20 @@
 // TMEM columns: the pair's MMAs (cta_group::2, 256 x 256, bf16 or e4m3) fill one while the epilogue
 // empties the other.
 //
-// Epilogue: eight warps a CTA in two groups of four, each group every second chunk of 32 columns, so
-// that one group's residual loads and stores overlap the other's arithmetic.  A thread holds 32
-// columns of one row; the row's scale is its own, the columns' bias and scale are a lane's and go
-// round by shuffles.  Outputs whose rows start on 16-byte boundaries leave through swizzled staging
-// boxes and TMA stores, others through the same boxes turned round, a warp storing 32 neighbouring
-// columns of one row at a time.
+// Epilogue: sixteen warps a CTA, each by itself (no barrier between them): 32 rows (its TMEM lanes)
+// and every fourth chunk of 32 columns.  A thread holds 32 columns of one row; the row's scale is its
+// own, the columns' bias and scale are a lane's and go round by shuffles.  Outputs whose rows start on
+// 16-byte boundaries leave through the warp's 4 KB of swizzled staging and TMA stores, others through
+// the same memory turned round, 32 neighbouring columns of one row at a time.  The residual's chunk
+// is brought into the staging by TMA one chunk ahead, so a tile's first while its MMAs run.
 //
-// 384 threads: warp 0 TMA producer (both CTAs), warp 1 MMA issuer (leader), warps 4..11 epilogue.
-// Every wait is bounded (tf_ptx.cuh); after an expiry each role stops, the producer and the issuer
-// wait (bounded) for what they have in flight, and both CTAs meet before TMEM is freed.
+// With few stages of k a tile is bound by this epilogue: 4096 x 8192 x 256 bf16 with silu takes
+// 56 us with eight warps in two groups that meet at barriers, EPI_SILU us as it is here; with the
+// bf16 residual 95 and EPI_RES.
+//
+// 640 threads: warp 0 TMA producer (both CTAs), warp 1 MMA issuer (leader), warps 4..19 epilogue.
+// Every wait is bounded (tf_ptx.cuh); after an expiry each role stops, the producer, the issuer and
+// the epilogue wait (bounded) for what they have in flight, and both CTAs meet before TMEM is freed.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -29,60 +33,78 @@ namespace tf {
 
 namespace {
 
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 5;
+constexpr int kEpiWarps = 16;
 
 struct PairL {
-  static constexpr int kThreads = 384;
+  static constexpr int kThreads = 128 + 32 * kEpiWarps;
   static constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kBoxOff = kPairStages * kStageBytes;
-  static constexpr int kBoxBytes = 128 * 128;  // a group's: 128 rows x 32 f32, or two of 32 bf16
-  static constexpr int kBarOff = kBoxOff + 2 * kBoxBytes;
-  // full[], empty[], accf[2], acce[2], drain; then the TMEM slot, the abort flag, the groups' go words.
-  static constexpr int kNumBars = 2 * kPairStages + 5;
-  static constexpr int kSmemBytes = 1024 + kBarOff + 8 * kNumBars + 32;
+  static constexpr int kBoxBytes = 32 * 128;  // an epilogue warp's: 32 rows x 32 f32, or two of 32 bf16
+  static constexpr int kBarOff = kBoxOff + kEpiWarps * kBoxBytes;
+  // full[], empty[], accf[2], acce[2], drain, resf[warps]; then the TMEM slot and the abort flag.
+  static constexpr int kNumBars = 2 * kPairStages + 5 + kEpiWarps;
+  static constexpr int kSmemBytes = 1024 + kBarOff + 8 * kNumBars + 16;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
-// Columns col .. col + CNT - 1 of one residual row (16-byte aligned groups), 0 beyond N.
-template <int CNT>
-__device__ __forceinline__ void load_residual(const LinearParams &p, int64_t row, int col, float (&v)[CNT]) {
+__device__ __forceinline__ void add_bf16x8(float *v, const uint4 &u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] += __uint_as_float(w[i] << 16);
+    v[2 * i + 1] += __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void add_f32x4(float *v, const float4 &f) {
+  v[0] += f.x;
+  v[1] += f.y;
+  v[2] += f.z;
+  v[3] += f.w;
+}
+
+// Adds row r of a residual box to v (stage_row's layout).
+__device__ __forceinline__ void add_staged(const uint8_t *box, int r, bool bf16, float (&v)[32]) {
+  if (bf16) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) add_bf16x8(v + 8 * u, *reinterpret_cast<const uint4 *>(box + r * 64 + ((u ^ ((r >> 1) & 3)) << 4)));
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) add_f32x4(v + 4 * u, *reinterpret_cast<const float4 *>(box + r * 128 + ((u ^ (r & 7)) << 4)));
+  }
+}
+
+// Adds columns col .. col + 31 of a residual row (16-byte aligned groups), those below N.
+__device__ __forceinline__ void add_row(const LinearParams &p, int64_t row, int col, float (&v)[32]) {
   if (p.res_bf16) {
     const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.residual) + row * p.ldr + col;
 #pragma unroll
-    for (int u = 0; u < CNT / 8; ++u) {
+    for (int u = 0; u < 4; ++u) {
       if (col + 8 * u + 8 <= p.N) {
-        const uint4 q = *reinterpret_cast<const uint4 *>(src + 8 * u);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[8 * u + 2 * i] = __uint_as_float(w[i] << 16);
-          v[8 * u + 2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
+        add_bf16x8(v + 8 * u, *reinterpret_cast<const uint4 *>(src + 8 * u));
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[8 * u + i] = col + 8 * u + i < p.N ? __bfloat162float(src[8 * u + i]) : 0.f;
+        for (int i = 0; i < 8; ++i)
+          if (col + 8 * u + i < p.N) v[8 * u + i] += __bfloat162float(src[8 * u + i]);
       }
     }
   } else {
     const float *src = static_cast<const float *>(p.residual) + row * p.ldr + col;
 #pragma unroll
-    for (int u = 0; u < CNT / 4; ++u) {
+    for (int u = 0; u < 8; ++u) {
       if (col + 4 * u + 4 <= p.N) {
-        const float4 q = *reinterpret_cast<const float4 *>(src + 4 * u);
-        v[4 * u] = q.x;
-        v[4 * u + 1] = q.y;
-        v[4 * u + 2] = q.z;
-        v[4 * u + 3] = q.w;
+        add_f32x4(v + 4 * u, *reinterpret_cast<const float4 *>(src + 4 * u));
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * u + i] = col + 4 * u + i < p.N ? src[4 * u + i] : 0.f;
+        for (int i = 0; i < 4; ++i)
+          if (col + 4 * u + i < p.N) v[4 * u + i] += src[4 * u + i];
       }
     }
   }
 }
 
-// Row r of a staging box: 32 f32 (128-B swizzle) or 32 bf16 (64-B swizzle), as the output maps say.
+// Row r (of 32) of a staging box: 32 f32 (128-B swizzle) or 32 bf16 (64-B swizzle), as the maps say.
 __device__ __forceinline__ void stage_row(uint8_t *box, int r, bool bf16, const float (&v)[32]) {
   if (bf16) {
 #pragma unroll
@@ -98,47 +120,45 @@ __device__ __forceinline__ void stage_row(uint8_t *box, int r, bool bf16, const 
   }
 }
 
-// The residual of a warp's 32 rows x 32 columns, a lane a column: v[l] of row row0 + l.  One load an
-// element, any alignment, all in flight together.
-__device__ __forceinline__ void load_turned(const LinearParams &p, int lane, int64_t row0, int col0, float (&v)[32]) {
-  const int rows = col0 + lane < p.N ? (int)(p.M - row0 < 32 ? p.M - row0 : 32) : 0;
-  const int64_t i = row0 * p.ldr + col0 + lane;
-  if (p.res_bf16) {
-    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.residual) + i;
-#pragma unroll
-    for (int l = 0; l < 32; ++l) v[l] = l < rows ? __bfloat162float(src[l * p.ldr]) : 0.f;
-  } else {
-    const float *src = static_cast<const float *>(p.residual) + i;
-#pragma unroll
-    for (int l = 0; l < 32; ++l) v[l] = l < rows ? src[l * p.ldr] : 0.f;
-  }
-}
-
 // A warp's 32 rows x 32 columns turned round through its own 4 KB (column j of row l at j ^ l) and
-// stored row by row, a lane a column, res[l] added to row l's.
-template <typename T>
-__device__ __forceinline__ void store_turned(float *buf, int lane, int rows, T *dst, int64_t ld, const float (&v)[32],
-                                             const float (&res)[32], bool add) {
+// stored row by row, a lane a column: any alignment.  R: the residual's type (void: none), added on
+// the way, eight rows' loads in flight.
+template <typename T, typename R>
+__device__ __forceinline__ void store_turned(float *buf, int lane, int rows, T *dst, int64_t ld, const R *res, int64_t ldr,
+                                             const float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) buf[lane * 32 + (j ^ lane)] = v[j];
   __syncwarp();
+#pragma unroll 1
+  for (int l0 = 0; l0 < rows; l0 += 8) {
+    float x[8];
 #pragma unroll
-  for (int l = 0; l < 32; ++l) {
-    if (l < rows) {
-      float x = buf[l * 32 + (lane ^ l)];
-      if (add) x += res[l];
-      if constexpr (sizeof(T) == 2) dst[l * ld] = __float2bfloat16_rn(x);
-      else dst[l * ld] = x;
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(R) == 2) x[i] = l0 + i < rows ? __bfloat162float(res[(l0 + i) * ldr]) : 0.f;
+      else if constexpr (sizeof(R) == 4) x[i] = l0 + i < rows ? res[(l0 + i) * ldr] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (l0 + i < rows) {
+        float y = buf[(l0 + i) * 32 + (lane ^ (l0 + i))];
+        if constexpr (sizeof(R) > 1) y += x[i];
+        if constexpr (sizeof(T) == 2) dst[(l0 + i) * ld] = __float2bfloat16_rn(y);
+        else dst[(l0 + i) * ld] = y;
+      }
     }
   }
   __syncwarp();
 }
-__device__ __forceinline__ void store_turned(const LinearParams &p, float *buf, int lane, int64_t row0, int col0, void *base,
-                                             int64_t ld, const float (&v)[32], const float (&res)[32], bool add) {
+struct NoResidual {};
+template <typename T>
+__device__ __forceinline__ void store_turned(const LinearParams &p, float *buf, int lane, int64_t row0, int col0, T *base,
+                                             int64_t ld, bool res, const float (&v)[32]) {
   const int rows = col0 + lane < p.N ? (int)(p.M - row0 < 32 ? p.M - row0 : 32) : 0;
-  const int64_t o = row0 * ld + col0 + lane;
-  if (p.out_bf16) store_turned(buf, lane, rows, static_cast<__nv_bfloat16 *>(base) + o, ld, v, res, add);
-  else store_turned(buf, lane, rows, static_cast<float *>(base) + o, ld, v, res, add);
+  T *dst = base + row0 * ld + col0 + lane;
+  const int64_t r = row0 * p.ldr + col0 + lane;
+  if (!res) store_turned(buf, lane, rows, dst, ld, static_cast<const NoResidual *>(nullptr), 0, v);
+  else if (p.res_bf16) store_turned(buf, lane, rows, dst, ld, static_cast<const __nv_bfloat16 *>(p.residual) + r, p.ldr, v);
+  else store_turned(buf, lane, rows, dst, ld, static_cast<const float *>(p.residual) + r, p.ldr, v);
 }
 
 // F8: e4m3 operands (both K-major).  AMN / BMN: A / B is MN-major (bf16).
@@ -146,7 +166,7 @@ template <bool F8, bool AMN, bool BMN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmP,
-                       const LinearParams p) {
+                       const __grid_constant__ CUtensorMap tmR, const LinearParams p) {
   using L = PairL;
   constexpr int STAGES = kPairStages;
   static_assert(!F8 || (!AMN && !BMN), "8-bit operands are K-major");
@@ -160,9 +180,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBarOff);
   // full[s] (leader's): both CTAs' bytes of slot s landed; empty[s]: the MMAs reading slot s are done
   // (both CTAs); accf[b]: accumulator b holds a tile (both CTAs); acce[b] (leader's): both CTAs'
-  // epilogues have read accumulator b; drain: MMAs in flight after an abort.
+  // epilogues have read accumulator b; drain: MMAs in flight after an abort; resf[w]: epilogue warp
+  // w's residual box landed.
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * STAGES, accf0 = empty0 + 8 * STAGES, acce0 = accf0 + 16,
-                 drainf = acce0 + 16;
+                 drainf = acce0 + 16, resf0 = drainf + 8;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
   volatile uint32_t *abort_flag = tmem_slot + 1;
   const WaitCtl wc{abort_flag, p.status, p.limit_ns};
@@ -181,9 +202,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(accf0 + 8 * b, 1);
-      mbar_init(acce0 + 8 * b, 16);  // lane 0 of the eight epilogue warps of both CTAs
+      mbar_init(acce0 + 8 * b, 2 * kEpiWarps);  // lane 0 of the epilogue warps of both CTAs
     }
     mbar_init(drainf, 1);
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(resf0 + 8 * w, 1);
     *abort_flag = 0u;
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
@@ -295,50 +317,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
       mbar_wait_drain_cluster(drainf, 0, p.limit_ns);
     }
   } else if (warp >= 4) {
-    // ---------------- epilogue (both CTAs): group g = warps 4 + 4 g .. 7 + 4 g ----------------
-    const int g = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
-    const bool first = r == 0;  // the group's thread that waits and stores
-    const uint32_t bar_a = 1 + 2 * g, bar_b = 2 + 2 * g;
-    const uint32_t lead_acce0 = map_to_cta(acce0, 0);
-    uint8_t *box = smem + L::kBoxOff + g * L::kBoxBytes;
-    volatile uint32_t *go = tmem_slot + 2 + 2 * g;  // by the tile's parity: a warp may lag one tile
-    const bool bf16 = p.out_bf16 != 0, pre = p.pre != nullptr, pingpong = bf16 && !pre;
-    uint32_t turn = 0;
-#pragma unroll 1
-    for (int i = 0; i < my_tiles; ++i) {
-      const int b = i & 1;
+    // ---------------- epilogue (both CTAs): warps 4..19 ----------------
+    // TMEM lanes 32 q .. + 31, chunks part and part + 4 of a tile's eight.
+    const int part = (warp - 4) >> 2, q = warp & 3;
+    const uint32_t lead_acce0 = map_to_cta(acce0, 0), resf = resf0 + 8 * (warp - 4);
+    uint8_t *box = smem + L::kBoxOff + (warp - 4) * L::kBoxBytes;
+    const bool bf16 = p.out_bf16 != 0, pre = p.pre != nullptr, pingpong = bf16 && !pre && !p.residual;
+    // The residual comes by TMA into the box, in whose place the chunk's output is then staged, but
+    // where pre needs the box first (f32 out or residual with pre): then by the row's own loads.
+    const bool res_tma = p.residual && p.vec && !(pre && (!bf16 || !p.res_bf16));
+    const uint32_t res_bytes = p.res_bf16 ? 2048u : 4096u;
+    uint32_t turn = 0, res_phase = 0;
+    bool res_flight = false;
+    auto tile_at = [&](int i, int &m0, int &n0) {
       int tm, tn;
       raster_tile(pair + i * npairs, tiles_m, tiles_n, kRasterGroup, tm, tn);
-      const int m0 = tm * 256 + (int)rank * 128, n0 = tn * 256;
-      const int64_t row = m0 + r;
-      const bool row_ok = row < p.M;
-      const float sa = p.a_scale && row_ok ? __ldg(p.a_scale + row) : 1.f;
-      // One thread waits (bounded) and publishes the outcome: the group's four warps take the same
-      // branch, and no named barrier below waits for a warp that gave up.
-      if (first) go[b] = mbar_wait_cluster(accf0 + 8 * b, (i >> 1) & 1, wc, 128) ? 1u : 0u;
-      named_barrier(bar_a, 128);
-      if (!go[b]) break;
-      tc_fence_after();
-      const uint32_t tacc = tmem + 256u * b + ((uint32_t)(q * 32) << 16);
+      m0 = tm * 256 + (int)rank * 128 + q * 32;  // this warp's first row
+      n0 = tn * 256;
+    };
+    auto inside = [&](int m0, int col0) { return m0 < p.M && col0 < p.N; };  // the same for the whole warp
+    // Starts the residual's way into the box, once the stores from it have read it.
+    auto fetch_residual = [&](int m0, int col0) {
+      if (!res_tma || !inside(m0, col0)) return;
+      if (lane == 0) {
+        bulk_wait_group_read0();
+        mbar_arrive_expect_tx(resf, res_bytes);
+        tma_load_2d(smem_u32(box), &tmR, col0, m0, resf);
+      }
+      res_flight = true;
+    };
+    int m0 = 0, n0 = 0;
+    if (my_tiles > 0) {
+      tile_at(0, m0, n0);
+      fetch_residual(m0, n0 + 32 * part);
+    }
+    bool ok = true;
 #pragma unroll 1
-      for (int c = g; c < 8; c += 2) {
-        const int col0 = n0 + c * 32;
-        if (m0 >= p.M || col0 >= p.N) break;  // the same for the whole group
-        uint32_t rr[32];
-        tmem_ld_32x32b_x32(tacc + c * 32, rr);
-        const bool lane_col = col0 + lane < p.N;
+    for (int i = 0; i < my_tiles && ok; ++i) {
+      const int b = i & 1;
+      const float sa = p.a_scale && m0 + lane < p.M ? __ldg(p.a_scale + m0 + lane) : 1.f;
+      int m1 = 0, n1 = 0;  // the next tile
+      if (i + 1 < my_tiles) tile_at(i + 1, m1, n1);
+      // Not unrolled: the body, with an activation's 32 copies, should stay in the instruction cache.
+#pragma unroll 1
+      for (int k = 0; k < 2; ++k) {
+        const int c = part + 4 * k, col0 = n0 + 32 * c;
+        const bool live = inside(m0, col0), lane_col = live && col0 + lane < p.N;
         const float bl = p.bias && lane_col ? __ldg(p.bias + col0 + lane) : 0.f;
         const float sl = p.b_scale && lane_col ? __ldg(p.b_scale + col0 + lane) : 1.f;
-        float res[32];
-        if (p.residual && p.vec && row_ok) {
-          load_residual(p, row, col0, res);
-        } else if (p.residual && !p.vec) {
-          load_turned(p, lane, m0 + q * 32, col0, res);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) res[j] = 0.f;
+        if (k == 0) {
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(accf0 + 8 * b, (i >> 1) & 1, wc, 64));
+          if (!ok) break;
+          tc_fence_after();
         }
-        tmem_ld_wait(rr);
+        uint32_t rr[32];
+        if (live) {
+          tmem_ld_32x32b_x32(tmem + 256u * b + ((uint32_t)(q * 32) << 16) + c * 32, rr);
+          tmem_ld_wait(rr);
+        }
+        if (k == 1) {  // this warp's last read of accumulator b is done: release it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(lead_acce0 + 8 * b);
+        }
+        if (!live) continue;
         float v[32];
         if constexpr (F8) {
 #pragma unroll
@@ -348,62 +390,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rr[j]) + __shfl_sync(0xFFFFFFFFu, bl, j);
         }
-        if (!p.vec) {
-          float *buf = reinterpret_cast<float *>(box) + q * 1024;
-          const int64_t row0 = m0 + q * 32;
-          if (pre) store_turned(p, buf, lane, row0, col0, p.pre, p.ldp, v, res, false);
-          with_activation(p.act, [&](auto act) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = activate<decltype(act)::value>(v[j]);
-          });
-          store_turned(p, buf, lane, row0, col0, p.out, p.ldo, v, res, p.residual != nullptr);
-          continue;
+        if (p.vec && !res_tma) {
+          // The box is free once the stores issued from it have read it: all but the last one when it
+          // has two bf16 halves to alternate between.
+          if (lane == 0) {
+            if (pingpong) bulk_wait_group_read1();
+            else bulk_wait_group_read0();
+          }
+          __syncwarp();
         }
-        // The boxes are free once the stores issued from them have read them: all but the last one
-        // when the bf16 box has two halves to alternate between.
-        if (first) {
-          if (pingpong) bulk_wait_group_read1();
-          else bulk_wait_group_read0();
-        }
-        named_barrier(bar_a, 128);
-        uint8_t *obox = pingpong ? box + (turn & 1) * 8192 : (bf16 && pre ? box + 8192 : box);
-        ++turn;
         if (pre) {
-          stage_row(box, r, bf16, v);
-          if (!bf16) {  // f32: the box holds one tile at a time
+          if (!p.vec) {
+            float *buf = reinterpret_cast<float *>(box);
+            if (bf16) store_turned(p, buf, lane, m0, col0, static_cast<__nv_bfloat16 *>(p.pre), p.ldp, false, v);
+            else store_turned(p, buf, lane, m0, col0, static_cast<float *>(p.pre), p.ldp, false, v);
+          } else {
+            stage_row(bf16 ? box + 2048 : box, lane, bf16, v);
             fence_proxy_async_smem();
-            named_barrier(bar_b, 128);
-            if (first) {
-              tma_store_2d(&tmP, smem_u32(box), col0, m0);
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmP, smem_u32(bf16 ? box + 2048 : box), col0, m0);
               bulk_commit_group();
-              bulk_wait_group_read0();
+              if (!bf16) bulk_wait_group_read0();  // f32: the box holds one chunk at a time
             }
-            named_barrier(bar_a, 128);
+            __syncwarp();
           }
         }
         with_activation(p.act, [&](auto act) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = activate<decltype(act)::value>(v[j]);
         });
-        if (p.residual) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += res[j];
+        if (!p.vec) {
+          float *buf = reinterpret_cast<float *>(box);
+          if (bf16) store_turned(p, buf, lane, m0, col0, static_cast<__nv_bfloat16 *>(p.out), p.ldo, p.residual != nullptr, v);
+          else store_turned(p, buf, lane, m0, col0, static_cast<float *>(p.out), p.ldo, p.residual != nullptr, v);
+          continue;
         }
-        stage_row(obox, r, bf16, v);
+        if (res_tma) {
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(resf, res_phase, wc));
+          if (!ok) break;
+          res_phase ^= 1u;
+          res_flight = false;
+          add_staged(box, lane, p.res_bf16 != 0, v);
+          __syncwarp();  // every row has been read before the output takes its place
+        } else if (p.residual && m0 + lane < p.M) {
+          add_row(p, m0 + lane, col0, v);
+        }
+        uint8_t *obox = pingpong && (turn & 1) ? box + 2048 : box;
+        ++turn;
+        stage_row(obox, lane, bf16, v);
         fence_proxy_async_smem();
-        named_barrier(bar_b, 128);
-        if (first) {
-          if (pre && bf16) tma_store_2d(&tmP, smem_u32(box), col0, m0);
+        __syncwarp();
+        if (lane == 0) {
           tma_store_2d(&tmO, smem_u32(obox), col0, m0);
           bulk_commit_group();
         }
+        if (k == 0) fetch_residual(m0, col0 + 128);
       }
-      // Every tcgen05.ld of accumulator b has completed (tmem_ld_wait): release it.
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(lead_acce0 + 8 * b);
+      m0 = m1;
+      n0 = n1;
+      if (ok && i + 1 < my_tiles && !res_flight) fetch_residual(m0, n0 + 32 * part);
     }
-    if (first) bulk_wait_group_read0();  // staging stays valid until read
+    if (lane == 0) {
+      if (res_flight) mbar_wait_drain(resf, res_phase, p.limit_ns);  // after an abort
+      bulk_wait_group_read0();  // staging stays valid until read
+    }
   }
 
   tc_fence_before();
@@ -449,7 +500,7 @@ int pair_clusters() {
 
 template <bool F8, bool AMN, bool BMN>
 cudaError_t launch_pair(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmO, const CUtensorMap &tmP,
-                        const LinearParams &p, cudaStream_t st) {
+                        const CUtensorMap &tmR, const LinearParams &p, cudaStream_t st) {
   const int clusters = pair_clusters<F8, AMN, BMN>();
   if (clusters <= 0) return cudaErrorInvalidConfiguration;
   const int64_t tiles = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
@@ -458,18 +509,19 @@ cudaError_t launch_pair(const CUtensorMap &tmA, const CUtensorMap &tmB, const CU
   cudaLaunchAttribute attr[1];
   pdl_attr(attr[0]);
   cudaLaunchConfig_t cfg = {dim3(2 * pairs), dim3(PairL::kThreads), (size_t)PairL::kSmemBytes, st, attr, 1};
-  return cudaLaunchKernelEx(&cfg, linear_pair_kernel<F8, AMN, BMN>, tmA, tmB, tmO, tmP, p);
+  return cudaLaunchKernelEx(&cfg, linear_pair_kernel<F8, AMN, BMN>, tmA, tmB, tmO, tmP, tmR, p);
 }
 
 }  // namespace
 
 cudaError_t launch_linear_pair(bool f8, bool a_mn, bool b_mn, const CUtensorMap &tmA, const CUtensorMap &tmB,
-                               const CUtensorMap &tmO, const CUtensorMap &tmP, const LinearParams &p, cudaStream_t st) {
+                               const CUtensorMap &tmO, const CUtensorMap &tmP, const CUtensorMap &tmR, const LinearParams &p,
+                               cudaStream_t st) {
   if (p.K <= 0 || (f8 && (a_mn || b_mn)) || (a_mn && !b_mn)) return cudaErrorInvalidValue;
-  if (f8) return launch_pair<true, false, false>(tmA, tmB, tmO, tmP, p, st);
-  if (a_mn) return launch_pair<false, true, true>(tmA, tmB, tmO, tmP, p, st);
-  return b_mn ? launch_pair<false, false, true>(tmA, tmB, tmO, tmP, p, st)
-              : launch_pair<false, false, false>(tmA, tmB, tmO, tmP, p, st);
+  if (f8) return launch_pair<true, false, false>(tmA, tmB, tmO, tmP, tmR, p, st);
+  if (a_mn) return launch_pair<false, true, true>(tmA, tmB, tmO, tmP, tmR, p, st);
+  return b_mn ? launch_pair<false, false, true>(tmA, tmB, tmO, tmP, tmR, p, st)
+              : launch_pair<false, false, false>(tmA, tmB, tmO, tmP, tmR, p, st);
 }
 
 }  // namespace tf
