@@ -112,23 +112,59 @@ struct RowCopy {
   int32_t dtype;
 };
 
-// Eight elements of a row that may start anywhere, into rows on 16-byte boundaries: single loads, one
-// store; what lies beyond a row's end within the last group is written as 0.
-template <typename S, typename D>
+// Sixteen bytes of the copy a thread.  The source row may start anywhere: 8- and 16-bit elements are
+// read as the aligned words around them and shifted into place, element by element only where a word
+// would reach outside the array.  What a row's last group holds beyond its end is not read by anyone.
+template <int ESZ>
 __device__ __forceinline__ void copy_groups(const RowCopy &j, int64_t first, int64_t step) {
+  constexpr int kPer = 16 / ESZ;
+  const int64_t groups = (j.cols + kPer - 1) / kPer, total = j.rows * groups;
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(j.src), end = begin + ((j.rows - 1) * j.lds + j.cols) * ESZ;
+  for (int64_t i = first; i < total; i += step) {
+    const int64_t r = i / groups, c = (i - r * groups) * kPer;
+    const uintptr_t at = begin + (uintptr_t)((r * j.lds + c) * ESZ), word = at & ~uintptr_t(3);
+    const uint32_t shift = 8u * (uint32_t)(at & 3);
+    uint32_t w[5] = {0, 0, 0, 0, 0};
+    if (word >= begin && word + (shift ? 20 : 16) <= end) {
+      const uint32_t *src = reinterpret_cast<const uint32_t *>(word);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = __ldg(src + k);
+      if (shift) {
+        w[4] = __ldg(src + 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], shift);
+      }
+    } else {
+      const int live = j.cols - c < kPer ? (int)(j.cols - c) : kPer;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        if (k < live) {
+          const uint32_t v = ESZ == 1 ? reinterpret_cast<const uint8_t *>(at)[k] : reinterpret_cast<const uint16_t *>(at)[k];
+          w[k * ESZ / 4] |= v << (8 * (k * ESZ % 4));
+        }
+      }
+    }
+    *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(j.dst) + (r * j.ldd + c) * ESZ) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+// f32 to bf16, eight elements a thread.
+__device__ __forceinline__ void convert_groups(const RowCopy &j, int64_t first, int64_t step) {
   const int64_t groups = (j.cols + 7) / 8, total = j.rows * groups;
+  const bool vec = (reinterpret_cast<uintptr_t>(j.src) & 15) == 0 && j.lds % 4 == 0;
   for (int64_t i = first; i < total; i += step) {
     const int64_t r = i / groups, c = (i - r * groups) * 8;
-    const S *s = static_cast<const S *>(j.src) + r * j.lds + c;
-    __align__(16) D v[8];
+    const float *s = static_cast<const float *>(j.src) + r * j.lds + c;
+    float v[8];
+    if (vec && c + 8 <= j.cols) {
+      const float4 a = __ldg(reinterpret_cast<const float4 *>(s)), b = __ldg(reinterpret_cast<const float4 *>(s) + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if constexpr (std::is_same<S, float>::value) v[k] = __float2bfloat16_rn(c + k < j.cols ? s[k] : 0.f);
-      else v[k] = c + k < j.cols ? s[k] : D{};
+      for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? __ldg(s + k) : 0.f;
     }
-    D *d = static_cast<D *>(j.dst) + r * j.ldd + c;
-    if constexpr (sizeof(D) == 2) *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(v);
-    else *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<const uint2 *>(v);
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(j.dst) + r * j.ldd + c) =
+        make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
   }
 }
 
@@ -140,9 +176,9 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const RowCopy a, const R
   const RowCopy &j = second ? b : a;
   const int64_t block = second ? blockIdx.x - split : blockIdx.x, blocks = second ? gridDim.x - split : split;
   const int64_t first = block * 256 + threadIdx.x, step = blocks * 256;
-  if (j.dtype == TFORGE_F32) copy_groups<float, __nv_bfloat16>(j, first, step);
-  else if (j.dtype == TFORGE_BF16) copy_groups<uint16_t, uint16_t>(j, first, step);
-  else copy_groups<uint8_t, uint8_t>(j, first, step);
+  if (j.dtype == TFORGE_F32) convert_groups(j, first, step);
+  else if (j.dtype == TFORGE_BF16) copy_groups<2>(j, first, step);
+  else copy_groups<1>(j, first, step);
 }
 
 int64_t padded(int64_t cols, int esz) { return (cols * esz + 15) / 16 * 16 / esz; }
@@ -174,7 +210,8 @@ class Copies {
       job_[i].dst = scratch.at(offset_[i]);
       operand_[i]->p = job_[i].dst;
       operand_[i]->ld = job_[i].ldd;
-      blocks[i] = (job_[i].rows * ((job_[i].cols + 7) / 8) + 255) / 256;
+      const int64_t per = job_[i].dtype == TFORGE_E4M3 ? 16 : 8;
+      blocks[i] = (job_[i].rows * ((job_[i].cols + per - 1) / per) + 255) / 256;
     }
     // Up to 16 blocks an SM, shared by the groups that each operand has.
     const int64_t most = 148 * 16, total = blocks[0] + blocks[1];
@@ -203,30 +240,34 @@ struct Choice {
   int splits;
 };
 
-// Least estimated time in us over the pair kernel and the slim kernel's tiles and splits.  The
-// estimates are fits to a sweep of 162 problems (M 1 .. 4096, nine N x K from 128 x 2048 to
-// 16384 x 4096, bf16 and e4m3) by every kernel: the choice is 2.5 % slower than the fastest on
-// average, and at worst 35 % (1024 x 512 x 8192: 27.3 us against 20.2).
+// The pair kernel where its tiles fill the 74 pairs once; else the least estimated time in us over it
+// and the slim kernel's tiles and splits.  The estimates are fits to a sweep of 162 problems (M 1 ..
+// 4096, nine N x K from 128 x 2048 to 16384 x 4096, bf16 and e4m3) by every kernel: the choice is
+// 2.8 % slower than the fastest on average, and at worst 25 % (2048 x 1024 x 1024: 13.8 us, 11.0).
 //   memory: operands and output once at the measured copy rate.
-//   pair:   waves of 74 pairs, each 0.367 us a stage of k (at least 7: an epilogue), or 1.68 x memory.
-//   slim:   a stage of k costs a CTA 0.246 us and 0.0005 per row of its tile, two CTAs an SM each
-//           0.65 of that (one with 256 rows); smoothly no less than 1.24 x memory; and per round of
-//           resident CTAs 2.7 us, the epilogue's rows, and what a cluster of S costs to meet.
+//   pair:   waves of 74 pairs, each 0.356 us a stage of k (at least 5.1: an epilogue), or 1.58 x memory.
+//   slim:   a stage of k costs a CTA 0.265 us and 0.0005 per row of its tile, two CTAs an SM each
+//           0.55 of that (one with 256 rows); smoothly no less than 1.17 x memory; per round of
+//           resident CTAs 2.6 us and what a cluster of S costs to meet; per CTA on an SM the
+//           epilogue's rows.
 Choice choose(int64_t M, int64_t N, int64_t K, bool t_mn, int esz) {
   const double nkb = (double)((K * esz + 127) / 128);
   const double memory = ((double)esz * K * (M + N) + 2.0 * M * N) / 6.55e6;
-  const double waves = std::ceil(std::ceil(M / 256.0) * std::ceil(N / 256.0) / 74.0);
+  const double tiles256 = std::ceil(M / 256.0) * std::ceil(N / 256.0);
   Choice best{0, 1};
-  double least = 4.28 + std::fmax(waves * std::fmax(0.367 * nkb, 7.0), 1.68 * memory);
+  if (K > 0 && tiles256 >= 74) return best;
+  double least = 5.65 + std::fmax(std::fmax(0.356 * nkb, 5.1), 1.58 * memory);
   if (K == 0) least = 1e300;  // the pair kernel needs a k
   for (int tile = t_mn ? 64 : 16; tile <= 256; tile *= 2) {
     const double tiles = std::ceil((double)M / tile) * std::ceil(N / 128.0), live = M < tile ? (double)M : tile;
     for (int s = 1; s <= 8; s *= 2) {
-      const double ctas = tiles * s, deep = std::ceil(ctas / 148.0);
-      const double load = (deep == 1 || tile == 256 ? deep : 0.65 * deep) * std::ceil(nkb / s) * (0.246 + 0.000535 * tile);
-      const double l2 = load * load, m2 = 1.24 * 1.24 * memory * memory;
-      const double rounds = std::ceil(ctas / (tile == 256 ? 148.0 : 296.0));
-      const double t = std::sqrt(std::sqrt(l2 * l2 + m2 * m2)) + rounds * (2.7 + 0.0375 * live + (s > 1 ? 0.245 + 0.357 * s : 0.0));
+      // CTAs that the SMs hold at once: clusters of 4 and 8 do not find a place on every SM.
+      const double slots = tile == 256 ? (s <= 2 ? 148 : s == 4 ? 132 : 120) : (s <= 2 ? 296 : s == 4 ? 284 : 264);
+      const double ctas = tiles * s, deep = std::ceil(ctas / 148.0), rounds = std::ceil(ctas / slots);
+      const double load = (deep == 1 || tile == 256 ? deep : 0.55 * deep) * std::ceil(nkb / s) * (0.265 + 0.000511 * tile);
+      const double l2 = load * load, m2 = 1.17 * 1.17 * memory * memory;
+      const double t = std::sqrt(std::sqrt(l2 * l2 + m2 * m2)) + rounds * (2.57 + (s > 1 ? 0.21 + 0.29 * s : 0.0)) +
+                       deep * live * (s > 1 ? 0.0351 : 0.0319);
       if (t < least) {
         least = t;
         best = Choice{tile, s};
