@@ -443,14 +443,15 @@ int grad_across(int64_t N) {
 }
 // Row blocks: up to 16 blocks an SM in all (several rounds of resident ones, so that the last is a
 // small part), each of at least 32 rows, so that the block sums are a few percent of what is read --
-// or fewer rows while there are fewer blocks than would fill the SMs once, down to 8.
+// or fewer rows while there are fewer blocks than would fill the SMs once, down to 8.  At most 256
+// blocks of rows: narrow matrices' block sums would take longer to add than to make.
 int grad_row_blocks(int64_t M, int64_t N) {
   const int across = grad_across(N);
   const int64_t cols = (N + 256 * across - 1) / (256 * across);
   int64_t rows = 32;
   while (rows > 8 && (M + rows - 1) / rows * cols < 148 * 4) rows /= 2;
   int64_t r = 148 * 16 / cols;
-  if (r > (M + rows - 1) / rows) r = (M + rows - 1) / rows;
+  r = std::min<int64_t>(std::min<int64_t>(r, 256), (M + rows - 1) / rows);
   return r < 1 ? 1 : (int)r;
 }
 

@@ -121,8 +121,8 @@ __device__ __forceinline__ void stage_row(uint8_t *box, int r, bool bf16, const 
 }
 
 // A warp's 32 rows x 32 columns turned round through its own 4 KB (column j of row l at j ^ l) and
-// stored row by row, a lane a column: any alignment.  R: the residual's type (void: none), added on
-// the way, eight rows' loads in flight.
+// stored row by row, a lane a column: any alignment.  R: the residual's type (NoResidual: none),
+// added on the way, sixteen rows' loads in flight.
 template <typename T, typename R>
 __device__ __forceinline__ void store_turned(float *buf, int lane, int rows, T *dst, int64_t ld, const R *res, int64_t ldr,
                                              const float (&v)[32]) {
@@ -130,15 +130,15 @@ __device__ __forceinline__ void store_turned(float *buf, int lane, int rows, T *
   for (int j = 0; j < 32; ++j) buf[lane * 32 + (j ^ lane)] = v[j];
   __syncwarp();
 #pragma unroll 1
-  for (int l0 = 0; l0 < rows; l0 += 8) {
-    float x[8];
+  for (int l0 = 0; l0 < rows; l0 += 16) {
+    float x[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 16; ++i) {
       if constexpr (sizeof(R) == 2) x[i] = l0 + i < rows ? __bfloat162float(res[(l0 + i) * ldr]) : 0.f;
       else if constexpr (sizeof(R) == 4) x[i] = l0 + i < rows ? res[(l0 + i) * ldr] : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 16; ++i) {
       if (l0 + i < rows) {
         float y = buf[(l0 + i) * 32 + (lane ^ (l0 + i))];
         if constexpr (sizeof(R) > 1) y += x[i];

@@ -13,7 +13,8 @@
 // ring's shared memory as f32, token by token; after a barrier (of the cluster, if it shares the
 // tile) each CTA takes 1/S of the tile's values in groups of eight neighbouring columns of a token,
 // adds the S CTAs' sums in order of z (the same bits every time) and finishes them: 16-byte
-// accesses where the caller's rows allow, single elements elsewhere.
+// accesses where the caller's rows allow; elsewhere the eight columns lie 16 apart, so that
+// neighbouring threads' single accesses are neighbouring elements.
 //
 // 256 threads: warp 0 TMA producer, warp 1 MMA issuer, then all eight warps the epilogue.  Every
 // wait is bounded (tf_ptx.cuh), and none begins before the kernel that this launch follows is done.
@@ -53,58 +54,103 @@ __device__ __forceinline__ void read8(const float *src, float (&v)[8]) {
   v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
-// Columns n .. n + 7 of an output row, those below N.
-__device__ __forceinline__ void put8(void *base, bool bf16, bool vec, int64_t i, int live, const float (&v)[8]) {
+// Column j of a thread's eight: n + j with VEC, else n + 16 j; below N by `live` = N - n.
+template <bool VEC>
+__device__ __forceinline__ void put8(void *base, bool bf16, int64_t i, int live, const float (&v)[8]) {
   if (bf16) {
     __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(base) + i;
-    if (vec) {
+    if constexpr (VEC) {
       *reinterpret_cast<uint4 *>(o) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
                                                  pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j < live) o[j] = __float2bfloat16_rn(v[j]);
+        if (16 * j < live) o[16 * j] = __float2bfloat16_rn(v[j]);
     }
   } else {
     float *o = static_cast<float *>(base) + i;
-    if (vec) {
+    if constexpr (VEC) {
       reinterpret_cast<float4 *>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
       reinterpret_cast<float4 *>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j < live) o[j] = v[j];
+        if (16 * j < live) o[16 * j] = v[j];
     }
   }
 }
+template <bool VEC>
+__device__ __forceinline__ void get8(const float *src, int live, float (&v)[8]) {
+  if constexpr (VEC) {
+    read8(src, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 16 * j < live ? src[16 * j] : 0.f;
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void get_residual(const LinearParams &p, int64_t i, int live, float (&v)[8]) {
+  if constexpr (VEC) {
+    if (p.res_bf16) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.residual) + i);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      }
+    } else {
+      read8(static_cast<const float *>(p.residual) + i, v);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 16 * j < live ? residual_at(p, i + 16 * j) : 0.f;
+  }
+}
 
-// Finishes the accumulated sums v of token m, columns n .. n + 7 (`live` of them below N).  vec: every
-// array of the epilogue has these eight on a 16-byte boundary.
-__device__ __forceinline__ void finish8(const LinearParams &p, float (&v)[8], int64_t m, int n, int live, bool vec,
-                                        const float (&res)[8]) {
-  float c[8];
+// Group g of the tile: token g / 16, eight columns; `part` holds its sums (token by token), in
+// `splits` CTAs' shared memory at `sbase`.
+template <bool VEC>
+__device__ __forceinline__ void finish8(const LinearParams &p, int g, int m0, int n0, const float *part, uint32_t sbase,
+                                        int splits) {
+  const int at = VEC ? 8 * (g & 15) : g & 15, n = n0 + at, live = p.N - n;
+  const int64_t m = m0 + (g >> 4);
+  if (live <= 0) return;
+  float res[8], v[8], c[8];
+  if (p.residual) get_residual<VEC>(p, m * p.ldr + n, live, res);
+  const int first = (g >> 4) * 128 + at;  // of the token-by-token sums
+  if (splits == 1) {
+    get8<VEC>(part + first, 1 << 30, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if (s < splits) {
+        const uint32_t src = map_to_cta(sbase + 4 * first, s);
+        if constexpr (VEC) {
+          const float4 a = ld_cluster_f32x4(src), b = ld_cluster_f32x4(src + 16);
+          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] += ld_cluster_f32(src + 64 * j);
+        }
+      }
+    }
+  }
   if (p.a_scale) {
     const float sa = __ldg(p.a_scale + m);
-    if (vec) {
-      read8(p.b_scale + n, c);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) c[j] = j < live ? p.b_scale[n + j] : 0.f;
-    }
+    get8<VEC>(p.b_scale + n, live, c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = v[j] * sa * c[j];
   }
   if (p.bias) {
-    if (vec) {
-      read8(p.bias + n, c);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) c[j] = j < live ? p.bias[n + j] : 0.f;
-    }
+    get8<VEC>(p.bias + n, live, c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += c[j];
   }
-  if (p.pre) put8(p.pre, p.out_bf16, vec, m * p.ldp + n, live, v);
+  if (p.pre) put8<VEC>(p.pre, p.out_bf16, m * p.ldp + n, live, v);
   with_activation(p.act, [&](auto act) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = activate<decltype(act)::value>(v[j]);
@@ -113,7 +159,7 @@ __device__ __forceinline__ void finish8(const LinearParams &p, float (&v)[8], in
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += res[j];
   }
-  put8(p.out, p.out_bf16, vec, m * p.ldo + n, live, v);
+  put8<VEC>(p.out, p.out_bf16, m * p.ldo + n, live, v);
 }
 
 // F8: e4m3 operands (both K-major).  WMN / TMN: the weights' / tokens' tile is MN-major (bf16).
@@ -254,50 +300,17 @@ __global__ void __launch_bounds__(256)
   }
   const bool all_ok = __syncthreads_and(ok);
   if (splits > 1) cluster_sync();
-  // Group g of eight columns: token g / 16, columns n0 + 8 (g % 16) ..; this CTA's share of them.
+  // This CTA's share of the tile's groups of eight columns, 16 a token.  A tile that reaches beyond N
+  // in the middle of a group goes element by element.
   const int groups = tokens * 16, share = (groups + splits - 1) / splits;
   const int g1 = (z + 1) * share < groups ? (z + 1) * share : groups;
+  const bool vec = p.vec && (p.N % 8 == 0 || n0 + 128 <= p.N);
+  if (all_ok) {
 #pragma unroll 1
-  for (int g = z * share + (int)threadIdx.x; g < g1; g += L::kThreads) {
-    const int n = n0 + 8 * (g & 15), live = p.N - n;
-    const int64_t m = m0 + (g >> 4);
-    if (live <= 0 || !all_ok) continue;
-    const bool vec = p.vec && live >= 8;
-    float res[8];
-    if (p.residual) {
-      const int64_t i = m * p.ldr + n;
-      if (vec && p.res_bf16) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.residual) + i);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          res[2 * j] = __uint_as_float(w[j] << 16);
-          res[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        }
-      } else if (vec) {
-        read8(static_cast<const float *>(p.residual) + i, res);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) res[j] = j < live ? residual_at(p, i + j) : 0.f;
-      }
+    for (int g = z * share + (int)threadIdx.x; g < g1; g += L::kThreads) {
+      if (vec) finish8<true>(p, g, m0, n0, part, sbase, splits);
+      else finish8<false>(p, g, m0, n0, part, sbase, splits);
     }
-    float v[8];
-    if (splits == 1) {
-      read8(part + 8 * g, v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        if (s < splits) {
-          const uint32_t src = map_to_cta(sbase + 32 * g, s);
-          const float4 a = ld_cluster_f32x4(src), b = ld_cluster_f32x4(src + 16);
-          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-        }
-      }
-    }
-    finish8(p, v, m, n, live, vec, res);
   }
   tc_fence_before();
   __syncthreads();
