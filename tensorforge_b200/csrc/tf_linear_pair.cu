@@ -122,43 +122,53 @@ __device__ __forceinline__ void stage_row(uint8_t *box, int r, bool bf16, const 
 
 // A warp's 32 rows x 32 columns turned round through its own 4 KB (column j of row l at j ^ l) and
 // stored row by row, a lane a column: any alignment.  R: the residual's type (NoResidual: none),
-// added on the way, sixteen rows' loads in flight.
+// added on the way, sixteen rows' loads in flight.  Whole tiles step pointers without conditions.
+struct NoResidual {};
+template <typename T>
+__device__ __forceinline__ void store_as(T *dst, float y) {
+  if constexpr (sizeof(T) == 2) *dst = __float2bfloat16_rn(y);
+  else *dst = y;
+}
 template <typename T, typename R>
-__device__ __forceinline__ void store_turned(float *buf, int lane, int rows, T *dst, int64_t ld, const R *res, int64_t ldr,
-                                             const float (&v)[32]) {
-#pragma unroll
-  for (int j = 0; j < 32; ++j) buf[lane * 32 + (j ^ lane)] = v[j];
-  __syncwarp();
+__device__ __forceinline__ void store_turned(const float *buf, int lane, int rows, T *dst, int64_t ld, const R *res, int64_t ldr) {
+  constexpr bool kRes = !std::is_same<R, NoResidual>::value;
+  if (__all_sync(0xFFFFFFFFu, rows == 32)) {
 #pragma unroll 1
-  for (int l0 = 0; l0 < rows; l0 += 16) {
-    float x[16];
+    for (int l0 = 0; l0 < 32; l0 += 16) {
+      float x[16];
+      if constexpr (kRes) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if constexpr (sizeof(R) == 2) x[i] = l0 + i < rows ? __bfloat162float(res[(l0 + i) * ldr]) : 0.f;
-      else if constexpr (sizeof(R) == 4) x[i] = l0 + i < rows ? res[(l0 + i) * ldr] : 0.f;
-    }
+        for (int i = 0; i < 16; ++i, res += ldr) x[i] = (float)*res;
+      }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (l0 + i < rows) {
+      for (int i = 0; i < 16; ++i, dst += ld) {
         float y = buf[(l0 + i) * 32 + (lane ^ (l0 + i))];
-        if constexpr (sizeof(R) > 1) y += x[i];
-        if constexpr (sizeof(T) == 2) dst[(l0 + i) * ld] = __float2bfloat16_rn(y);
-        else dst[(l0 + i) * ld] = y;
+        if constexpr (kRes) y += x[i];
+        store_as(dst, y);
       }
     }
+  } else {
+#pragma unroll 1
+    for (int l = 0; l < rows; ++l) {
+      float y = buf[l * 32 + (lane ^ l)];
+      if constexpr (kRes) y += (float)res[l * ldr];
+      store_as(dst + l * ld, y);
+    }
   }
-  __syncwarp();
 }
-struct NoResidual {};
 template <typename T>
 __device__ __forceinline__ void store_turned(const LinearParams &p, float *buf, int lane, int64_t row0, int col0, T *base,
                                              int64_t ld, bool res, const float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) buf[lane * 32 + (j ^ lane)] = v[j];
+  __syncwarp();
   const int rows = col0 + lane < p.N ? (int)(p.M - row0 < 32 ? p.M - row0 : 32) : 0;
   T *dst = base + row0 * ld + col0 + lane;
   const int64_t r = row0 * p.ldr + col0 + lane;
-  if (!res) store_turned(buf, lane, rows, dst, ld, static_cast<const NoResidual *>(nullptr), 0, v);
-  else if (p.res_bf16) store_turned(buf, lane, rows, dst, ld, static_cast<const __nv_bfloat16 *>(p.residual) + r, p.ldr, v);
-  else store_turned(buf, lane, rows, dst, ld, static_cast<const float *>(p.residual) + r, p.ldr, v);
+  if (!res) store_turned(buf, lane, rows, dst, ld, static_cast<const NoResidual *>(nullptr), 0);
+  else if (p.res_bf16) store_turned(buf, lane, rows, dst, ld, static_cast<const __nv_bfloat16 *>(p.residual) + r, p.ldr);
+  else store_turned(buf, lane, rows, dst, ld, static_cast<const float *>(p.residual) + r, p.ldr);
+  __syncwarp();
 }
 
 // F8: e4m3 operands (both K-major).  AMN / BMN: A / B is MN-major (bf16).
