@@ -71,12 +71,13 @@ inline void pdl_attr(cudaLaunchAttribute &a) {
   a.val.programmaticStreamSerializationAllowed = 1;
 }
 
-// Launches `kern` as a programmatic dependent of the kernel before it on the stream.
+// Launches `kern` as a programmatic dependent of the kernel before it on the stream, with `smem` bytes
+// of dynamic shared memory.
 template <typename... P, typename... A>
-inline cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, dim3 block, cudaStream_t stream, A... args) {
+inline cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, dim3 block, cudaStream_t stream, int smem, A... args) {
   cudaLaunchAttribute attr[1];
   pdl_attr(attr[0]);
-  cudaLaunchConfig_t cfg = {grid, block, 0, stream, attr, 1};
+  cudaLaunchConfig_t cfg = {grid, block, (size_t)smem, stream, attr, 1};
   return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
 }
 
@@ -239,9 +240,10 @@ struct NormBwdArgs {
 };
 // norm false: the row quantizer (out_kind 2).
 cudaError_t launch_rms_norm(const NormArgs &p, bool norm, cudaStream_t stream);
-// Blocks of the gradient kernel, and so rows of its scratch `part` (rows x N f32; null: no dweight).
+// Blocks (clusters) of the gradient kernel, and so rows of its scratch `part` (rows x N f32; null: no
+// dweight).
 int rms_norm_bwd_blocks(const NormBwdArgs &p);
-cudaError_t launch_rms_norm_bwd(const NormBwdArgs &p, float *part, int grid, cudaStream_t stream);
+cudaError_t launch_rms_norm_bwd(const NormBwdArgs &p, float *part, int blocks, cudaStream_t stream);
 // out[n] = sum over r < rows, in a fixed order, of part[r * N + n].
 cudaError_t launch_column_sum(const float *part, int rows, int64_t N, float *out, cudaStream_t stream);
 

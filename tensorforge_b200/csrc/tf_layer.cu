@@ -219,7 +219,7 @@ class Copies {
       blocks[0] = std::max<int64_t>(1, most * blocks[0] / total);
       if (blocks[1]) blocks[1] = std::max<int64_t>(1, most - blocks[0]);
     }
-    cudaError_t e = launch_dependent(copy_rows_kernel, dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), st, job_[0],
+    cudaError_t e = launch_dependent(copy_rows_kernel, dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), st, 0, job_[0],
                                      job_[n_ - 1], (int)blocks[0]);
     return e == cudaSuccess ? TFORGE_OK : cuda_failure(e, "operand copy");
   }
@@ -463,7 +463,7 @@ cudaError_t launch_activation_grad(int act, const void *dout, int64_t lddo, cons
                    (act == TFORGE_ACT_NONE || (at(pre, 16) && ldp * e % 16 == 0));
   const dim3 g((unsigned)((N + 256 * across - 1) / (256 * across)), (unsigned)row_blocks);
   auto kern = vec ? activation_grad_kernel<T, true> : activation_grad_kernel<T, false>;
-  return launch_dependent(kern, g, dim3(256), st, act, across, static_cast<const T *>(dout), lddo, static_cast<const T *>(pre),
+  return launch_dependent(kern, g, dim3(256), st, 0, act, across, static_cast<const T *>(dout), lddo, static_cast<const T *>(pre),
                           ldp, static_cast<__nv_bfloat16 *>(dz), ldz, part, M, N);
 }
 

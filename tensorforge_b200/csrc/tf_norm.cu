@@ -123,6 +123,24 @@ __device__ __forceinline__ void row_reduce(float &a, uint32_t &b, uint32_t *sm) 
   }
 }
 
+// The sum over a row that a cluster of CL blocks of T threads shares.  `sm`: CL T / 32 words of this
+// block, written by all of them; not written again before the next reduction's barrier but one.
+template <int T, int CL>
+__device__ __forceinline__ float cluster_sum(float a, float *sm) {
+  constexpr int W = T / 32, N = CL * W;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane < CL) st_cluster_f32(map_to_cta(smem_u32(sm + cluster_ctarank() * W + w), lane), a);
+  cluster_sync();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < (N + 31) / 32; ++i) s += N % 32 == 0 || lane + 32 * i < N ? sm[lane + 32 * i] : 0.f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  return s;
+}
+
 __device__ __forceinline__ float weight_at(const NormArgs &p, int64_t c) {
   if (!p.weight) return 1.f;
   return p.w_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.weight)[c])
@@ -370,20 +388,23 @@ struct RawRow {
 template <int T>
 constexpr int kBwdBlock = T <= 32 ? 256 : T;
 
-// How the gradient kernel holds a row: as it was loaded; the same, with the next row's loads under way
-// while a row is reduced and written; or not at all, reading it again after the reduction.
-enum Hold : int { HOLD_ROW = 0, HOLD_NEXT = 1, HOLD_NONE = 2 };
-
-// Row groups b, b + gridDim.x, ... of block b.  part: gridDim.x rows of N f32, this block's column sums (null: no dweight).
-template <typename X, bool VEC, int T, int E, int HOLD>
-__global__ void __launch_bounds__(kBwdBlock<T>) norm_bwd_kernel(const NormBwdArgs p, float *__restrict__ part) {
+// Row groups b, b + gridDim.x / CL, ... of block (or of cluster of CL blocks, each with T E columns of
+// the row) b.  AHEAD: the next rows' loads are under way while a row is reduced and written.  part:
+// gridDim.x / CL rows of N f32, this block's column sums (null: no dweight).
+template <typename X, bool VEC, int T, int E, int CL, bool AHEAD>
+__global__ void __launch_bounds__(kBwdBlock<T>, T == 512 ? 2 : 1) norm_bwd_kernel(const NormBwdArgs p, float *__restrict__ part) {
   grid_dependency_wait();
   grid_launch_dependents();
   using Raw = RawRow<X, VEC, E>;
   constexpr int kRows = kBwdBlock<T> / T;
-  __shared__ __align__(16) uint32_t sm[2][64];
+  static_assert(CL == 1 || kRows == 1, "a cluster has one row at a time");
+  __shared__ __align__(16) uint32_t sm[2][CL * T / 32 > 64 ? CL * T / 32 : 64];
   __shared__ float comb[kRows > 1 ? kRows * T * E : 1];
   const int t = threadIdx.x & (T - 1), sub = threadIdx.x / T;
+  // This block's columns: c0 .. c0 + width - 1.
+  const int64_t c0 = CL > 1 ? (int64_t)cluster_ctarank() * (T * E) : 0;
+  const int width = CL > 1 ? (int)(p.N - c0 < 0 ? 0 : p.N - c0 < T * E ? p.N - c0 : T * E) : (int)p.N;
+  const int block = (int)blockIdx.x / CL, blocks = (int)gridDim.x / CL;
   NormArgs wa{};
   wa.weight = p.weight;
   wa.w_bf16 = p.w_bf16;
@@ -391,7 +412,7 @@ __global__ void __launch_bounds__(kBwdBlock<T>) norm_bwd_kernel(const NormBwdArg
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int c = Raw::template col<T>(e, t);
-    w[e] = c < p.N ? weight_at(wa, c) : 0.f;
+    w[e] = c < width ? weight_at(wa, c0 + c) : 0.f;
     acc[e] = 0.f;
   }
   struct Rows {
@@ -399,23 +420,23 @@ __global__ void __launch_bounds__(kBwdBlock<T>) norm_bwd_kernel(const NormBwdArg
     float rstd;
   };
   Rows next;
-  auto fetch = [&](int64_t m0, bool first) {
+  auto fetch = [&](int64_t m0) {
     const bool live = m0 + sub < p.M;  // a part of a warp without a row goes along with no columns
     const int64_t m = live ? m0 + sub : 0;
-    const int n = live ? (int)p.N : 0;
-    next.y.template load<T>(static_cast<const X *>(p.dy) + m * p.lddy, t, n);
-    next.s.template load<T>(static_cast<const X *>(p.s) + m * p.lds, t, n);
-    if (p.ds && !(HOLD == HOLD_NONE && first)) next.d.template load<T>(static_cast<const X *>(p.ds) + m * p.ldds, t, n);
+    const int n = live ? width : 0;
+    next.y.template load<T>(static_cast<const X *>(p.dy) + m * p.lddy + c0, t, n);
+    next.s.template load<T>(static_cast<const X *>(p.s) + m * p.lds + c0, t, n);
+    if (p.ds) next.d.template load<T>(static_cast<const X *>(p.ds) + m * p.ldds + c0, t, n);
     next.rstd = __ldg(p.rstd + m);
   };
-  const int64_t step = (int64_t)gridDim.x * kRows;
-  int64_t m0 = (int64_t)blockIdx.x * kRows;
-  if (HOLD == HOLD_NEXT && m0 < p.M) fetch(m0, true);
+  const int64_t step = (int64_t)blocks * kRows;
+  int64_t m0 = (int64_t)block * kRows;
+  if (AHEAD && m0 < p.M) fetch(m0);
   int par = 0;
   for (; m0 < p.M; m0 += step, par ^= 1) {
     // The row is kept as it was loaded, and unpacked before and after the reduction: fewer registers.
-    if constexpr (HOLD != HOLD_NEXT) fetch(m0, true);
-    Rows row = next;
+    if constexpr (!AHEAD) fetch(m0);
+    const Rows row = next;
     float dot = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -423,20 +444,20 @@ __global__ void __launch_bounds__(kBwdBlock<T>) norm_bwd_kernel(const NormBwdArg
       acc[e] = fmaf(y, h, acc[e]);
       dot = fmaf(y * w[e], h, dot);
     }
-    if (HOLD == HOLD_NEXT && m0 + step < p.M) fetch(m0 + step, true);
-    uint32_t none = 0u;
-    row_reduce<T, false>(dot, none, sm[par]);
-    const float c1 = dot * p.inv_n;
-    if constexpr (HOLD == HOLD_NONE) {
-      fetch(m0, false);
-      row = next;
+    if (AHEAD && m0 + step < p.M) fetch(m0 + step);
+    if constexpr (CL > 1) {
+      dot = cluster_sum<T, CL>(dot, reinterpret_cast<float *>(sm[par]));
+    } else {
+      uint32_t none = 0u;
+      row_reduce<T, false>(dot, none, sm[par]);
     }
+    const float c1 = dot * p.inv_n;
     float g[E];
 #pragma unroll
     for (int e = 0; e < E; ++e)
       g[e] = fmaf(row.rstd, fmaf(-row.s.get(e) * row.rstd, c1, row.y.get(e) * w[e]), p.ds ? row.d.get(e) : 0.f);
-    const int n = m0 + sub < p.M ? (int)p.N : 0;
-    X *dx = static_cast<X *>(p.dx) + (m0 + sub) * p.lddx;
+    const int n = m0 + sub < p.M ? width : 0;
+    X *dx = static_cast<X *>(p.dx) + (m0 + sub) * p.lddx + c0;
     if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < E / 8; ++i) {
@@ -450,7 +471,7 @@ __global__ void __launch_bounds__(kBwdBlock<T>) norm_bwd_kernel(const NormBwdArg
     }
   }
   if (!part) return;
-  float *row = part + (int64_t)blockIdx.x * p.N;
+  float *row = part + (int64_t)block * p.N + c0;
   if constexpr (kRows > 1) {
 #pragma unroll
     for (int e = 0; e < E; ++e) comb[(sub * E + e) * T + t] = acc[e];
@@ -461,30 +482,38 @@ __global__ void __launch_bounds__(kBwdBlock<T>) norm_bwd_kernel(const NormBwdArg
 #pragma unroll 4
       for (int q = 0; q < kRows; ++q) v += comb[q * E * T + i];
       const int c = Raw::template col<T>(i / T, i % T);
-      if (c < p.N) row[c] = v;
+      if (c < width) row[c] = v;
     }
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = Raw::template col<T>(e, t);
-      if (c < p.N) row[c] = acc[e];
+      if (c < width) row[c] = acc[e];
     }
   }
 }
 
-// Rows longer than the register kernel holds: two passes; the column sums are kept in this block's
-// row of `part`, each element read and written by one thread.
-template <typename X>
-__global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwdArgs p, float *__restrict__ part) {
+// Wider rows than eight blocks hold: two passes over a row, the second mostly from L2, the column sums
+// in this block's row of `part`, each element read and written by one thread.  VEC: eight elements a
+// thread and step; else one.
+template <typename X, bool VEC>
+__global__ void __launch_bounds__(512, 2) norm_bwd_wide_kernel(const NormBwdArgs p, float *__restrict__ part) {
   grid_dependency_wait();
   grid_launch_dependents();
+  using Raw = RawRow<X, VEC, VEC ? 8 : 1>;
+  constexpr int V = VEC ? 8 : 1;
   __shared__ __align__(16) uint32_t sm[2][64];
   NormArgs wa{};
   wa.weight = p.weight;
   wa.w_bf16 = p.w_bf16;
-  float *row = part ? part + (int64_t)blockIdx.x * p.N : nullptr;
-  int par = 0;
+  float *acc = part ? part + (int64_t)blockIdx.x * p.N : nullptr;
   bool first = true;
+  // Groups of V columns; a thread's own are 512 V apart.
+  auto weights = [&](int64_t c, float (&w)[V]) {
+    if constexpr (VEC) weight8(wa, c, w);
+    else w[0] = weight_at(wa, c);
+  };
+  int par = 0;
   for (int64_t m = blockIdx.x; m < p.M; m += gridDim.x, par ^= 1, first = false) {
     const X *dy = static_cast<const X *>(p.dy) + m * p.lddy;
     const X *s = static_cast<const X *>(p.s) + m * p.lds;
@@ -493,16 +522,34 @@ __global__ void __launch_bounds__(1024) norm_bwd_long_kernel(const NormBwdArgs p
     const float rstd = __ldg(p.rstd + m);
     float dot = 0.f;
     uint32_t none = 0u;
-#pragma unroll 4
-    for (int64_t c = threadIdx.x; c < p.N; c += 1024)
-      dot = fmaf(to_f32(dy[c]) * weight_at(wa, c), to_f32(s[c]) * rstd, dot);
-    row_reduce<1024, false>(dot, none, sm[par]);
+#pragma unroll 2
+    for (int64_t c = (int64_t)threadIdx.x * V; c < p.N; c += 512 * V) {
+      Raw y, h;
+      float w[V];
+      y.template load<1>(dy + c, 0, V);
+      h.template load<1>(s + c, 0, V);
+      weights(c, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) dot = fmaf(y.get(j) * w[j], h.get(j) * rstd, dot);
+    }
+    row_reduce<512, false>(dot, none, sm[par]);
     const float c1 = dot * p.inv_n;
-#pragma unroll 4
-    for (int64_t c = threadIdx.x; c < p.N; c += 1024) {
-      const float y = to_f32(dy[c]), h = to_f32(s[c]) * rstd, d = ds ? to_f32(ds[c]) : 0.f;
-      if (row) row[c] = first ? y * h : fmaf(y, h, row[c]);
-      store1(dx + c, fmaf(rstd, fmaf(-h, c1, y * weight_at(wa, c)), d));
+#pragma unroll 2
+    for (int64_t c = (int64_t)threadIdx.x * V; c < p.N; c += 512 * V) {
+      Raw y, h, d;
+      float w[V], g[V];
+      y.template load<1>(dy + c, 0, V);
+      h.template load<1>(s + c, 0, V);
+      if (ds) d.template load<1>(ds + c, 0, V);
+      weights(c, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float a = y.get(j), b = h.get(j) * rstd;
+        if (acc) acc[c + j] = first ? a * b : fmaf(a, b, acc[c + j]);
+        g[j] = fmaf(rstd, fmaf(-b, c1, a * w[j]), ds ? d.get(j) : 0.f);
+      }
+      if constexpr (VEC) store8(dx + c, g);
+      else store1(dx + c, g[0]);
     }
   }
 }
@@ -535,17 +582,17 @@ template <typename X, int OUT, bool VEC, bool NORM>
 cudaError_t launch_norm_rows(const NormArgs &p, cudaStream_t st) {
   auto grid = [&](int rows) { return dim3((unsigned)((p.M + rows - 1) / rows)); };
   if constexpr (VEC) {
-    if (p.N <= 64) return launch_dependent(norm_row_kernel<X, OUT, VEC, 8, 8, NORM>, grid(32), dim3(256), st, p);
-    if (p.N <= 128) return launch_dependent(norm_row_kernel<X, OUT, VEC, 16, 8, NORM>, grid(16), dim3(256), st, p);
+    if (p.N <= 64) return launch_dependent(norm_row_kernel<X, OUT, VEC, 8, 8, NORM>, grid(32), dim3(256), st, 0, p);
+    if (p.N <= 128) return launch_dependent(norm_row_kernel<X, OUT, VEC, 16, 8, NORM>, grid(16), dim3(256), st, 0, p);
   }
-  if (p.N <= 256) return launch_dependent(norm_row_kernel<X, OUT, VEC, 32, 8, NORM>, grid(8), dim3(256), st, p);
-  if (p.N <= 512) return launch_dependent(norm_row_kernel<X, OUT, VEC, 32, 16, NORM>, grid(8), dim3(256), st, p);
-  if (p.N <= 1024) return launch_dependent(norm_row_kernel<X, OUT, VEC, 128, 8, NORM>, grid(1), dim3(128), st, p);
-  if (p.N <= 2048) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 8, NORM>, grid(1), dim3(256), st, p);
-  if (p.N <= 4096) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 16, NORM>, grid(1), dim3(256), st, p);
-  if (p.N <= 8192) return launch_dependent(norm_row_kernel<X, OUT, VEC, 512, 16, NORM>, grid(1), dim3(512), st, p);
-  if (p.N <= 16384) return launch_dependent(norm_row_kernel<X, OUT, VEC, 512, 32, NORM>, grid(1), dim3(512), st, p);
-  return launch_dependent(norm_long_kernel<X, OUT, NORM>, grid(1), dim3(1024), st, p);
+  if (p.N <= 256) return launch_dependent(norm_row_kernel<X, OUT, VEC, 32, 8, NORM>, grid(8), dim3(256), st, 0, p);
+  if (p.N <= 512) return launch_dependent(norm_row_kernel<X, OUT, VEC, 32, 16, NORM>, grid(8), dim3(256), st, 0, p);
+  if (p.N <= 1024) return launch_dependent(norm_row_kernel<X, OUT, VEC, 128, 8, NORM>, grid(1), dim3(128), st, 0, p);
+  if (p.N <= 2048) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 8, NORM>, grid(1), dim3(256), st, 0, p);
+  if (p.N <= 4096) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 16, NORM>, grid(1), dim3(256), st, 0, p);
+  if (p.N <= 8192) return launch_dependent(norm_row_kernel<X, OUT, VEC, 512, 16, NORM>, grid(1), dim3(512), st, 0, p);
+  if (p.N <= 16384) return launch_dependent(norm_row_kernel<X, OUT, VEC, 512, 32, NORM>, grid(1), dim3(512), st, 0, p);
+  return launch_dependent(norm_long_kernel<X, OUT, NORM>, grid(1), dim3(1024), st, 0, p);
 }
 
 template <typename X, int OUT, bool NORM>
@@ -558,37 +605,43 @@ cudaError_t launch_norm_vec(const NormArgs &p, cudaStream_t st) {
   return vec ? launch_norm_rows<X, OUT, true, NORM>(p, st) : launch_norm_rows<X, OUT, false, NORM>(p, st);
 }
 
-// The gradient kernel of a call: eight elements a thread up to 8192 columns, sixteen up to 16384.
+// The gradient kernel of a call: eight elements a thread, and from 8193 columns a cluster of four or
+// eight blocks of 512 threads a row.  4096 x 16384 bf16 / f32 136 / 226 us; with two blocks of 1024
+// 150 / 210; with one block and sixteen elements a thread, which spill, 153 / 277.  320 x 13376 f32
+// (few rows): 29 us, 31 and 41.
 struct BwdKernel {
   void (*kern)(const NormBwdArgs, float *);
-  int threads, rows, id;  // of a block; a number of its own
+  int threads, rows;  // of a block
+  int cluster;
+  int id;  // a number of its own
 };
-template <typename X, bool VEC, int T, int E>
+template <typename X, bool VEC, int T, int CL = 1>
 BwdKernel bwd_kernel(int id) {
   // Two rows' pieces fit the registers for bf16 in 16-byte pieces; elsewhere a thread's loads are
-  // enough by themselves.  Sixteen elements a thread do not fit even once at 1024 threads.
-  constexpr int kHold = E > 8 ? HOLD_NONE : VEC && sizeof(X) == 2 ? HOLD_NEXT : HOLD_ROW;
-  return {norm_bwd_kernel<X, VEC, T, E, kHold>, kBwdBlock<T>, kBwdBlock<T> / T, id};
+  // enough by themselves.
+  constexpr bool kAhead = VEC && sizeof(X) == 2;
+  return {norm_bwd_kernel<X, VEC, T, 8, CL, kAhead>, kBwdBlock<T>, kBwdBlock<T> / T, CL, id};
 }
 template <typename X, bool VEC>
 BwdKernel pick_bwd(int64_t N, int id) {
   if constexpr (VEC) {
-    if (N <= 64) return bwd_kernel<X, VEC, 8, 8>(id);
-    if (N <= 128) return bwd_kernel<X, VEC, 16, 8>(id + 1);
+    if (N <= 64) return bwd_kernel<X, VEC, 8>(id);
+    if (N <= 128) return bwd_kernel<X, VEC, 16>(id + 1);
   }
-  if (N <= 256) return bwd_kernel<X, VEC, 32, 8>(id + 2);
-  if (N <= 512) return bwd_kernel<X, VEC, 64, 8>(id + 9);
-  if (N <= 1024) return bwd_kernel<X, VEC, 128, 8>(id + 3);
-  if (N <= 2048) return bwd_kernel<X, VEC, 256, 8>(id + 4);
-  if (N <= 4096) return bwd_kernel<X, VEC, 512, 8>(id + 5);
-  if (N <= 8192) return bwd_kernel<X, VEC, 1024, 8>(id + 6);
-  if (N <= 16384) return bwd_kernel<X, VEC, 1024, 16>(id + 7);
-  return {norm_bwd_long_kernel<X>, 1024, 1, id + 8};
+  if (N <= 256) return bwd_kernel<X, VEC, 32>(id + 2);
+  if (N <= 512) return bwd_kernel<X, VEC, 64>(id + 3);
+  if (N <= 1024) return bwd_kernel<X, VEC, 128>(id + 4);
+  if (N <= 2048) return bwd_kernel<X, VEC, 256>(id + 5);
+  if (N <= 4096) return bwd_kernel<X, VEC, 512>(id + 6);
+  if (N <= 8192) return bwd_kernel<X, VEC, 1024>(id + 7);
+  if (N <= 16384) return bwd_kernel<X, VEC, 512, 4>(id + 8);
+  if (N <= 32768) return bwd_kernel<X, VEC, 512, 8>(id + 9);
+  return {norm_bwd_wide_kernel<X, VEC>, 512, 1, 1, id + 10};
 }
 
 bool bwd_vec(const NormBwdArgs &p) {
   const int e = p.x_bf16 ? 2 : 4;
-  return p.N % 8 == 0 && at16(p.dy) && at16(p.s) && at16(p.ds) && at16(p.dx) && p.lddy * e % 16 == 0 &&
+  return p.N % 8 == 0 && at16(p.weight) && at16(p.dy) && at16(p.s) && at16(p.ds) && at16(p.dx) && p.lddy * e % 16 == 0 &&
          p.lds * e % 16 == 0 && p.ldds * e % 16 == 0 && p.lddx * e % 16 == 0;
 }
 
@@ -609,33 +662,53 @@ cudaError_t launch_rms_norm(const NormArgs &p, bool norm, cudaStream_t st) {
 
 static BwdKernel pick_bwd(const NormBwdArgs &p) {
   const bool vec = bwd_vec(p);
-  if (p.x_bf16) return vec ? pick_bwd<__nv_bfloat16, true>(p.N, 0) : pick_bwd<__nv_bfloat16, false>(p.N, 10);
-  return vec ? pick_bwd<float, true>(p.N, 20) : pick_bwd<float, false>(p.N, 30);
+  if (p.x_bf16) return vec ? pick_bwd<__nv_bfloat16, true>(p.N, 0) : pick_bwd<__nv_bfloat16, false>(p.N, 11);
+  return vec ? pick_bwd<float, true>(p.N, 22) : pick_bwd<float, false>(p.N, 33);
 }
 
+static void cluster_attr(cudaLaunchAttribute &a, int cluster) {
+  a.id = cudaLaunchAttributeClusterDimension;
+  a.val.clusterDim.x = (unsigned)cluster;
+  a.val.clusterDim.y = a.val.clusterDim.z = 1;
+}
+
+// Blocks (or clusters of them) that the SMs hold at once, no more than there are row groups.
 int rms_norm_bwd_blocks(const NormBwdArgs &p) {
-  // As many blocks as the SMs hold at once, no more than there are row groups.
   const BwdKernel k = pick_bwd(p);
-  static std::atomic<int> resident[40];
+  static std::atomic<int> resident[44];
   int n = resident[k.id].load(std::memory_order_relaxed);
   if (n == 0) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k.kern, k.threads, 0) != cudaSuccess || n <= 0) {
+    cudaError_t e;
+    if (k.cluster > 1) {
+      cudaLaunchAttribute attr[1];
+      cluster_attr(attr[0], k.cluster);
+      cudaLaunchConfig_t cfg = {dim3(148 * 8), dim3((unsigned)k.threads), 0, nullptr, attr, 1};
+      e = cudaOccupancyMaxActiveClusters(&n, k.kern, &cfg);
+    } else {
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k.kern, k.threads, 0);
+      n *= 148;
+    }
+    if (e != cudaSuccess || n <= 0) {
       cudaGetLastError();
-      n = 1;
+      n = 148 / k.cluster;
     }
     resident[k.id].store(n, std::memory_order_relaxed);
   }
-  const int64_t groups = (p.M + k.rows - 1) / k.rows, most = 148LL * n;
-  return (int)(groups < most ? groups : most);
+  const int64_t groups = (p.M + k.rows - 1) / k.rows;
+  return (int)(groups < n ? groups : n);
 }
 
-cudaError_t launch_rms_norm_bwd(const NormBwdArgs &p, float *part, int grid, cudaStream_t st) {
+cudaError_t launch_rms_norm_bwd(const NormBwdArgs &p, float *part, int blocks, cudaStream_t st) {
   const BwdKernel k = pick_bwd(p);
-  return launch_dependent(k.kern, dim3((unsigned)grid), dim3((unsigned)k.threads), st, p, part);
+  cudaLaunchAttribute attr[2];
+  pdl_attr(attr[0]);
+  cluster_attr(attr[1], k.cluster);
+  cudaLaunchConfig_t cfg = {dim3((unsigned)(blocks * k.cluster)), dim3((unsigned)k.threads), 0, st, attr, k.cluster > 1 ? 2u : 1u};
+  return cudaLaunchKernelEx(&cfg, k.kern, p, part);
 }
 
 cudaError_t launch_column_sum(const float *part, int rows, int64_t N, float *out, cudaStream_t st) {
-  return launch_dependent(column_sum_kernel, dim3((unsigned)((N + 31) / 32)), dim3(32, 32), st, part, rows, N, out);
+  return launch_dependent(column_sum_kernel, dim3((unsigned)((N + 31) / 32)), dim3(32, 32), st, 0, part, rows, N, out);
 }
 
 }  // namespace tf

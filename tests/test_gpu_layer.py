@@ -388,7 +388,7 @@ def test_linear_backward_against_differences(act):
 # ---- the norm -----------------------------------------------------------------------------------
 
 
-WIDTHS = [1, 7, 8, 32, 200, 256, 257, 264, 1000, 1024, 1111, 2048, 2056, 4096, 4100, 8192, 8200, 16384, 16392, 20001]
+WIDTHS = [1, 7, 8, 32, 200, 256, 257, 264, 1000, 1024, 1111, 2048, 2056, 4096, 4100, 8192, 8200, 16384, 16392, 20001, 32760, 32770, 40000]
 
 
 def check_rms_norm(m, n, dtype=torch.bfloat16, out=torch.bfloat16, residual=True, weight=torch.float32, pad=0, shift=0,
