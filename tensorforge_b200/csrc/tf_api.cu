@@ -129,6 +129,18 @@ uint32_t *existing_status_word() {
   return g_status[dev];
 }
 
+// What the library makes on first use may be asked for while a stream is being captured: this lets
+// the calls of this thread through that a capture would refuse.
+class OutsideCapture {
+ public:
+  OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode_); }
+  ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode_); }
+  OutsideCapture(const OutsideCapture &) = delete;
+
+ private:
+  cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+};
+
 int status_word(uint32_t **out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -136,21 +148,18 @@ int status_word(uint32_t **out) {
   if (dev < 0 || dev >= kMaxDev) return TFORGE_ERR_UNSUPPORTED;
   std::lock_guard<std::mutex> lk(g_status_mu);
   if (!g_status[dev]) {
-    // The first call may come while a stream is being captured: allocate outside any capture
-    // (relaxed mode for this thread) and clear on a stream of its own.
+    OutsideCapture outside;
     void *p = nullptr;
-    cudaStream_t own = nullptr;
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    e = cudaThreadExchangeStreamCaptureMode(&mode);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaThreadExchangeStreamCaptureMode");
+    cudaStream_t own = nullptr;  // cleared on a stream of its own
     e = cudaMalloc(&p, 256);
     if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
     if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, 256, own);
     if (e == cudaSuccess) e = cudaStreamSynchronize(own);
     if (own) cudaStreamDestroy(own);
-    if (e != cudaSuccess && p) cudaFree(p);
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    if (e != cudaSuccess) return cuda_fail(e, "status word");
+    if (e != cudaSuccess) {
+      if (p) cudaFree(p);
+      return cuda_fail(e, "status word");
+    }
     g_status[dev] = static_cast<uint32_t *>(p);
   }
   *out = g_status[dev];
@@ -170,6 +179,7 @@ int scratch_pool(cudaMemPool_t *out) {
   if (dev < 0 || dev >= kMaxDev) return TFORGE_ERR_UNSUPPORTED;
   std::lock_guard<std::mutex> lk(g_status_mu);
   if (!g_pool[dev]) {
+    OutsideCapture outside;
     cudaMemPoolProps props{};
     props.allocType = cudaMemAllocationTypePinned;
     props.handleTypes = cudaMemHandleTypeNone;

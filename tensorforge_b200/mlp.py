@@ -81,9 +81,197 @@ class MLP2:
         return h, out
 
 
+class FeedForward:
+    """A transformer's feed-forward block on torch tensors of one GPU, through the C-ABI:
+
+        s = x + residual;  out = s + act(rms_norm(s) @ W1 + b1) @ W2 + b2
+
+    x, residual, s and out are bf16, M x D; W1 is D x H, W2 H x D.  mode "bf16": weights in bf16 as
+    given.  mode "fp8": each output feature's weights in 8 bits with a scale, the activations in 8
+    bits with a scale a row -- the norm writes the first product's, the quantizer the second's.
+    Calls run on the current stream of x's device.  `__call__(..., keep=True)` keeps what `backward`
+    needs until it is called (mode "bf16")."""
+
+    def __init__(self, w1, b1, w2, b2, norm_weight, activation: str = "gelu_tanh", mode: str = "bf16", eps: float = 1e-5):
+        import torch
+
+        if mode not in ("bf16", "fp8"):
+            raise ValueError("FeedForward takes mode 'bf16' or 'fp8'")
+        if activation not in _lib.ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}")
+        self.d, self.h = w1.shape
+        if w2.shape != (self.h, self.d) or b1.shape != (self.h,) or b2.shape != (self.d,) or norm_weight.shape != (self.d,):
+            raise ValueError("FeedForward expects W1 d x h, b1 h, W2 h x d, b2 d, norm weight d")
+        self.mode, self.activation, self.eps = mode, activation, eps
+        self.b1, self.b2, self.norm_weight = (t.float().contiguous() for t in (b1, b2, norm_weight))
+        self.kept = None
+        if mode == "bf16":
+            self.w1, self.w2 = w1.bfloat16().contiguous(), w2.bfloat16().contiguous()
+            return
+        with torch.cuda.device(w1.device):
+            self.w1, self.s1 = self._quantize(w1.float().t().contiguous())
+            self.w2, self.s2 = self._quantize(w2.float().t().contiguous())
+
+    @staticmethod
+    def _stream(t):
+        import torch
+
+        return torch.cuda.current_stream(t.device).cuda_stream
+
+    def _quantize(self, x):
+        """Rows of x (f32 or bf16) in 8 bits, and their scales."""
+        import torch
+
+        m, n = x.shape
+        q = torch.empty((m, n), device=x.device, dtype=torch.float8_e4m3fn)
+        scale = torch.empty((m,), device=x.device)
+        _lib.quantize_e4m3(x.data_ptr(), q.data_ptr(), scale.data_ptr(), m, n,
+                           _lib.F32 if x.dtype == torch.float32 else _lib.BF16, stream=self._stream(x))
+        return q, scale
+
+    def __call__(self, x, residual=None, keep: bool = False):
+        """(out, s).  s is what the next block adds its own output to when blocks are chained by hand;
+        out already holds it."""
+        import torch
+
+        if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != self.d or not x.is_contiguous():
+            raise ValueError("FeedForward takes contiguous bf16 rows of its width")
+        if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape or not residual.is_contiguous()):
+            raise ValueError("the residual is like x")
+        if keep and self.mode != "bf16":
+            raise ValueError("only mode 'bf16' has a gradient")
+        m, fp8 = x.shape[0], self.mode == "fp8"
+        with torch.cuda.device(x.device):
+            st = self._stream(x)
+
+            def new(*shape, dtype=torch.bfloat16):
+                return torch.empty(shape, device=x.device, dtype=dtype)
+
+            s = new(m, self.d) if residual is not None else x
+            n = new(m, self.d, dtype=torch.float8_e4m3fn if fp8 else torch.bfloat16)
+            scale = new(m, dtype=torch.float32) if fp8 else None
+            rstd = new(m, dtype=torch.float32) if keep else None
+            _lib.rms_norm(x.data_ptr(), n.data_ptr(), m, self.d, self.eps, weight=self.norm_weight.data_ptr(),
+                          residual=residual.data_ptr() if residual is not None else None,
+                          sum_out=s.data_ptr() if residual is not None else None, rstd=rstd.data_ptr() if keep else None,
+                          scale=scale.data_ptr() if fp8 else None, out_dtype=_lib.E4M3 if fp8 else _lib.BF16, stream=st)
+            hid, out = new(m, self.h), new(m, self.d)
+            pre = new(m, self.h) if keep and self.activation != "none" else None
+            if fp8:
+                e4m3 = dict(a_dtype=_lib.E4M3, b_dtype=_lib.E4M3, trans_b=True, stream=st)
+                _lib.linear(n.data_ptr(), self.w1.data_ptr(), hid.data_ptr(), m, self.h, self.d, self.activation,
+                            bias=self.b1.data_ptr(), a_scale=scale.data_ptr(), b_scale=self.s1.data_ptr(), **e4m3)
+                q, qs = self._quantize(hid)
+                _lib.linear(q.data_ptr(), self.w2.data_ptr(), out.data_ptr(), m, self.d, self.h, bias=self.b2.data_ptr(),
+                            residual=s.data_ptr(), a_scale=qs.data_ptr(), b_scale=self.s2.data_ptr(), **e4m3)
+            else:
+                _lib.linear(n.data_ptr(), self.w1.data_ptr(), hid.data_ptr(), m, self.h, self.d, self.activation,
+                            bias=self.b1.data_ptr(), pre=pre.data_ptr() if pre is not None else None, stream=st)
+                _lib.linear(hid.data_ptr(), self.w2.data_ptr(), out.data_ptr(), m, self.d, self.h, bias=self.b2.data_ptr(),
+                            residual=s.data_ptr(), stream=st)
+        if keep:
+            self.kept = (s, rstd, n, pre, hid)
+        return out, s
+
+    def backward(self, dout) -> dict:
+        """Gradients from out's gradient (bf16, M x D): dx (the residual's too), dw1, db1, dw2, db2 and
+        dnorm_weight; the weights' in bf16, the vectors' in f32."""
+        import torch
+
+        if self.kept is None:
+            raise ValueError("backward needs a call with keep=True before it")
+        s, rstd, n, pre, hid = self.kept
+        if dout.dtype != torch.bfloat16 or dout.shape != s.shape or not dout.is_contiguous():
+            raise ValueError("backward takes out's gradient: contiguous bf16 rows like out's")
+        self.kept = None
+        m = s.shape[0]
+        with torch.cuda.device(s.device):
+            st = self._stream(s)
+
+            def new(*shape, dtype=torch.bfloat16):
+                return torch.empty(shape, device=s.device, dtype=dtype)
+
+            g = {"dx": new(m, self.d), "dw1": new(self.d, self.h), "db1": new(self.h, dtype=torch.float32),
+                 "dw2": new(self.h, self.d), "db2": new(self.d, dtype=torch.float32),
+                 "dnorm_weight": new(self.d, dtype=torch.float32)}
+            dhid, dn = new(m, self.h), new(m, self.d)
+            _lib.linear_backward(dout.data_ptr(), hid.data_ptr(), self.w2.data_ptr(), m, self.d, self.h, dA=dhid.data_ptr(),
+                                 dB=g["dw2"].data_ptr(), dbias=g["db2"].data_ptr(), stream=st)
+            _lib.linear_backward(dhid.data_ptr(), n.data_ptr(), self.w1.data_ptr(), m, self.h, self.d, self.activation,
+                                 pre=pre.data_ptr() if pre is not None else None, dA=dn.data_ptr(), dB=g["dw1"].data_ptr(),
+                                 dbias=g["db1"].data_ptr(), stream=st)
+            _lib.rms_norm_backward(dn.data_ptr(), s.data_ptr(), rstd.data_ptr(), g["dx"].data_ptr(), m, self.d,
+                                   weight=self.norm_weight.data_ptr(), ds=dout.data_ptr(), dweight=g["dnorm_weight"].data_ptr(),
+                                   stream=st)
+        return g
+
+
 def flops(m: int, d: int, h: int) -> float:
     """2 M N K per layer (the reference's convention), two layers."""
     return 2.0 * m * d * h * 2
+
+
+def run_block(args, x, w1, b1, w2, b2, world: int, rank: int) -> int:
+    """Times the FeedForward block (with --train and its gradient) on this rank's rows and checks a
+    seeded subset of them against 64 bits, from the block's own 8- or 16-bit weights."""
+    import numpy as np
+    import torch
+    import torch.distributed as dist
+
+    dev = x.device
+    norm_weight = torch.ones(args.d, device=dev)
+    model = FeedForward(w1, b1, w2, b2, norm_weight, mode=args.mode)
+    x = x.bfloat16()
+    dout = (x * 0.01).contiguous()
+
+    def step():
+        out, _ = model(x, keep=args.train)
+        return out, model.backward(dout) if args.train else None
+
+    for _ in range(args.warmup):
+        out, _ = step()
+    torch.cuda.synchronize()
+    stream = torch.cuda.current_stream(dev)
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    if world > 1:
+        dist.barrier()
+    e0.record(stream)
+    for _ in range(args.steps):
+        out, _ = step()
+    e1.record(stream)
+    torch.cuda.synchronize()
+    ms = torch.tensor([e0.elapsed_time(e1) / args.steps], device=dev, dtype=torch.float64)
+    if world > 1:
+        dist.all_reduce(ms, op=dist.ReduceOp.MAX)
+    status = _lib.device_status(stream.cuda_stream)
+
+    rows = x.shape[0]
+    sel = torch.from_numpy(np.sort(np.random.default_rng(rank).choice(rows, min(args.check_rows, rows), replace=False))).to(dev)
+    s64 = x[sel].double()
+    n64 = s64 * (s64.square().mean(1, keepdim=True) + model.eps).rsqrt()
+    if args.mode == "fp8":
+        d1, d2 = model.w1.double() * model.s1.double()[:, None], model.w2.double() * model.s2.double()[:, None]
+        d1, d2 = d1.t(), d2.t()
+    else:
+        d1, d2 = model.w1.double(), model.w2.double()
+    z = n64 @ d1 + b1.double()
+    hid = 0.5 * z * (1 + torch.tanh((2 / np.pi) ** 0.5 * (z + 0.044715 * z ** 3)))
+    want = s64 + hid @ d2 + b2.double()
+    err = float((out[sel].double() - want).norm() / want.norm())
+    # Relative to the whole row: two roundings of the activations (2^-8 each way, or 2^-4 in 8 bits)
+    # and one of the output.
+    bound = 2.0 ** -3 if args.mode == "fp8" else 2.0 ** -6
+    ok = torch.tensor([int(err <= bound and status == 0)], device=dev)
+    if world > 1:
+        dist.all_reduce(ok, op=dist.ReduceOp.MIN)
+    if rank == 0:
+        t = float(ms.item())
+        fl = flops(args.m, args.d, args.h) * (3 if args.train else 1)
+        print(json.dumps({"workload": f"feed-forward block X {args.m}x{args.d}, W1 {args.d}x{args.h}, W2 {args.h}x{args.d}",
+                          "mode": args.mode, "gradient": bool(args.train), "n_gpus": world, "ms_per_step": t,
+                          "tflops": fl / (t * 1e-3) / 1e12, "rel_err": err, "rel_err_bound": bound,
+                          "checked_rows_per_rank": int(len(sel)), "pass": bool(ok.item())}), flush=True)
+    return 0 if ok.item() else 1
 
 
 def main(argv=None) -> int:
@@ -96,7 +284,10 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("--shape", default="65536x4096x16384",
                     help="MxDxH: rows of X in total (sharded over ranks), model width, hidden width")
-    ap.add_argument("--mode", default="fp32", choices=["fp32", "tf32", "bf16"])
+    ap.add_argument("--mode", default="fp32", choices=["fp32", "tf32", "bf16", "fp8"])
+    ap.add_argument("--block", action="store_true",
+                    help="the transformer block around the two layers (norm, residual, gelu; bf16 or fp8)")
+    ap.add_argument("--train", action="store_true", help="with --block: time the gradient too (bf16)")
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--check-rows", type=int, default=16, help="rows checked against FP64 per layer")
@@ -104,6 +295,10 @@ def main(argv=None) -> int:
                     help="hidden activation storage (auto: bf16 in BF16 mode, else f32)")
     args = ap.parse_args(argv)
     args.m, args.d, args.h = (int(x) for x in args.shape.lower().split("x"))
+    if args.block != (args.mode == "fp8") and not (args.block and args.mode == "bf16"):
+        ap.error("--block takes --mode bf16 or fp8, and fp8 needs --block")
+    if args.train and not (args.block and args.mode == "bf16"):
+        ap.error("--train needs --block --mode bf16")
 
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))
@@ -134,6 +329,12 @@ def main(argv=None) -> int:
         b2.normal_(0.0, 0.02, generator=g0)
     broadcast_weights(w1, b1)
     broadcast_weights(w2, b2)
+    if args.block:
+        rc = run_block(args, x, w1, b1, w2, b2, world, rank)
+        if world > 1:
+            dist.barrier()
+            dist.destroy_process_group()
+        return rc
     model = MLP2(w1, b1, w2, b2, args.mode, None if args.h_dtype == "auto" else args.h_dtype == "bf16")
     h = torch.empty((rows, args.h), device=dev, dtype=model.h_dtype)
     out = torch.empty((rows, args.d), device=dev)

@@ -661,3 +661,192 @@ def test_rms_norm_backward_against_differences():
         want = (value(s.double() + d) - value(s.double() - d)) / (2 * h)
         # f32 arithmetic on a sum of 24 terms of size up to about 10, and h^2 of third derivatives.
         assert bool(((dx[:, i].double() - want).abs() <= 1e-5 + 2.0 ** -18 * dy.double().abs().sum(1)).all())
+
+
+# ---- together -----------------------------------------------------------------------------------
+
+
+def block(d, h, act, mode, seed=0):
+    from tensorforge_b200.mlp import FeedForward
+
+    w1, w2 = rand(d, h, seed=seed, scale=1 / math.sqrt(d)), rand(h, d, seed=seed + 1, scale=1 / math.sqrt(h))
+    b1, b2, g = rand(h, seed=seed + 2, scale=0.1), rand(d, seed=seed + 3, scale=0.1), 1 + rand(d, seed=seed + 4, scale=0.1)
+    return FeedForward(w1, b1, w2, b2, g, act, mode)
+
+
+def block64(m, x, r):
+    """The block in 64 bits from its own weights, as a differentiable function."""
+    s = x + r if r is not None else x
+    n = s * (s.square().mean(1, keepdim=True) + m.eps).rsqrt() * m.p["g"]
+    return s + act64(n @ m.p["w1"] + m.p["b1"], m.activation)[0] @ m.p["w2"] + m.p["b2"]
+
+
+def weights64(m):
+    if m.mode == "fp8":
+        w1, w2 = (m.w1.double() * m.s1.double()[:, None]).T, (m.w2.double() * m.s2.double()[:, None]).T
+    else:
+        w1, w2 = m.w1.double(), m.w2.double()
+    m.p = {"w1": w1, "w2": w2, "b1": m.b1.double(), "b2": m.b2.double(), "g": m.norm_weight.double()}
+
+
+@pytest.mark.parametrize("mode", ["bf16", "fp8"])
+@pytest.mark.parametrize("act", ["gelu_tanh", "silu", "none"])
+@pytest.mark.parametrize("rows,d,h", [(1, 256, 512), (37, 200, 328), (300, 512, 1024)])
+@pytest.mark.parametrize("residual", [True, False])
+def test_block(mode, act, rows, d, h, residual):
+    """A feed-forward block: norm, product, (quantizer,) product and residual, from one token up."""
+    m = block(d, h, act, mode)
+    x = rand(rows, d, dtype=torch.bfloat16, seed=7)
+    r = rand(rows, d, dtype=torch.bfloat16, seed=8) if residual else None
+    out, s = m(x, r)
+    weights64(m)
+    want = block64(m, x.double(), r.double() if residual else None)
+    # The branch's values are rounded three times (n, hid, out), in 8 bits by half a step of 2^-3
+    # relative (2^-4), in bf16 2^-8, each the root of a sum over many: three halves of a step cover
+    # the norm of a row, and s itself one rounding of bf16.
+    half = 2.0 ** -4 if mode == "fp8" else 2.0 ** -8
+    branch = want - (x.double() + (r.double() if residual else 0.0))
+    assert float((out.double() - want).norm()) <= 3 * half * float(branch.norm()) + 2 * 2.0 ** -8 * float(want.norm())
+    assert torch.equal(s, (x.float() + r.float()).bfloat16() if residual else x)
+
+
+@pytest.mark.parametrize("act", ["gelu_tanh", "gelu", "silu", "relu"])
+@pytest.mark.parametrize("rows,d,h", [(5, 128, 256), (130, 256, 520)])
+def test_block_gradient(act, rows, d, h):
+    """The block's gradients against the 64-bit function's own."""
+    m = block(d, h, act, "bf16")
+    x, r = rand(rows, d, dtype=torch.bfloat16, seed=7), rand(rows, d, dtype=torch.bfloat16, seed=8)
+    dout = rand(rows, d, dtype=torch.bfloat16, seed=9)
+    m(x, r, keep=True)
+    got = m.backward(dout)
+    weights64(m)
+    x64 = x.double().requires_grad_()
+    for v in m.p.values():
+        v.requires_grad_()
+    block64(m, x64, r.double()).backward(dout.double())
+    want = {"dx": x64.grad, "dw1": m.p["w1"].grad, "db1": m.p["b1"].grad, "dw2": m.p["w2"].grad, "db2": m.p["b2"].grad,
+            "dnorm_weight": m.p["g"].grad}
+    for name, w in want.items():
+        # At most six values on the way are in bf16 (n, pre, hid, dhid, dz, dn): half a step each.
+        # The rectifier's slope jumps: where pre rounds across 0 no bound holds, which at these sizes
+        # touches under one value in a hundred of the branch.
+        rel = float((got[name].double() - w).norm() / w.norm())
+        assert rel <= 6 * 2.0 ** -8 + (0.1 if act == "relu" else 0.0), (name, rel)
+    with pytest.raises(ValueError):
+        m.backward(dout)  # nothing kept
+
+
+def test_block_refusals():
+    m = block(64, 128, "silu", "fp8")
+    x = rand(4, 64, dtype=torch.bfloat16)
+    for bad in (lambda: m(x.float()), lambda: m(rand(4, 32, dtype=torch.bfloat16)), lambda: m(x, x.float()), lambda: m(x, keep=True),
+                lambda: m(rand(64, 4, dtype=torch.bfloat16).T), lambda: block(64, 128, "tanh", "bf16"),
+                lambda: block(64, 128, "silu", "fp4")):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.parametrize("mode", ["bf16", "fp8"])
+def test_block_captured_and_replayed(mode):
+    """Two captured graphs of one block, replayed in turn with new inputs and beside eager calls."""
+    m = block(256, 512, "gelu_tanh", mode)
+    st = torch.cuda.Stream()
+    graphs = []
+    for rows in (3, 200):
+        x, r = rand(rows, 256, dtype=torch.bfloat16, seed=rows), rand(rows, 256, dtype=torch.bfloat16, seed=rows + 1)
+        with torch.cuda.stream(st):
+            m(x, r)
+            st.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                out, _ = m(x, r)
+        graphs.append((g, x, r, out))
+    for k in range(3):
+        for g, x, r, out in graphs:
+            x.copy_(rand(*x.shape, dtype=torch.bfloat16, seed=50 + k))
+            want = m(x, r)[0].clone()
+            out.zero_()
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+
+
+def test_gradient_captured_and_replayed():
+    m = block(256, 512, "silu", "bf16")
+    x, dout = rand(100, 256, dtype=torch.bfloat16), rand(100, 256, dtype=torch.bfloat16, seed=1)
+    st = torch.cuda.Stream()
+
+    def step():
+        m(x, keep=True)
+        return m.backward(dout)
+
+    with torch.cuda.stream(st):
+        step()
+        st.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            got = step()
+    for seed in (3, 4):
+        x.copy_(rand(100, 256, dtype=torch.bfloat16, seed=seed))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.cuda.synchronize()
+        for k in want:
+            assert torch.equal(got[k], want[k]), k
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on the GPU share nothing: scratch comes from the pool in stream order."""
+    calls = [Linear(200, 264, 133, act="gelu", residual=torch.bfloat16, seed=k) for k in range(2)]
+    want = []
+    for c in calls:
+        c.call()
+        torch.cuda.synchronize()
+        want.append(c.out.clone())
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(30):
+        for c, s in zip(calls, streams):
+            c.call(s.cuda_stream)
+    torch.cuda.synchronize()
+    for c, w in zip(calls, want):
+        assert torch.equal(c.out, w)
+
+
+def test_first_call_inside_a_capture():
+    """A process whose very first calls are captured: everything the library makes on first use is
+    made outside the capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from tensorforge_b200 import _lib
+a, b = torch.randn(40, 136, device="cuda").bfloat16(), torch.randn(72, 136, device="cuda").bfloat16()
+out, y, rstd = torch.zeros(40, 72, device="cuda"), torch.zeros(40, 136, device="cuda"), torch.ones(40, device="cuda")
+db, dw, dx = torch.zeros(72, 136, device="cuda"), torch.zeros(136, device="cuda"), torch.zeros(40, 136, device="cuda").bfloat16()
+dout = torch.randn(40, 72, device="cuda")
+torch.cuda.synchronize()
+st, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+with torch.cuda.stream(st):
+    with torch.cuda.graph(g, stream=st):
+        s = st.cuda_stream
+        _lib.linear(a.data_ptr(), b.data_ptr(), out.data_ptr(), 40, 72, 136, out_dtype=_lib.F32, trans_b=True, stream=s)
+        _lib.rms_norm(a.data_ptr(), y.data_ptr(), 40, 136, 1e-5, out_dtype=_lib.F32, stream=s)
+        _lib.linear_backward(dout.data_ptr(), a.data_ptr(), b.data_ptr(), 40, 72, 136, dB=db.data_ptr(), dtype=_lib.F32,
+                             grad_dtype=_lib.F32, trans_b=True, stream=s)
+        _lib.rms_norm_backward(a.data_ptr(), a.data_ptr(), rstd.data_ptr(), dx.data_ptr(), 40, 136, dweight=dw.data_ptr(), stream=s)
+g.replay()
+torch.cuda.synchronize()
+assert torch.allclose(out.double(), a.double() @ b.double().T, atol=1e-3)
+assert torch.allclose(y.double(), a.double() * (a.double().square().mean(1, keepdim=True) + 1e-5).rsqrt(), atol=1e-5)
+assert torch.allclose(db.double(), dout.bfloat16().double().T @ a.double(), atol=1e-3)
+assert torch.allclose(dw.double(), (a.double() * a.double()).sum(0), rtol=1e-5)
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parent.parent)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]

@@ -157,3 +157,12 @@ def test_forced_kernel_values():
     assert f(1, 64, 3) == _lib.ERR_MODE
     assert f(9, 0, 0) == _lib.ERR_MODE
     assert f(0, 0, 0) == _lib.OK
+
+
+def test_mlp_command_refuses_what_the_block_lacks(capsys):
+    from tensorforge_b200 import mlp
+
+    for argv in (["--mode", "fp8"], ["--block", "--mode", "fp32"], ["--block", "--mode", "tf32"], ["--train", "--mode", "bf16"],
+                 ["--block", "--mode", "fp8", "--train"]):
+        with pytest.raises(SystemExit):
+            mlp.main(argv)
