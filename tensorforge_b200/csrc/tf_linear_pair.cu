@@ -16,8 +16,8 @@
 // is brought into the staging by TMA one chunk ahead, so a tile's first while its MMAs run.
 //
 // With few stages of k a tile is bound by this epilogue: 4096 x 8192 x 256 bf16 with silu takes
-// 56 us with eight warps in two groups that meet at barriers, EPI_SILU us as it is here; with the
-// bf16 residual 95 and EPI_RES.
+// 56 us with eight warps in two groups that meet at barriers and read the residual themselves, 46 as
+// it is here; with the bf16 residual 95 and 59.
 //
 // 640 threads: warp 0 TMA producer (both CTAs), warp 1 MMA issuer (leader), warps 4..19 epilogue.
 // Every wait is bounded (tf_ptx.cuh); after an expiry each role stops, the producer, the issuer and
@@ -33,18 +33,22 @@ namespace tf {
 
 namespace {
 
-constexpr int kPairStages = 5;
 constexpr int kEpiWarps = 16;
 
+// Two divisions of the shared memory: five stages and 4 KB of staging an epilogue warp, for every
+// call; six stages and 2 KB (deep), for many stages of k and bf16 rows on 16-byte boundaries whose
+// chunk needs one box at a time (pair_deep).
+template <bool DEEP>
 struct PairL {
+  static constexpr int kStages = DEEP ? 6 : 5;
   static constexpr int kThreads = 128 + 32 * kEpiWarps;
   static constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kBoxOff = kPairStages * kStageBytes;
-  static constexpr int kBoxBytes = 32 * 128;  // an epilogue warp's: 32 rows x 32 f32, or two of 32 bf16
+  static constexpr int kBoxOff = kStages * kStageBytes;
+  static constexpr int kBoxBytes = DEEP ? 2048 : 4096;  // 32 rows x 32 bf16; or f32, or two of bf16
   static constexpr int kBarOff = kBoxOff + kEpiWarps * kBoxBytes;
   // full[], empty[], accf[2], acce[2], drain, resf[warps]; then the TMEM slot and the abort flag.
-  static constexpr int kNumBars = 2 * kPairStages + 5 + kEpiWarps;
+  static constexpr int kNumBars = 2 * kStages + 5 + kEpiWarps;
   static constexpr int kSmemBytes = 1024 + kBarOff + 8 * kNumBars + 16;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
@@ -172,13 +176,13 @@ __device__ __forceinline__ void store_turned(const LinearParams &p, float *buf, 
 }
 
 // F8: e4m3 operands (both K-major).  AMN / BMN: A / B is MN-major (bf16).
-template <bool F8, bool AMN, bool BMN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
+template <bool F8, bool AMN, bool BMN, bool DEEP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmP,
                        const __grid_constant__ CUtensorMap tmR, const LinearParams p) {
-  using L = PairL;
-  constexpr int STAGES = kPairStages;
+  using L = PairL<DEEP>;
+  constexpr int STAGES = L::kStages;
   static_assert(!F8 || (!AMN && !BMN), "8-bit operands are K-major");
   constexpr int kBK = F8 ? 128 : 64;
   constexpr uint32_t kIdesc = instr_desc_majors(F8 ? 0u : 1u, 256, 256, AMN, BMN);
@@ -332,11 +336,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
     const int part = (warp - 4) >> 2, q = warp & 3;
     const uint32_t lead_acce0 = map_to_cta(acce0, 0), resf = resf0 + 8 * (warp - 4);
     uint8_t *box = smem + L::kBoxOff + (warp - 4) * L::kBoxBytes;
-    const bool bf16 = p.out_bf16 != 0, pre = p.pre != nullptr, pingpong = bf16 && !pre && !p.residual;
+    const bool bf16 = DEEP || p.out_bf16, pre = p.pre != nullptr, vec = DEEP || p.vec, res_bf16 = DEEP || p.res_bf16;
+    const bool pingpong = !DEEP && bf16 && !pre && !p.residual;
     // The residual comes by TMA into the box, in whose place the chunk's output is then staged, but
     // where pre needs the box first (f32 out or residual with pre): then by the row's own loads.
-    const bool res_tma = p.residual && p.vec && !(pre && (!bf16 || !p.res_bf16));
-    const uint32_t res_bytes = p.res_bf16 ? 2048u : 4096u;
+    const bool res_tma = p.residual && vec && !(pre && (!bf16 || !res_bf16));
+    const uint32_t res_bytes = res_bf16 ? 2048u : 4096u;
     uint32_t turn = 0, res_phase = 0;
     bool res_flight = false;
     auto tile_at = [&](int i, int &m0, int &n0) {
@@ -400,7 +405,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rr[j]) + __shfl_sync(0xFFFFFFFFu, bl, j);
         }
-        if (p.vec && !res_tma) {
+        if (vec && !res_tma) {
           // The box is free once the stores issued from it have read it: all but the last one when it
           // has two bf16 halves to alternate between.
           if (lane == 0) {
@@ -410,18 +415,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
           __syncwarp();
         }
         if (pre) {
-          if (!p.vec) {
+          if (!vec) {
             float *buf = reinterpret_cast<float *>(box);
             if (bf16) store_turned(p, buf, lane, m0, col0, static_cast<__nv_bfloat16 *>(p.pre), p.ldp, false, v);
             else store_turned(p, buf, lane, m0, col0, static_cast<float *>(p.pre), p.ldp, false, v);
           } else {
-            stage_row(bf16 ? box + 2048 : box, lane, bf16, v);
+            const bool beside = !DEEP && bf16;  // the output has a place of its own
+            uint8_t *pbox = beside ? box + 2048 : box;
+            stage_row(pbox, lane, bf16, v);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_2d(&tmP, smem_u32(bf16 ? box + 2048 : box), col0, m0);
+              tma_store_2d(&tmP, smem_u32(pbox), col0, m0);
               bulk_commit_group();
-              if (!bf16) bulk_wait_group_read0();  // f32: the box holds one chunk at a time
+              if (!beside) bulk_wait_group_read0();
             }
             __syncwarp();
           }
@@ -430,7 +437,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = activate<decltype(act)::value>(v[j]);
         });
-        if (!p.vec) {
+        if (!vec) {
           float *buf = reinterpret_cast<float *>(box);
           if (bf16) store_turned(p, buf, lane, m0, col0, static_cast<__nv_bfloat16 *>(p.out), p.ldo, p.residual != nullptr, v);
           else store_turned(p, buf, lane, m0, col0, static_cast<float *>(p.out), p.ldo, p.residual != nullptr, v);
@@ -441,7 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
           if (!ok) break;
           res_phase ^= 1u;
           res_flight = false;
-          add_staged(box, lane, p.res_bf16 != 0, v);
+          add_staged(box, lane, res_bf16, v);
           __syncwarp();  // every row has been read before the output takes its place
         } else if (p.residual && m0 + lane < p.M) {
           add_row(p, m0 + lane, col0, v);
@@ -477,22 +484,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL::kThreads, 1)
 }
 
 // Co-resident clusters of one instantiation on the current device (0 on failure).
-template <bool F8, bool AMN, bool BMN>
+template <bool F8, bool AMN, bool BMN, bool DEEP>
 int pair_clusters() {
-  auto kern = linear_pair_kernel<F8, AMN, BMN>;
+  using L = PairL<DEEP>;
+  auto kern = linear_pair_kernel<F8, AMN, BMN, DEEP>;
   static int cached[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   int *slot = &cached[dev & 63];
   int v = __atomic_load_n(slot, __ATOMIC_ACQUIRE);
   if (v > 0) return v;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PairL::kSmemBytes) != cudaSuccess) return 0;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes) != cudaSuccess) return 0;
   int sms = 0;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * (sms / 2 > 0 ? sms / 2 : 1), 1, 1);
-  cfg.blockDim = dim3(PairL::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = PairL::kSmemBytes;
+  cfg.blockDim = dim3(L::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::kSmemBytes;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -508,18 +516,34 @@ int pair_clusters() {
   return n;
 }
 
-template <bool F8, bool AMN, bool BMN>
-cudaError_t launch_pair(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmO, const CUtensorMap &tmP,
+template <bool F8, bool AMN, bool BMN, bool DEEP>
+cudaError_t launch_pair_form(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmO, const CUtensorMap &tmP,
                         const CUtensorMap &tmR, const LinearParams &p, cudaStream_t st) {
-  const int clusters = pair_clusters<F8, AMN, BMN>();
+  using L = PairL<DEEP>;
+  const int clusters = pair_clusters<F8, AMN, BMN, DEEP>();
   if (clusters <= 0) return cudaErrorInvalidConfiguration;
   const int64_t tiles = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
   if (tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
   const int pairs = tiles < clusters ? (int)tiles : clusters;
   cudaLaunchAttribute attr[1];
   pdl_attr(attr[0]);
-  cudaLaunchConfig_t cfg = {dim3(2 * pairs), dim3(PairL::kThreads), (size_t)PairL::kSmemBytes, st, attr, 1};
-  return cudaLaunchKernelEx(&cfg, linear_pair_kernel<F8, AMN, BMN>, tmA, tmB, tmO, tmP, tmR, p);
+  cudaLaunchConfig_t cfg = {dim3(2 * pairs), dim3(L::kThreads), (size_t)L::kSmemBytes, st, attr, 1};
+  return cudaLaunchKernelEx(&cfg, linear_pair_kernel<F8, AMN, BMN, DEEP>, tmA, tmB, tmO, tmP, tmR, p);
+}
+
+// The deep form from 32 stages of k: 4096 x 16384 x 4096 bf16 424 us and, with tanh gelu and pre, 447
+// (five stages 434 and 459; calls in a row under the power cap).  With few stages the epilogue's
+// second box counts for more.  It takes bf16 outputs whose rows start on 16-byte boundaries, with pre
+// or a bf16 residual but not both.
+bool pair_deep(const LinearParams &p, int esz) {
+  return (int64_t)p.K * esz >= 32 * 128 && p.out_bf16 && p.vec && !(p.pre && p.residual) && (!p.residual || p.res_bf16);
+}
+
+template <bool F8, bool AMN, bool BMN>
+cudaError_t launch_pair(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmO, const CUtensorMap &tmP,
+                        const CUtensorMap &tmR, const LinearParams &p, cudaStream_t st) {
+  return pair_deep(p, F8 ? 1 : 2) ? launch_pair_form<F8, AMN, BMN, true>(tmA, tmB, tmO, tmP, tmR, p, st)
+                                  : launch_pair_form<F8, AMN, BMN, false>(tmA, tmB, tmO, tmP, tmR, p, st);
 }
 
 }  // namespace
