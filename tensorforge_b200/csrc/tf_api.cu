@@ -616,6 +616,27 @@ int encode_rows_map(CUtensorMap *m, const void *base, int esz, int64_t rows, int
   return TFORGE_OK;
 }
 
+int encode_mn_map(CUtensorMap *m, const void *base, int64_t rows, int64_t cols, int64_t ld, uint32_t n, int32_t *blocks) {
+  *blocks = cols % 64 == 0;
+  if (!*blocks) return encode_rows_map(m, base, 2, rows, cols, ld, 64, 64);
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) {
+    g_last_error = "cuTensorMapEncodeTiled unavailable";
+    return TFORGE_ERR_CUDA;
+  }
+  cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)(cols / 64)};
+  cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), 128};
+  cuuint32_t box[3] = {64, 64, n}, estr[3] = {1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    g_last_error = "cuTensorMapEncodeTiled failed for an MN-major operand (" + std::to_string((int)r) + ")";
+    return TFORGE_ERR_CUDA;
+  }
+  return TFORGE_OK;
+}
+
 int encode_out_map(CUtensorMap *m, const void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld) {
   return make_tmap(m, base, bf16, rows, cols, ld, 32, 32, bf16 ? SW64 : SW128);
 }

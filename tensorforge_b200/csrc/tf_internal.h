@@ -184,6 +184,10 @@ int device_status_word(uint32_t **out);
 // The error text and TFORGE_ERR_CUDA of a failed CUDA call (tf_api.cu).
 int cuda_failure(cudaError_t e, const char *what);
 
+// Tensor map of an MN-major bf16 operand, stored rows (of k) x cols: *blocks = 1 and boxes of `n` blocks
+// of 64 columns x 64 rows if cols is a multiple of 64 (in others a block would reach over a row's
+// end), else boxes of one block.
+int encode_mn_map(CUtensorMap *m, const void *base, int64_t rows, int64_t cols, int64_t ld, uint32_t n, int32_t *blocks);
 // Tensor map of bf16 (esz 2) or 8-bit (esz 1) rows, boxes in the 128-byte swizzle (tf_api.cu).
 int encode_rows_map(CUtensorMap *m, const void *base, int esz, int64_t rows, int64_t cols, int64_t ld,
                     uint32_t box_cols, uint32_t box_rows);
@@ -202,13 +206,15 @@ struct LinearParams {
   uint64_t limit_ns;              // bounded-wait limit
   int32_t debug_skip;             // test hook: skip the first stage's loads
   int32_t splits;                 // slim kernel: CTAs that share a tile's k (1, 2, 4 or 8)
+  // 1: the rows' (columns') operand is MN-major and its map has blocks (encode_mn_map).
+  int32_t rows_blocks, cols_blocks;
   // Every array of the epilogue that is there starts its rows on 16-byte boundaries: the pair kernel
   // then stores tiles by TMA (tmO, tmP), the slim kernel eight columns at a time.
   int32_t vec;
 };
 // One-CTA kernel of 128 columns x bt tokens (16, 32, 64, 128, 256; from 64 with t_mn).  tmT: A as
-// {128 B of k x bt rows} boxes, or with t_mn (A stored k x m) {64 columns x 64 rows}; tmW: B stored
-// n x k as {128 B x 128 rows} boxes, or with w_mn (stored k x n) {64 columns x 64 rows}.
+// {128 B of k x bt rows} boxes, or with t_mn (A stored k x m) an encode_mn_map of bt / 64 blocks; tmW:
+// B stored n x k as {128 B x 128 rows} boxes, or with w_mn (stored k x n) an encode_mn_map of two.
 cudaError_t launch_linear_slim(bool f8, bool w_mn, bool t_mn, int bt, const CUtensorMap &tmT, const CUtensorMap &tmW,
                                const LinearParams &p, cudaStream_t stream);
 

@@ -303,8 +303,8 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
   if (c.tile == 0) {
     CUtensorMap tmA{}, tmB{}, tmO{}, tmP{}, tmR{};
     const uint32_t bk = 128 / esz;
-    rc = t_mn ? encode_rows_map(&tmA, rows.p, esz, K, M, rows.ld, 64, 64) : encode_rows_map(&tmA, rows.p, esz, M, K, rows.ld, bk, 128);
-    if (!rc) rc = w_mn ? encode_rows_map(&tmB, cols.p, esz, K, N, cols.ld, 64, 64) : encode_rows_map(&tmB, cols.p, esz, N, K, cols.ld, bk, 128);
+    rc = t_mn ? encode_mn_map(&tmA, rows.p, K, M, rows.ld, 2, &p.rows_blocks) : encode_rows_map(&tmA, rows.p, esz, M, K, rows.ld, bk, 128);
+    if (!rc) rc = w_mn ? encode_mn_map(&tmB, cols.p, K, N, cols.ld, 2, &p.cols_blocks) : encode_rows_map(&tmB, cols.p, esz, N, K, cols.ld, bk, 128);
     if (!rc && p.vec) rc = encode_out_map(&tmO, p.out, p.out_bf16 != 0, M, N, p.ldo);
     if (!rc && p.vec && p.pre) rc = encode_out_map(&tmP, p.pre, p.out_bf16 != 0, M, N, p.ldp);
     if (!rc && p.vec && p.residual) rc = encode_out_map(&tmR, p.residual, p.res_bf16 != 0, M, N, p.ldr);
@@ -316,10 +316,10 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
   CUtensorMap tmT{}, tmW{};
   if (K > 0) {
     const uint32_t bk = 128 / esz;
-    rc = t_mn ? encode_rows_map(&tmT, rows.p, esz, K, M, rows.ld, 64, 64)
+    rc = t_mn ? encode_mn_map(&tmT, rows.p, K, M, rows.ld, (uint32_t)c.tile / 64, &p.rows_blocks)
               : encode_rows_map(&tmT, rows.p, esz, M, K, rows.ld, bk, (uint32_t)c.tile);
     if (rc) return rc;
-    rc = w_mn ? encode_rows_map(&tmW, cols.p, esz, K, N, cols.ld, 64, 64)
+    rc = w_mn ? encode_mn_map(&tmW, cols.p, K, N, cols.ld, 2, &p.cols_blocks)
               : encode_rows_map(&tmW, cols.p, esz, N, K, cols.ld, bk, 128);
     if (rc) return rc;
   }

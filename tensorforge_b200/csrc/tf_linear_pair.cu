@@ -175,6 +175,18 @@ __device__ __forceinline__ void store_turned(const LinearParams &p, float *buf, 
   __syncwarp();
 }
 
+// This CTA's 128 columns from c0 of an MN-major operand, 64 rows of k: two blocks of 64 columns, in one
+// load where the map has blocks.  One load instead of two: 8192 x 4096 x 16384's weight gradient,
+// both operands MN-major, 870 -> 830 us (calls in a row under the power cap).
+__device__ __forceinline__ void load_mn(uint32_t dst, const void *tmap, int32_t blocks, int c0, int kc, uint32_t bar) {
+  if (blocks) {
+    tma_load_3d_pair(dst, tmap, 0, kc, c0 / 64, bar);
+  } else {
+    tma_load_2d_pair(dst, tmap, c0, kc, bar);
+    tma_load_2d_pair(dst + 8192, tmap, c0 + 64, kc, bar);
+  }
+}
+
 // F8: e4m3 operands (both K-major).  AMN / BMN: A / B is MN-major (bf16).
 template <bool F8, bool AMN, bool BMN, bool DEEP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThreads, 1)
@@ -259,14 +271,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThread
         const uint32_t slot = sbase + s * L::kStageBytes, bar = lead_full0 + 8 * s;
         if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * L::kStageBytes);
         if constexpr (AMN) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) tma_load_2d_pair(slot + j * 8192, &tmA, m0 + 64 * j, kc, bar);
+          load_mn(slot, &tmA, p.rows_blocks, m0, kc, bar);
         } else {
           tma_load_2d_pair(slot, &tmA, kc, m0, bar);
         }
         if constexpr (BMN) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) tma_load_2d_pair(slot + L::kABytes + j * 8192, &tmB, n0 + 64 * j, kc, bar);
+          load_mn(slot + L::kABytes, &tmB, p.cols_blocks, n0, kc, bar);
         } else {
           tma_load_2d_pair(slot + L::kABytes, &tmB, kc, n0, bar);
         }

@@ -226,15 +226,24 @@ __global__ void __launch_bounds__(256)
       const uint32_t slot = sbase + s * L::kStageBytes, bar = full0 + 8 * s;
       const int kc = (kb0 + kb) * kBK;
       mbar_arrive_expect_tx(bar, L::kStageBytes);
+      // MN-major: blocks of 64 columns, in one load where the map has blocks.
       if constexpr (WMN) {
+        if (p.cols_blocks) {
+          tma_load_3d(slot, &tmW, 0, kc, n0 / 64, bar);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) tma_load_2d(slot + j * 8192, &tmW, n0 + 64 * j, kc, bar);
+          for (int j = 0; j < 2; ++j) tma_load_2d(slot + j * 8192, &tmW, n0 + 64 * j, kc, bar);
+        }
       } else {
         tma_load_2d(slot, &tmW, kc, n0, bar);
       }
       if constexpr (TMN) {
+        if (p.rows_blocks) {
+          tma_load_3d(slot + L::kWBytes, &tmT, 0, kc, m0 / 64, bar);
+        } else {
 #pragma unroll
-        for (int j = 0; j < BT / 64; ++j) tma_load_2d(slot + L::kWBytes + j * 8192, &tmT, m0 + 64 * j, kc, bar);
+          for (int j = 0; j < BT / 64; ++j) tma_load_2d(slot + L::kWBytes + j * 8192, &tmT, m0 + 64 * j, kc, bar);
+        }
       } else {
         tma_load_2d(slot + L::kWBytes, &tmT, kc, m0, bar);
       }
