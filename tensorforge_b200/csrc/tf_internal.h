@@ -208,6 +208,9 @@ struct LinearParams {
   int32_t splits;                 // slim kernel: CTAs that share a tile's k (1, 2, 4 or 8)
   // 1: the rows' (columns') operand is MN-major and its map has blocks (encode_mn_map).
   int32_t rows_blocks, cols_blocks;
+  // f32 outputs: stages of k after which the tensor core's sum is put aside and begun anew
+  // (tf_epilogue.cuh); 0: not.
+  int32_t sum_stages;
   // Every array of the epilogue that is there starts its rows on 16-byte boundaries: the pair kernel
   // then stores tiles by TMA (tmO, tmP), the slim kernel eight columns at a time.
   int32_t vec;

@@ -250,8 +250,11 @@ struct Choice {
 //           0.55 of that (one with 256 rows); smoothly no less than 1.17 x memory; per round of
 //           resident CTAs 2.6 us and what a cluster of S costs to meet; per CTA on an SM the
 //           epilogue's rows.
-Choice choose(int64_t M, int64_t N, int64_t K, bool t_mn, int esz) {
+// f32 outputs take only kernels that sum in pieces short enough: the pair kernel always can, the slim
+// kernel's accumulators share a CTA's k.
+Choice choose(int64_t M, int64_t N, int64_t K, bool t_mn, int esz, bool f32_out) {
   const double nkb = (double)((K * esz + 127) / 128);
+  const double most = f32_out ? (esz == 1 ? 64.0 : 12.0) : 1e300;  // stages of k in one sum
   const double memory = ((double)esz * K * (M + N) + 2.0 * M * N) / 6.55e6;
   const double tiles256 = std::ceil(M / 256.0) * std::ceil(N / 256.0);
   Choice best{0, 1};
@@ -261,6 +264,7 @@ Choice choose(int64_t M, int64_t N, int64_t K, bool t_mn, int esz) {
   for (int tile = t_mn ? 64 : 16; tile <= 256; tile *= 2) {
     const double tiles = std::ceil((double)M / tile) * std::ceil(N / 128.0), live = M < tile ? (double)M : tile;
     for (int s = 1; s <= 8; s *= 2) {
+      if (std::ceil(nkb / s) > most * (256 / tile)) continue;
       // CTAs that the SMs hold at once: clusters of 4 and 8 do not find a place on every SM.
       const double slots = tile == 256 ? (s <= 2 ? 148 : s == 4 ? 132 : 120) : (s <= 2 ? 296 : s == 4 ? 284 : 264);
       const double ctas = tiles * s, deep = std::ceil(ctas / 148.0), rounds = std::ceil(ctas / slots);
@@ -295,11 +299,14 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
   const int eo = p.out_bf16 ? 2 : 4;
   p.vec = rows16(p.out, p.ldo, eo) && rows16(p.pre, p.ldp, eo) && rows16(p.residual, p.ldr, p.res_bf16 ? 2 : 4) &&
           at(p.bias, 16) && at(p.b_scale, 16);
-  Choice c = choose(M, N, K, t_mn, esz);
+  Choice c = choose(M, N, K, t_mn, esz, !p.out_bf16);
   const uint32_t force = g_force.load();
   if ((force & 255) == 1) c = Choice{(int)((force >> 8) & 0xFFFF), (int)(force >> 24)};
   else if ((force & 255) == 2) c = Choice{0, 1};
   if ((c.tile == 0 && K == 0) || (c.tile != 0 && t_mn && c.tile < 64)) return TFORGE_ERR_UNSUPPORTED;
+  // f32 outputs: sums in pieces (of the pair kernel; the slim kernel divides its k by its accumulators).
+  const int64_t stages = (K * esz + 127) / 128, piece = f8 ? 64 : 8;
+  p.sum_stages = !p.out_bf16 && stages > piece ? (int32_t)piece : 0;
   if (c.tile == 0) {
     CUtensorMap tmA{}, tmB{}, tmO{}, tmP{}, tmR{};
     const uint32_t bk = 128 / esz;

@@ -35,6 +35,10 @@ namespace {
 
 constexpr int kEpiWarps = 16;
 
+// Forms of the kernel: any call; many stages of k (DEEP); f32 outputs over a long k, whose sums are
+// taken in pieces of p.sum_stages stages (SUMS).
+enum Form : int { FORM_ANY = 0, FORM_DEEP = 1, FORM_SUMS = 2 };
+
 // Two divisions of the shared memory: five stages and 4 KB of staging an epilogue warp, for every
 // call; six stages and 2 KB (deep), for many stages of k and bf16 rows on 16-byte boundaries whose
 // chunk needs one box at a time (pair_deep).
@@ -188,11 +192,12 @@ __device__ __forceinline__ void load_mn(uint32_t dst, const void *tmap, int32_t 
 }
 
 // F8: e4m3 operands (both K-major).  AMN / BMN: A / B is MN-major (bf16).
-template <bool F8, bool AMN, bool BMN, bool DEEP>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThreads, 1)
+template <bool F8, bool AMN, bool BMN, int FORM>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_DEEP>::kThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmP,
                        const __grid_constant__ CUtensorMap tmR, const LinearParams p) {
+  constexpr bool DEEP = FORM == FORM_DEEP, SUMS = FORM == FORM_SUMS;
   using L = PairL<DEEP>;
   constexpr int STAGES = L::kStages;
   static_assert(!F8 || (!AMN && !BMN), "8-bit operands are K-major");
@@ -220,6 +225,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThread
   const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
   const int my_tiles = pair < tiles ? (tiles - 1 - pair) / npairs + 1 : 0;
   const int nkb = (p.K + kBK - 1) / kBK;
+  // Pieces of a tile's k, an accumulator each in turn.
+  const int per = SUMS ? p.sum_stages : nkb, pieces = SUMS ? (nkb + per - 1) / per : 1;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -305,12 +312,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThread
     int s = 0;
     uint32_t phase = 0, bar = full0;
     uint64_t so = 0;
-    for (int i = 0; i < my_tiles && ok; ++i) {
-      const int b = i & 1;
+    for (int u = 0; u < my_tiles * pieces && ok; ++u) {
+      const int b = u & 1;
       const uint32_t acc = tmem + 256u * b;
-      if (i >= 2 && !mbar_wait_cluster(acce0 + 8 * b, ((i >> 1) - 1) & 1, wc)) break;
+      if (u >= 2 && !mbar_wait_cluster(acce0 + 8 * b, ((u >> 1) - 1) & 1, wc)) break;
       tc_fence_after();
-      for (int kb = 0; kb < nkb; ++kb) {
+      const int kb0 = SUMS ? u % pieces * per : 0, kb1 = SUMS && kb0 + per < nkb ? kb0 + per : nkb;
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait_cluster(bar, phase, wc)) {
           ok = false;
           break;
@@ -319,8 +327,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThread
         const uint64_t ad = a_d0 + so, bd = b_d0 + so;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          if constexpr (F8) mma_ss_pair_f8(acc, ad + ks * kAStep, bd + ks * kBStep, kIdesc, (kb | ks) ? 1u : 0u);
-          else mma_ss_pair<false>(acc, ad + ks * kAStep, bd + ks * kBStep, kIdesc, (kb | ks) ? 1u : 0u);
+          const uint32_t add = kb != kb0 || ks ? 1u : 0u;
+          if constexpr (F8) mma_ss_pair_f8(acc, ad + ks * kAStep, bd + ks * kBStep, kIdesc, add);
+          else mma_ss_pair<false>(acc, ad + ks * kAStep, bd + ks * kBStep, kIdesc, add);
         }
         mma_commit_pair(bar + 8 * STAGES, 0x3);
         if (++s == STAGES) {
@@ -346,7 +355,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThread
     const int part = (warp - 4) >> 2, q = warp & 3;
     const uint32_t lead_acce0 = map_to_cta(acce0, 0), resf = resf0 + 8 * (warp - 4);
     uint8_t *box = smem + L::kBoxOff + (warp - 4) * L::kBoxBytes;
-    const bool bf16 = DEEP || p.out_bf16, pre = p.pre != nullptr, vec = DEEP || p.vec, res_bf16 = DEEP || p.res_bf16;
+    const bool bf16 = !SUMS && (DEEP || p.out_bf16), pre = p.pre != nullptr, vec = DEEP || p.vec, res_bf16 = DEEP || p.res_bf16;
     const bool pingpong = !DEEP && bf16 && !pre && !p.residual;
     // The residual comes by TMA into the box, in whose place the chunk's output is then staged, but
     // where pre needs the box first (f32 out or residual with pre): then by the row's own loads.
@@ -379,10 +388,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThread
     bool ok = true;
 #pragma unroll 1
     for (int i = 0; i < my_tiles && ok; ++i) {
-      const int b = i & 1;
+      const int u = i * pieces + pieces - 1, b = u & 1;  // the tile's last piece
       const float sa = p.a_scale && m0 + lane < p.M ? __ldg(p.a_scale + m0 + lane) : 1.f;
       int m1 = 0, n1 = 0;  // the next tile
       if (i + 1 < my_tiles) tile_at(i + 1, m1, n1);
+      const uint32_t lanes = (uint32_t)(q * 32) << 16;
+      if constexpr (SUMS) {
+        // The pieces' sums, in order, in registers; then back into the last piece's accumulator, from
+        // where they go on as a whole sum would.
+        float sum[64];
+#pragma unroll
+        for (int j = 0; j < 64; ++j) sum[j] = 0.f;
+#pragma unroll 1
+        for (int w = i * pieces; w <= u && ok; ++w) {
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(accf0 + 8 * (w & 1), (w >> 1) & 1, wc, 64));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            uint32_t rr[8];
+            tmem_ld_32x32b_x8(tmem + 256u * (w & 1) + lanes + (part + 4 * (g / 4)) * 32 + g % 4 * 8, rr);
+            tmem_ld_wait(rr);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[8 * g + j] += __uint_as_float(rr[j]);
+          }
+          if (w < u) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(lead_acce0 + 8 * (w & 1));
+          }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t rr[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) rr[j] = __float_as_uint(sum[32 * k + j]);
+          tmem_st_32x32b_x32(tmem + 256u * b + lanes + (part + 4 * k) * 32, rr);
+        }
+        tmem_st_wait();
+      }
       // Not unrolled: the body, with an activation's 32 copies, should stay in the instruction cache.
 #pragma unroll 1
       for (int k = 0; k < 2; ++k) {
@@ -390,14 +435,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThread
         const bool live = inside(m0, col0), lane_col = live && col0 + lane < p.N;
         const float bl = p.bias && lane_col ? __ldg(p.bias + col0 + lane) : 0.f;
         const float sl = p.b_scale && lane_col ? __ldg(p.b_scale + col0 + lane) : 1.f;
-        if (k == 0) {
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(accf0 + 8 * b, (i >> 1) & 1, wc, 64));
+        if (!SUMS && k == 0) {
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(accf0 + 8 * b, (u >> 1) & 1, wc, 64));
           if (!ok) break;
           tc_fence_after();
         }
         uint32_t rr[32];
         if (live) {
-          tmem_ld_32x32b_x32(tmem + 256u * b + ((uint32_t)(q * 32) << 16) + c * 32, rr);
+          tmem_ld_32x32b_x32(tmem + 256u * b + lanes + c * 32, rr);
           tmem_ld_wait(rr);
         }
         if (k == 1) {  // this warp's last read of accumulator b is done: release it
@@ -494,10 +539,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<DEEP>::kThread
 }
 
 // Co-resident clusters of one instantiation on the current device (0 on failure).
-template <bool F8, bool AMN, bool BMN, bool DEEP>
+template <bool F8, bool AMN, bool BMN, int FORM>
 int pair_clusters() {
-  using L = PairL<DEEP>;
-  auto kern = linear_pair_kernel<F8, AMN, BMN, DEEP>;
+  using L = PairL<FORM == FORM_DEEP>;
+  auto kern = linear_pair_kernel<F8, AMN, BMN, FORM>;
   static int cached[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
@@ -526,11 +571,11 @@ int pair_clusters() {
   return n;
 }
 
-template <bool F8, bool AMN, bool BMN, bool DEEP>
+template <bool F8, bool AMN, bool BMN, int FORM>
 cudaError_t launch_pair_form(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmO, const CUtensorMap &tmP,
                         const CUtensorMap &tmR, const LinearParams &p, cudaStream_t st) {
-  using L = PairL<DEEP>;
-  const int clusters = pair_clusters<F8, AMN, BMN, DEEP>();
+  using L = PairL<FORM == FORM_DEEP>;
+  const int clusters = pair_clusters<F8, AMN, BMN, FORM>();
   if (clusters <= 0) return cudaErrorInvalidConfiguration;
   const int64_t tiles = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
   if (tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
@@ -538,7 +583,7 @@ cudaError_t launch_pair_form(const CUtensorMap &tmA, const CUtensorMap &tmB, con
   cudaLaunchAttribute attr[1];
   pdl_attr(attr[0]);
   cudaLaunchConfig_t cfg = {dim3(2 * pairs), dim3(L::kThreads), (size_t)L::kSmemBytes, st, attr, 1};
-  return cudaLaunchKernelEx(&cfg, linear_pair_kernel<F8, AMN, BMN, DEEP>, tmA, tmB, tmO, tmP, tmR, p);
+  return cudaLaunchKernelEx(&cfg, linear_pair_kernel<F8, AMN, BMN, FORM>, tmA, tmB, tmO, tmP, tmR, p);
 }
 
 // The deep form from 32 stages of k: 4096 x 16384 x 4096 bf16 424 us and, with tanh gelu and pre, 447
@@ -552,8 +597,9 @@ bool pair_deep(const LinearParams &p, int esz) {
 template <bool F8, bool AMN, bool BMN>
 cudaError_t launch_pair(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmO, const CUtensorMap &tmP,
                         const CUtensorMap &tmR, const LinearParams &p, cudaStream_t st) {
-  return pair_deep(p, F8 ? 1 : 2) ? launch_pair_form<F8, AMN, BMN, true>(tmA, tmB, tmO, tmP, tmR, p, st)
-                                  : launch_pair_form<F8, AMN, BMN, false>(tmA, tmB, tmO, tmP, tmR, p, st);
+  if (p.sum_stages) return launch_pair_form<F8, AMN, BMN, FORM_SUMS>(tmA, tmB, tmO, tmP, tmR, p, st);
+  return pair_deep(p, F8 ? 1 : 2) ? launch_pair_form<F8, AMN, BMN, FORM_DEEP>(tmA, tmB, tmO, tmP, tmR, p, st)
+                                  : launch_pair_form<F8, AMN, BMN, FORM_ANY>(tmA, tmB, tmO, tmP, tmR, p, st);
 }
 
 }  // namespace

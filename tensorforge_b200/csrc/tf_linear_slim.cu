@@ -39,7 +39,8 @@ struct SlimLayout {
   static constexpr int kBarOff = kRing;
   // full[STAGES], empty[STAGES], accf; then the TMEM slot and the abort flag.
   static constexpr int kSmemBytes = 1024 + kBarOff + 8 * (2 * STAGES + 1) + 16;
-  static constexpr int kTmemCols = BT < 32 ? 32 : BT;
+  // Columns of one accumulator and, for sums in pieces, of as many as two CTAs an SM can have.
+  static constexpr int kTmemCols = BT < 32 ? 32 : BT, kSumCols = 256, kAccs = kSumCols / BT;
   static_assert(BT * 512 <= kRing, "the partial sums reuse the ring");
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
@@ -205,8 +206,11 @@ __global__ void __launch_bounds__(256)
       tma_prefetch_desc(&tmW);
     }
   }
+  // Accumulators of `per` stages each, BT columns apart (one of all stages unless p.sum_stages).
+  const int per = p.sum_stages ? max(1, (nkb + L::kAccs - 1) / L::kAccs) : max(1, nkb), accs = (nkb + per - 1) / per;
+  const uint32_t tmem_cols = p.sum_stages ? L::kSumCols : L::kTmemCols;
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), L::kTmemCols);
+    tmem_alloc(smem_u32(tmem_slot), tmem_cols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -261,16 +265,20 @@ __global__ void __launch_bounds__(256)
     const uint64_t w_d0 = WMN ? MN::desc(sbase, 0, false) : smem_desc(sbase, 16, 1024, 2);
     const uint64_t t_d0 = TMN ? MN::desc(sbase + L::kWBytes, 0, false) : smem_desc(sbase + L::kWBytes, 16, 1024, 2);
     constexpr uint32_t kWStep = WMN ? MN::step(false) >> 4 : 2u, kTStep = TMN ? MN::step(false) >> 4 : 2u;
-    int s = 0;
-    uint32_t phase = 0;
+    int s = 0, piece = 0;  // stages in the current accumulator
+    uint32_t phase = 0, acc = tmem;
     uint64_t so = 0;
     for (int kb = 0; kb < nkb; ++kb) {
       if (!mbar_wait(full0 + 8 * s, phase, wc)) break;
       tc_fence_after();
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        if constexpr (F8) mma_ss_f8(tmem, w_d0 + so + ks * kWStep, t_d0 + so + ks * kTStep, kIdesc, (kb | ks) ? 1u : 0u);
-        else mma_ss<false>(tmem, w_d0 + so + ks * kWStep, t_d0 + so + ks * kTStep, kIdesc, (kb | ks) ? 1u : 0u);
+        if constexpr (F8) mma_ss_f8(acc, w_d0 + so + ks * kWStep, t_d0 + so + ks * kTStep, kIdesc, (piece | ks) ? 1u : 0u);
+        else mma_ss<false>(acc, w_d0 + so + ks * kWStep, t_d0 + so + ks * kTStep, kIdesc, (piece | ks) ? 1u : 0u);
+      }
+      if (++piece == per) {
+        piece = 0;
+        acc += BT;
       }
       mma_commit(empty0 + 8 * s);
       so += L::kStageBytes >> 4;
@@ -296,16 +304,20 @@ __global__ void __launch_bounds__(256)
   const uint32_t tacc = tmem + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
   for (int c = half; 16 * c < tokens; c += 2) {
-    uint32_t rr[16];
-    if (__all_sync(0xFFFFFFFFu, ok && nkb > 0)) {
-      tmem_ld_32x32b_x16(tacc + 16 * c, rr);
-      tmem_ld_wait(rr);
-    } else {
+    float v[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) rr[j] = 0u;
+    for (int j = 0; j < 16; ++j) v[j] = 0.f;
+    if (__all_sync(0xFFFFFFFFu, ok)) {
+      for (int a = 0; a < accs; ++a) {
+        uint32_t rr[16];
+        tmem_ld_32x32b_x16(tacc + BT * a + 16 * c, rr);
+        tmem_ld_wait(rr);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(rr[j]);
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) part[(16 * c + j) * 128 + r] = __uint_as_float(rr[j]);
+    for (int j = 0; j < 16; ++j) part[(16 * c + j) * 128 + r] = v[j];
   }
   const bool all_ok = __syncthreads_and(ok);
   if (splits > 1) cluster_sync();
@@ -326,7 +338,7 @@ __global__ void __launch_bounds__(256)
   if (splits > 1) cluster_sync();  // no CTA leaves while another may read its sums
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, L::kTmemCols);
+    tmem_dealloc(tmem, tmem_cols);
   }
 }
 

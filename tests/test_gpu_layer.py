@@ -239,6 +239,7 @@ def test_linear_pair_kernel(dtype, trans_b, out, pre, pad, shift):
     _lib.check(_lib.lib().tforge_debug_linear_kernel(2, 0, 0))
     Linear(300, 520, 200, dtype, "gelu", residual=out, out=out, pre=pre, trans_b=trans_b, pad=pad, shift=shift).call().check()
     Linear(5, 40, 1000, dtype, "silu", out=out, pre=pre, trans_b=trans_b, pad=pad, shift=shift).call().check()
+    Linear(300, 520, 4500, dtype, "gelu", residual=out, out=out, pre=pre, trans_b=trans_b, pad=pad, shift=shift).call().check()
 
 
 @pytest.mark.parametrize("dtype,trans_b", [(torch.bfloat16, False), (torch.float8_e4m3fn, True)])
@@ -256,6 +257,35 @@ def test_linear_backward_pair_kernel(trans_b):
     _lib.check(_lib.lib().tforge_debug_linear_kernel(2, 0, 0))
     check_linear_backward(300, 520, 264, trans_b=trans_b)
     check_linear_backward(77, 131, 65, trans_b=trans_b, grad=torch.float32)
+
+
+@pytest.mark.parametrize("force", [(0, 0, 0), (1, 16, 2), (1, 64, 8), (2, 0, 0)])
+@pytest.mark.parametrize("trans_b", [True, False])
+def test_linear_f32_output_of_a_long_k(force, trans_b):
+    """The tensor core cuts each addition to an f32 accumulator, 2^-23 of it at most, and adds 16
+    products at a time.  An f32 output is off by no more than a piece of 768 can be (48 additions) and
+    the joining of the pieces, where one sum over 16384 would be 1.9e-5 off."""
+    m, n, k = 40, 264, 16384
+    _lib.check(_lib.lib().tforge_debug_linear_kernel(*force))
+    c = Linear(m, n, k, bias=False, out=torch.float32, trans_b=trans_b, pre=True, residual=torch.float32).call()
+    want = c.a.double() @ (c.b.double().T if trans_b else c.b.double())
+    bound = 48 * 2.0 ** -23 + 22 * 2.0 ** -24
+    assert float((c.pre.double() - want).norm()) <= bound * float(want.norm())
+    want = want + c.residual.double()
+    assert float((c.out.double() - want).norm()) <= bound * float(want.norm())
+
+
+def test_linear_backward_f32_gradients_of_a_long_batch():
+    """The same for the gradients' products: dB sums over the batch."""
+    m, n, k = 12000, 72, 136
+    a, dout = rand(m, k, dtype=torch.bfloat16), rand(m, n, dtype=torch.bfloat16, seed=1)
+    db = torch.empty(n, k, device="cuda")
+    for force in ((0, 0, 0), (2, 0, 0)):
+        _lib.check(_lib.lib().tforge_debug_linear_kernel(*force))
+        _lib.linear_backward(ptr(dout), ptr(a), None, m, n, k, dB=ptr(db), grad_dtype=_lib.F32, trans_b=True,
+                             stream=torch.cuda.current_stream().cuda_stream)
+        want = dout.double().T @ a.double()
+        assert float((db.double() - want).norm()) <= (48 * 2.0 ** -23 + 22 * 2.0 ** -24) * float(want.norm())
 
 
 def test_linear_infinities_and_nan():
