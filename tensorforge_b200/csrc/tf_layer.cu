@@ -305,7 +305,7 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
   else if ((force & 255) == 2) c = Choice{0, 1};
   if ((c.tile == 0 && K == 0) || (c.tile != 0 && t_mn && c.tile < 64)) return TFORGE_ERR_UNSUPPORTED;
   // f32 outputs: sums in pieces (of the pair kernel; the slim kernel divides its k by its accumulators).
-  const int64_t stages = (K * esz + 127) / 128, piece = f8 ? 64 : 8;
+  const int64_t stages = (K * esz + 127) / 128, piece = f8 ? 64 : 12;
   p.sum_stages = !p.out_bf16 && stages > piece ? (int32_t)piece : 0;
   if (c.tile == 0) {
     CUtensorMap tmA{}, tmB{}, tmO{}, tmP{}, tmR{};
