@@ -401,6 +401,7 @@ __global__ void __launch_bounds__(kBwdBlock<T>, T == 512 ? 2 : 1) norm_bwd_kerne
   __shared__ __align__(16) uint32_t sm[2][CL * T / 32 > 64 ? CL * T / 32 : 64];
   __shared__ float comb[kRows > 1 ? kRows * T * E : 1];
   const int t = threadIdx.x & (T - 1), sub = threadIdx.x / T;
+  if constexpr (CL > 1) cluster_sync();  // every block has started before another writes its memory
   // This block's columns: c0 .. c0 + width - 1.
   const int64_t c0 = CL > 1 ? (int64_t)cluster_ctarank() * (T * E) : 0;
   const int width = CL > 1 ? (int)(p.N - c0 < 0 ? 0 : p.N - c0 < T * E ? p.N - c0 : T * E) : (int)p.N;
