@@ -128,9 +128,9 @@ __device__ __forceinline__ void copy_groups(const RowCopy &j, int64_t first, int
     if (word >= begin && word + (shift ? 20 : 16) <= end) {
       const uint32_t *src = reinterpret_cast<const uint32_t *>(word);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = __ldg(src + k);
+      for (int k = 0; k < 4; ++k) w[k] = src[k];
       if (shift) {
-        w[4] = __ldg(src + 4);
+        w[4] = src[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], shift);
       }
@@ -156,12 +156,12 @@ __device__ __forceinline__ void convert_groups(const RowCopy &j, int64_t first, 
     const float *s = static_cast<const float *>(j.src) + r * j.lds + c;
     float v[8];
     if (vec && c + 8 <= j.cols) {
-      const float4 a = __ldg(reinterpret_cast<const float4 *>(s)), b = __ldg(reinterpret_cast<const float4 *>(s) + 1);
+      const float4 a = reinterpret_cast<const float4 *>(s)[0], b = reinterpret_cast<const float4 *>(s)[1];
       v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
       v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? __ldg(s + k) : 0.f;
+      for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? s[k] : 0.f;
     }
     *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(j.dst) + r * j.ldd + c) =
         make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
@@ -344,9 +344,8 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
 // arithmetic: 8192 x 16384 bf16.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-    activation_grad_kernel(int act, int across, const T *__restrict__ dout, int64_t lddo, const T *__restrict__ pre,
-                           int64_t ldp, __nv_bfloat16 *__restrict__ dz, int64_t ldz, float *__restrict__ part, int64_t M,
-                           int64_t N) {
+    activation_grad_kernel(int act, int across, const T *dout, int64_t lddo, const T *pre, int64_t ldp, __nv_bfloat16 *dz,
+                           int64_t ldz, float *part, int64_t M, int64_t N) {
   grid_dependency_wait();
   grid_launch_dependents();
   __shared__ float sm[8][256];
@@ -364,7 +363,7 @@ __global__ void __launch_bounds__(256)
     if constexpr (VEC) {
 #pragma unroll
       for (int h = 0; h < (int)sizeof(T) / 2; ++h)
-        q.v[h] = c0 + lane * 8 < N ? __ldg(reinterpret_cast<const uint4 *>(row + c0 + lane * 8) + h) : make_uint4(0, 0, 0, 0);
+        q.v[h] = c0 + lane * 8 < N ? reinterpret_cast<const uint4 *>(row + c0 + lane * 8)[h] : make_uint4(0, 0, 0, 0);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) q.v[j] = c0 + off(j) < N ? row[c0 + off(j)] : T(0.f);

@@ -389,7 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_D
 #pragma unroll 1
     for (int i = 0; i < my_tiles && ok; ++i) {
       const int u = i * pieces + pieces - 1, b = u & 1;  // the tile's last piece
-      const float sa = p.a_scale && m0 + lane < p.M ? __ldg(p.a_scale + m0 + lane) : 1.f;
+      const float sa = p.a_scale && m0 + lane < p.M ? p.a_scale[m0 + lane] : 1.f;
       int m1 = 0, n1 = 0;  // the next tile
       if (i + 1 < my_tiles) tile_at(i + 1, m1, n1);
       const uint32_t lanes = (uint32_t)(q * 32) << 16;
@@ -433,8 +433,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_D
       for (int k = 0; k < 2; ++k) {
         const int c = part + 4 * k, col0 = n0 + 32 * c;
         const bool live = inside(m0, col0), lane_col = live && col0 + lane < p.N;
-        const float bl = p.bias && lane_col ? __ldg(p.bias + col0 + lane) : 0.f;
-        const float sl = p.b_scale && lane_col ? __ldg(p.b_scale + col0 + lane) : 1.f;
+        const float bl = p.bias && lane_col ? p.bias[col0 + lane] : 0.f;
+        const float sl = p.b_scale && lane_col ? p.b_scale[col0 + lane] : 1.f;
         if (!SUMS && k == 0) {
           ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(accf0 + 8 * b, (u >> 1) & 1, wc, 64));
           if (!ok) break;

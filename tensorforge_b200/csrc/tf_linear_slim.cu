@@ -141,7 +141,7 @@ __device__ __forceinline__ void finish8(const LinearParams &p, int g, int m0, in
     }
   }
   if (p.a_scale) {
-    const float sa = __ldg(p.a_scale + m);
+    const float sa = p.a_scale[m];
     get8<VEC>(p.b_scale + n, live, c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = v[j] * sa * c[j];

@@ -392,7 +392,7 @@ constexpr int kBwdBlock = T <= 32 ? 256 : T;
 // the row) b.  AHEAD: the next rows' loads are under way while a row is reduced and written.  part:
 // gridDim.x / CL rows of N f32, this block's column sums (null: no dweight).
 template <typename X, bool VEC, int T, int E, int CL, bool AHEAD>
-__global__ void __launch_bounds__(kBwdBlock<T>, T == 512 ? 2 : 1) norm_bwd_kernel(const NormBwdArgs p, float *__restrict__ part) {
+__global__ void __launch_bounds__(kBwdBlock<T>, T == 512 ? 2 : 1) norm_bwd_kernel(const NormBwdArgs p, float *part) {
   grid_dependency_wait();
   grid_launch_dependents();
   using Raw = RawRow<X, VEC, E>;
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kBwdBlock<T>, T == 512 ? 2 : 1) norm_bwd_kerne
     next.y.template load<T>(static_cast<const X *>(p.dy) + m * p.lddy + c0, t, n);
     next.s.template load<T>(static_cast<const X *>(p.s) + m * p.lds + c0, t, n);
     if (p.ds) next.d.template load<T>(static_cast<const X *>(p.ds) + m * p.ldds + c0, t, n);
-    next.rstd = __ldg(p.rstd + m);
+    next.rstd = p.rstd[m];
   };
   const int64_t step = (int64_t)blocks * kRows;
   int64_t m0 = (int64_t)block * kRows;
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(kBwdBlock<T>, T == 512 ? 2 : 1) norm_bwd_kerne
 // in this block's row of `part`, each element read and written by one thread.  VEC: eight elements a
 // thread and step; else one.
 template <typename X, bool VEC>
-__global__ void __launch_bounds__(512, 2) norm_bwd_wide_kernel(const NormBwdArgs p, float *__restrict__ part) {
+__global__ void __launch_bounds__(512, 2) norm_bwd_wide_kernel(const NormBwdArgs p, float *part) {
   grid_dependency_wait();
   grid_launch_dependents();
   using Raw = RawRow<X, VEC, VEC ? 8 : 1>;
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_wide_kernel(const NormBwdArgs
     const X *s = static_cast<const X *>(p.s) + m * p.lds;
     const X *ds = p.ds ? static_cast<const X *>(p.ds) + m * p.ldds : nullptr;
     X *dx = static_cast<X *>(p.dx) + m * p.lddx;
-    const float rstd = __ldg(p.rstd + m);
+    const float rstd = p.rstd[m];
     float dot = 0.f;
     uint32_t none = 0u;
 #pragma unroll 2
@@ -557,8 +557,7 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_wide_kernel(const NormBwdArgs
 
 // out[c] = sum over r = 0 .. rows - 1, in a fixed order, of part[r * N + c]: 32 columns a block, 32
 // threads share a column's rows.
-__global__ void __launch_bounds__(1024) column_sum_kernel(const float *__restrict__ part, int rows, int64_t N,
-                                                          float *__restrict__ out) {
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float *part, int rows, int64_t N, float *out) {
   grid_dependency_wait();
   grid_launch_dependents();
   __shared__ float sm[32][33];

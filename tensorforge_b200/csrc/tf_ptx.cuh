@@ -185,7 +185,10 @@ __device__ __forceinline__ void named_barrier(uint32_t id, uint32_t count) {
 // Programmatic dependent launch.  grid_dependency_wait: block until the grid this launch
 // depends on has completed and its memory writes are visible (immediately, when the launch
 // had no programmatic dependency).  grid_launch_dependents: let the grids that depend on this
-// one start launching (their CTAs can set up while this grid finishes).
+// one start launching (their CTAs can set up while this grid finishes).  A kernel that waits reads what
+// an earlier grid may have written by plain loads only, not by __ldg or through const __restrict__
+// pointers: those promise that the memory does not change while the kernel exists, and may be moved
+// above the wait.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
