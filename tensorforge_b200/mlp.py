@@ -89,8 +89,9 @@ class FeedForward:
     x, residual, s and out are bf16, M x D; W1 is D x H, W2 H x D.  mode "bf16": weights in bf16 as
     given.  mode "fp8": each output feature's weights in 8 bits with a scale, the activations in 8
     bits with a scale a row -- the norm writes the first product's, the quantizer the second's.
-    Calls run on the current stream of x's device.  `__call__(..., keep=True)` keeps what `backward`
-    needs until it is called (mode "bf16")."""
+    x is on the weights' GPU, and calls run on its current stream.  `__call__(..., keep=True)` keeps what
+    `backward` needs until it is called, on the same stream (mode "bf16"): x or s among it, which may
+    not change before then."""
 
     def __init__(self, w1, b1, w2, b2, norm_weight, activation: str = "gelu_tanh", mode: str = "bf16", eps: float = 1e-5):
         import torch
@@ -102,6 +103,8 @@ class FeedForward:
         self.d, self.h = w1.shape
         if w2.shape != (self.h, self.d) or b1.shape != (self.h,) or b2.shape != (self.d,) or norm_weight.shape != (self.d,):
             raise ValueError("FeedForward expects W1 d x h, b1 h, W2 h x d, b2 d, norm weight d")
+        if w1.device.type != "cuda" or any(t.device != w1.device for t in (b1, w2, b2, norm_weight)):
+            raise ValueError("FeedForward expects its weights on one GPU")
         self.mode, self.activation, self.eps = mode, activation, eps
         self.b1, self.b2, self.norm_weight = (t.float().contiguous() for t in (b1, b2, norm_weight))
         self.kept = None
@@ -136,6 +139,8 @@ class FeedForward:
 
         if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != self.d or not x.is_contiguous():
             raise ValueError("FeedForward takes contiguous bf16 rows of its width")
+        if x.device != self.b1.device or (residual is not None and residual.device != x.device):
+            raise ValueError("FeedForward takes rows on its weights' GPU")
         if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape or not residual.is_contiguous()):
             raise ValueError("the residual is like x")
         if keep and self.mode != "bf16":
@@ -170,7 +175,7 @@ class FeedForward:
                 _lib.linear(hid.data_ptr(), self.w2.data_ptr(), out.data_ptr(), m, self.d, self.h, bias=self.b2.data_ptr(),
                             residual=s.data_ptr(), stream=st)
         if keep:
-            self.kept = (s, rstd, n, pre, hid)
+            self.kept = (s, rstd, n, pre, hid, st)
         return out, s
 
     def backward(self, dout) -> dict:
@@ -180,13 +185,14 @@ class FeedForward:
 
         if self.kept is None:
             raise ValueError("backward needs a call with keep=True before it")
-        s, rstd, n, pre, hid = self.kept
-        if dout.dtype != torch.bfloat16 or dout.shape != s.shape or not dout.is_contiguous():
+        s, rstd, n, pre, hid, st = self.kept
+        if dout.dtype != torch.bfloat16 or dout.shape != s.shape or not dout.is_contiguous() or dout.device != s.device:
             raise ValueError("backward takes out's gradient: contiguous bf16 rows like out's")
+        if self._stream(s) != st:
+            raise ValueError("backward runs on the stream of the call that it follows")
         self.kept = None
         m = s.shape[0]
         with torch.cuda.device(s.device):
-            st = self._stream(s)
 
             def new(*shape, dtype=torch.bfloat16):
                 return torch.empty(shape, device=s.device, dtype=dtype)

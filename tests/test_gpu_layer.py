@@ -880,3 +880,95 @@ print("captured")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
                        cwd=Path(__file__).resolve().parent.parent)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+# ---- calls that the documentation allows ---------------------------------------------------------
+
+
+def slices(rows, widths, dtype):
+    """Matrices that are neighbouring column slices of one buffer, each width a column apart, and the
+    check that the columns between them stay NaN."""
+    whole = torch.full((rows, sum(widths) + len(widths)), float("nan"), device="cuda", dtype=dtype)
+    views, gaps, c = [], [], 0
+    for w in widths:
+        views.append(whole[:, c:c + w])
+        gaps.append(c + w)
+        c += w + 1
+    return views, lambda: bool(whole[:, gaps].isnan().all())
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 64, 48), (130, 33, 200), (700, 264, 72)])
+def test_slices_of_one_buffer(m, n, k):
+    """Operands and outputs that lie side by side in one buffer."""
+    (a, res, out, pre, da, s, y), gaps = slices(m, (k, n, n, n, k, k, k), torch.bfloat16)
+    a.copy_(rand(m, k))
+    res.copy_(rand(m, n, seed=1))
+    b, bias = rand(n, k, dtype=torch.bfloat16, seed=2, scale=1 / math.sqrt(k)), rand(n, seed=3)
+    ld, st = a.stride(0), torch.cuda.current_stream().cuda_stream
+    ref, refp, refd = torch.empty_like(res.contiguous()), torch.empty_like(res.contiguous()), torch.empty(m, k, device="cuda").bfloat16()
+    ac, rc = a.contiguous(), res.contiguous()
+    _lib.linear(ptr(a), ptr(b), ptr(out), m, n, k, "silu", ptr(bias), ptr(res), ptr(pre), trans_b=True, lda=ld, ldr=ld, ldo=ld,
+                ldp=ld, stream=st)
+    _lib.linear(ptr(ac), ptr(b), ptr(ref), m, n, k, "silu", ptr(bias), ptr(rc), ptr(refp), trans_b=True, stream=st)
+    _lib.linear_backward(ptr(out), None, ptr(b), m, n, k, "silu", ptr(pre), dA=ptr(da), trans_b=True, lddo=ld, ldp=ld, ldda=ld, stream=st)
+    _lib.linear_backward(ptr(ref), None, ptr(b), m, n, k, "silu", ptr(refp), dA=ptr(refd), trans_b=True, stream=st)
+    assert torch.equal(out, ref) and torch.equal(pre, refp) and torch.equal(da, refd)
+    rstd, refs, refy = torch.empty(m, device="cuda"), torch.empty_like(ac), torch.empty_like(ac)
+    _lib.rms_norm(ptr(a), ptr(y), m, k, 1e-5, residual=ptr(da), sum_out=ptr(s), rstd=ptr(rstd), ldx=ld, ldr=ld, lds=ld, ldo=ld, stream=st)
+    _lib.rms_norm(ptr(ac), ptr(refy), m, k, 1e-5, residual=ptr(refd), sum_out=ptr(refs), rstd=ptr(rstd), stream=st)
+    assert torch.equal(s, refs)
+    # The unaligned rows' sums are taken in another order: a step of bf16 at most.
+    assert bool(((y.double() - refy.double()).abs() <= 2.0 ** -7 * refy.double().abs()).all())
+    assert gaps()
+
+
+def test_inputs_written_just_before():
+    """A call sees what the launches before it wrote, though its blocks may start before they end:
+    small vectors and whole operands, from torch's kernels and from the library's own."""
+    m, n, k = 48, 512, 256
+    st = torch.cuda.current_stream().cuda_stream
+    x, b = rand(m, k, dtype=torch.bfloat16), rand(n, k, dtype=torch.bfloat16, seed=1, scale=1 / 16)
+    weight, bias, dw = torch.ones(k, device="cuda"), torch.zeros(n, device="cuda"), torch.empty(k, device="cuda")
+    y, out, dx = torch.empty_like(x), torch.empty(m, n, device="cuda").bfloat16(), torch.empty_like(x)
+    rstd = torch.empty(m, device="cuda")
+    outs = []
+    for i in range(40):
+        f = 2.0 ** (i % 5)
+        weight.fill_(f)
+        bias.fill_(256 * f)
+        rstd.zero_()
+        _lib.rms_norm(ptr(x), ptr(y), m, k, 1e-5, weight=ptr(weight), rstd=ptr(rstd), stream=st)
+        _lib.linear(ptr(y), ptr(b), ptr(out), m, n, k, bias=ptr(bias), trans_b=True, stream=st)
+        _lib.rms_norm_backward(ptr(x), ptr(x), ptr(rstd), ptr(dx), m, k, weight=ptr(weight), dweight=ptr(dw), stream=st)
+        outs.append([(t.float() / f).sum() for t in (y, out, dx)] + [dw.sum()])
+    torch.cuda.synchronize()
+    # Powers of two scale through every one of them without a rounding.
+    for o in outs[1:]:
+        for got, want in zip(o, outs[0]):
+            assert float(got) == float(want)
+
+
+@pytest.mark.parametrize("mode", ["bf16", "fp8"])
+def test_block_of_no_rows(mode):
+    m = block(64, 128, "silu", mode)
+    x = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16)
+    out, s = m(x, x.clone(), keep=mode == "bf16")
+    assert out.shape == x.shape and s.shape == x.shape
+    if mode == "bf16":
+        g = m.backward(x)
+        assert all(bool((g[k] == 0).all()) for k in ("dw1", "db1", "dw2", "db2", "dnorm_weight")) and g["dx"].shape == x.shape
+
+
+def test_block_refuses_other_places():
+    """Rows, residuals and gradients that are not on the weights' GPU; a gradient on another stream."""
+    m = block(64, 128, "silu", "bf16")
+    x = rand(4, 64, dtype=torch.bfloat16)
+    for bad in (lambda: m(x.cpu()), lambda: m(x, x.cpu())):
+        with pytest.raises(ValueError):
+            bad()
+    m(x, keep=True)
+    with pytest.raises(ValueError):
+        m.backward(x.cpu())
+    with torch.cuda.stream(torch.cuda.Stream()), pytest.raises(ValueError):
+        m.backward(x)
+    assert m.backward(x)["dx"].shape == x.shape  # what was kept is still there

@@ -166,3 +166,30 @@ def test_mlp_command_refuses_what_the_block_lacks(capsys):
                  ["--block", "--mode", "fp8", "--train"]):
         with pytest.raises(SystemExit):
             mlp.main(argv)
+
+
+@pytest.mark.parametrize("call,dims", [(linear, "MNK"), (backward, "MNK"), (norm, "MN"), (norm_backward, "MN")])
+def test_sizes_end_at_two_to_the_thirtieth(call, dims):
+    for d in dims:
+        assert call(**{d: (1 << 30) + 1}) == _lib.ERR_SHAPE
+
+
+@pytest.mark.parametrize("call,kw", [
+    (linear, dict(ldo=34, ldp=34, pre=5 * P + 2 * 15)),  # pre begins in out's last column
+    (linear, dict(ldo=31, ldp=31, pre=5 * P + 2 * 16)),  # pre's last column is out's first of the next row
+    (linear, dict(ldo=32, ldp=33, pre=5 * P + 2 * 16)),  # the pitches differ
+    (linear, dict(lda=64, ldo=64, out=P + 2 * 23)),
+    (linear, dict(lda=64, ldo=64, out=P - 2 * 15)),
+    (norm, dict(out_dtype=_lib.BF16, lds=32, ldo=32, out=4 * P + 2 * 17)),
+])
+def test_slices_of_one_buffer_that_overlap(call, kw):
+    assert call(**kw) == _lib.ERR_ALIAS
+
+
+def test_block_takes_no_weights_outside_a_gpu():
+    torch = pytest.importorskip("torch")
+    from tensorforge_b200.mlp import FeedForward
+
+    for mode in ("bf16", "fp8"):
+        with pytest.raises(ValueError):
+            FeedForward(torch.ones(8, 16), torch.ones(16), torch.ones(16, 8), torch.ones(8), torch.ones(8), "silu", mode)
