@@ -112,6 +112,26 @@ __device__ __forceinline__ void add_row(const LinearParams &p, int64_t row, int 
   }
 }
 
+// f(j, x[col0 + j]) for a chunk's columns, those from N on with 0: four at a time by loads that the
+// whole warp shares where they are on 16-byte boundaries, else a column a lane by shuffles.
+template <typename F>
+__device__ __forceinline__ void with_columns(const float *x, int col0, int n, bool vec, int lane, F &&f) {
+  if (vec && col0 + 32 <= n) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float4 q = reinterpret_cast<const float4 *>(x + col0)[u];
+      f(4 * u, q.x);
+      f(4 * u + 1, q.y);
+      f(4 * u + 2, q.z);
+      f(4 * u + 3, q.w);
+    }
+  } else {
+    const float own = col0 + lane < n ? x[col0 + lane] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f(j, __shfl_sync(0xFFFFFFFFu, own, j));
+  }
+}
+
 // Row r (of 32) of a staging box: 32 f32 (128-B swizzle) or 32 bf16 (64-B swizzle), as the maps say.
 __device__ __forceinline__ void stage_row(uint8_t *box, int r, bool bf16, const float (&v)[32]) {
   if (bf16) {
@@ -383,34 +403,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_D
     int m0 = 0, n0 = 0;
     if (my_tiles > 0) {
       tile_at(0, m0, n0);
-      fetch_residual(m0, n0 + 32 * part);
+      if (!SUMS) fetch_residual(m0, n0 + 32 * part);
     }
     bool ok = true;
 #pragma unroll 1
     for (int i = 0; i < my_tiles && ok; ++i) {
       const int u = i * pieces + pieces - 1, b = u & 1;  // the tile's last piece
-      const float sa = p.a_scale && m0 + lane < p.M ? p.a_scale[m0 + lane] : 1.f;
-      int m1 = 0, n1 = 0;  // the next tile
-      if (i + 1 < my_tiles) tile_at(i + 1, m1, n1);
       const uint32_t lanes = (uint32_t)(q * 32) << 16;
       if constexpr (SUMS) {
-        // The pieces' sums, in order, in registers; then back into the last piece's accumulator, from
-        // where they go on as a whole sum would.
-        float sum[64];
+        // The pieces' sums, in order: half of them in registers, half in the warp's box; the last piece's
+        // go back into its accumulator, from where they go on as a whole sum would.  (What does not fit
+        // the registers is spilled past the small L1 to L2: with all of them in registers 4096 x 1024 ->
+        // 4096 takes 55 us instead of 45.)
+        constexpr int kBoxed = 4;  // groups of eight columns whose sums are in the box
+        if (lane == 0) bulk_wait_group_read0();
+        __syncwarp();
+        float *boxed = reinterpret_cast<float *>(box) + lane;
+        float sum[64 - 8 * kBoxed];
 #pragma unroll
-        for (int j = 0; j < 64; ++j) sum[j] = 0.f;
+        for (int j = 0; j < 64 - 8 * kBoxed; ++j) sum[j] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8 * kBoxed; ++j) boxed[32 * j] = 0.f;
 #pragma unroll 1
-        for (int w = i * pieces; w <= u && ok; ++w) {
+        for (int w = i * pieces; w <= u; ++w) {
           ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(accf0 + 8 * (w & 1), (w >> 1) & 1, wc, 64));
           if (!ok) break;
           tc_fence_after();
+          const uint32_t tacc = tmem + 256u * (w & 1) + lanes + part * 32;
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
             uint32_t rr[8];
-            tmem_ld_32x32b_x8(tmem + 256u * (w & 1) + lanes + (part + 4 * (g / 4)) * 32 + g % 4 * 8, rr);
+            tmem_ld_32x32b_x8(tacc + g / 4 * 128 + g % 4 * 8, rr);
             tmem_ld_wait(rr);
+            if (g < kBoxed) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[8 * g + j] += __uint_as_float(rr[j]);
+              for (int j = 0; j < 8; ++j) {
+                const float x = boxed[32 * (8 * g + j)] + __uint_as_float(rr[j]);
+                boxed[32 * (8 * g + j)] = x;
+                rr[j] = __float_as_uint(x);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) sum[8 * (g - kBoxed) + j] += __uint_as_float(rr[j]);
+              if (w == u) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) rr[j] = __float_as_uint(sum[8 * (g - kBoxed) + j]);
+              }
+            }
+            if (w == u) tmem_st_32x32b_x8(tacc + g / 4 * 128 + g % 4 * 8, rr);
           }
           if (w < u) {
             tc_fence_before();
@@ -419,22 +459,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_D
           }
         }
         if (!ok) break;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t rr[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) rr[j] = __float_as_uint(sum[32 * k + j]);
-          tmem_st_32x32b_x32(tmem + 256u * b + lanes + (part + 4 * k) * 32, rr);
-        }
         tmem_st_wait();
+        fence_proxy_async_smem();  // the sums' accesses of the box, before TMA writes there
+        __syncwarp();
+        fetch_residual(m0, n0 + 32 * part);
       }
+      const float sa = p.a_scale && m0 + lane < p.M ? p.a_scale[m0 + lane] : 1.f;
       // Not unrolled: the body, with an activation's 32 copies, should stay in the instruction cache.
 #pragma unroll 1
       for (int k = 0; k < 2; ++k) {
         const int c = part + 4 * k, col0 = n0 + 32 * c;
-        const bool live = inside(m0, col0), lane_col = live && col0 + lane < p.N;
-        const float bl = p.bias && lane_col ? p.bias[col0 + lane] : 0.f;
-        const float sl = p.b_scale && lane_col ? p.b_scale[col0 + lane] : 1.f;
+        const bool live = inside(m0, col0);
         if (!SUMS && k == 0) {
           ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(accf0 + 8 * b, (u >> 1) & 1, wc, 64));
           if (!ok) break;
@@ -452,14 +487,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_D
         }
         if (!live) continue;
         float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rr[j]);
         if constexpr (F8) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            v[j] = __uint_as_float(rr[j]) * sa * __shfl_sync(0xFFFFFFFFu, sl, j) + __shfl_sync(0xFFFFFFFFu, bl, j);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rr[j]) + __shfl_sync(0xFFFFFFFFu, bl, j);
+          for (int j = 0; j < 32; ++j) v[j] *= sa;
+          with_columns(p.b_scale, col0, p.N, vec, lane, [&](int j, float x) { v[j] *= x; });
         }
+        if (p.bias) with_columns(p.bias, col0, p.N, vec, lane, [&](int j, float x) { v[j] += x; });
         if (vec && !res_tma) {
           // The box is free once the stores issued from it have read it: all but the last one when it
           // has two bf16 halves to alternate between.
@@ -519,9 +554,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_D
         }
         if (k == 0) fetch_residual(m0, col0 + 128);
       }
-      m0 = m1;
-      n0 = n1;
-      if (ok && i + 1 < my_tiles && !res_flight) fetch_residual(m0, n0 + 32 * part);
+      if (ok && i + 1 < my_tiles) {
+        tile_at(i + 1, m0, n0);
+        if (!SUMS) fetch_residual(m0, n0 + 32 * part);
+      }
     }
     if (lane == 0) {
       if (res_flight) mbar_wait_drain(resf, res_phase, p.limit_ns);  // after an abort

@@ -972,3 +972,13 @@ def test_block_refuses_other_places():
     with torch.cuda.stream(torch.cuda.Stream()), pytest.raises(ValueError):
         m.backward(x)
     assert m.backward(x)["dx"].shape == x.shape  # what was kept is still there
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 264, 1500), (129, 77, 1000)])
+@pytest.mark.parametrize("residual", [None, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (1, 1)])
+def test_sums_in_pieces_with_the_whole_epilogue(m, n, k, residual, pad, shift):
+    """f32 outputs whose sums are taken in pieces by CTA pairs: bias, pre, activation and residual after."""
+    _lib.check(_lib.lib().tforge_debug_linear_kernel(2, 0, 0))
+    for pre in (False, True):
+        Linear(m, n, k, act="gelu", residual=residual, out=torch.float32, pre=pre, pad=pad, shift=shift).call().check()
