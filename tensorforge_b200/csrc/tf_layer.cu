@@ -581,6 +581,7 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
     dz.p = scratch.at(z_at);
     dz.ld = padded(a.N, 2);
   }
+  bool part_launched = false;
   if (some && (need_dz || want_bias)) {
     void *z = need_dz ? const_cast<void *>(dz.p) : nullptr;
     float *part = want_bias && rb > 1 ? reinterpret_cast<float *>(scratch.at(part_at)) : nullptr;
@@ -590,13 +591,17 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
                         : launch_activation_grad<float>(a.activation, a.dout, a.lddo, a.pre, a.ldp, z, dz.ld, sums, rb, a.M, a.N, st);
     if (e == cudaSuccess && part) e = launch_column_sum(part, rb, a.N, a.dbias, st);
     if (e != cudaSuccess) return cuda_failure(e, "activation gradient");
+    part_launched = part != nullptr;
   } else if (want_bias) {
     cudaError_t e = cudaMemsetAsync(a.dbias, 0, (size_t)a.N * 4, st);
     if (e != cudaSuccess) return cuda_failure(e, "cudaMemsetAsync(dbias)");
   }
+  // The two products need dz and the copies, which are complete once the column sums (or the first
+  // product) have begun: they start beside those and join them at their end.  500 x 1000 x 1000 16.8 us, one after the other 21.0.
   LinearParams p{};
   p.act = TFORGE_ACT_NONE;
   p.out_bf16 = a.grad_dtype == TFORGE_BF16;
+  p.late = part_launched;
   if (want_a) {
     p.out = a.dA;
     p.ldo = a.ldda;
@@ -604,6 +609,7 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
     if (rc) return rc;
   }
   if (want_b) {
+    p.late |= want_a;
     p.out = a.dB;
     p.ldo = a.lddb;
     rc = a.trans_b ? product(dz, true, A, true, false, a.N, a.K, a.M, p, st)
