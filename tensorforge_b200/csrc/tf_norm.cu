@@ -16,6 +16,8 @@
 // time).
 //
 // Both are bound by HBM: x, residual, sum and out (or dy, s, ds and dx) cross it once each.
+// 16384 x 8192 bf16 with residual to 8 bits 143 us, 6.6 TB/s; the gradient of 16384 x 4096 bf16 with ds
+// 88 us, 6.1 TB/s; 4097 x 1111 f32, single elements, 7 us, 5.3 TB/s; 16 x 4096, a launch, 2.4 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -198,7 +200,7 @@ struct RowFactors {
   }
 };
 
-// One row on T threads, E elements a thread in registers; below 128 threads a block of 256 holds
+// One row on T threads, E elements a thread in registers; up to 32 threads a block of 256 holds
 // several rows.  VEC: groups of eight consecutive elements (all rows on 16-byte boundaries, N a
 // multiple of 8); else single elements, T apart.  NORM false: the quantizer (y = x).
 template <typename X, int OUT, bool VEC, int T, int E, bool NORM>
@@ -311,7 +313,7 @@ __global__ void __launch_bounds__(T <= 32 ? 256 : T) norm_row_kernel(const NormA
   }
 }
 
-// Rows longer than the register kernels hold: two passes over the row, the second mostly from L2.
+// Rows longer than the register kernels hold (16384): two passes over the row, the second mostly from L2.
 // The first pass only reads (sum_out may be the residual's or x's own rows), the second writes.
 template <typename X, int OUT, bool NORM>
 __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs p) {
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(kBwdBlock<T>, T == 512 ? 2 : 1) norm_bwd_kerne
   grid_launch_dependents();
   using Raw = RawRow<X, VEC, E>;
   constexpr int kRows = kBwdBlock<T> / T;
-  static_assert(CL == 1 || kRows == 1, "a cluster has one row at a time");
+  static_assert(CL == 1 || (kRows == 1 && T >= 64), "a cluster has one row at a time");
   __shared__ __align__(16) uint32_t sm[2][CL * T / 32 > 64 ? CL * T / 32 : 64];
   __shared__ float comb[kRows > 1 ? kRows * T * E : 1];
   const int t = threadIdx.x & (T - 1), sub = threadIdx.x / T;
@@ -576,23 +578,26 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float *part, int
   if (threadIdx.x == 0 && cc < N) out[cc] = v;
 }
 
+// Rows that one an SM takes: then a row's own time counts, and more threads on it (16 x 4096 bf16 with
+// residual to 8 bits 2.4 us on 256 x 16, 3.1 on 128 x 32).
+constexpr int64_t kFewRows = 148;
+
 bool at16(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 
-template <typename X, int OUT, bool VEC, bool NORM>
+// The first of the row kernels whose T threads x E elements hold N columns.  In 16-byte pieces many
+// elements on few threads, two steps a power of two: threads without columns cost most, and blocks that
+// end at a barrier soonest (50 331 648 elements bf16 to bf16 in rows of 640 5.3 TB/s on 32 x 24, 2.5 on
+// 128 x 8; of 1024 5.7 on 32 x 32, 3.8 on 128 x 8; of 4160 5.1 on 256 x 24, 3.8 on 512 x 16).  f32
+// rows of 1024 with residual 6.8 on 128 x 8, 6.4 on 32 x 32.  Single elements: 2 to 4 TB/s in bf16,
+// the more threads the better (rows of 1660 4.1 on 256 x 8, 2.7 on 128 x 16).
+template <typename X, int OUT, bool VEC, bool NORM, int T, int E, int... MORE>
 cudaError_t launch_norm_rows(const NormArgs &p, cudaStream_t st) {
-  auto grid = [&](int rows) { return dim3((unsigned)((p.M + rows - 1) / rows)); };
-  if constexpr (VEC) {
-    if (p.N <= 64) return launch_dependent(norm_row_kernel<X, OUT, VEC, 8, 8, NORM>, grid(32), dim3(256), st, 0, p);
-    if (p.N <= 128) return launch_dependent(norm_row_kernel<X, OUT, VEC, 16, 8, NORM>, grid(16), dim3(256), st, 0, p);
-  }
-  if (p.N <= 256) return launch_dependent(norm_row_kernel<X, OUT, VEC, 32, 8, NORM>, grid(8), dim3(256), st, 0, p);
-  if (p.N <= 512) return launch_dependent(norm_row_kernel<X, OUT, VEC, 32, 16, NORM>, grid(8), dim3(256), st, 0, p);
-  if (p.N <= 1024) return launch_dependent(norm_row_kernel<X, OUT, VEC, 128, 8, NORM>, grid(1), dim3(128), st, 0, p);
-  if (p.N <= 2048) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 8, NORM>, grid(1), dim3(256), st, 0, p);
-  if (p.N <= 4096) return launch_dependent(norm_row_kernel<X, OUT, VEC, 256, 16, NORM>, grid(1), dim3(256), st, 0, p);
-  if (p.N <= 8192) return launch_dependent(norm_row_kernel<X, OUT, VEC, 512, 16, NORM>, grid(1), dim3(512), st, 0, p);
-  if (p.N <= 16384) return launch_dependent(norm_row_kernel<X, OUT, VEC, 512, 32, NORM>, grid(1), dim3(512), st, 0, p);
-  return launch_dependent(norm_long_kernel<X, OUT, NORM>, grid(1), dim3(1024), st, 0, p);
+  constexpr int kRows = T <= 32 ? 256 / T : 1;
+  if (p.N <= T * E)
+    return launch_dependent(norm_row_kernel<X, OUT, VEC, T, E, NORM>, dim3((unsigned)((p.M + kRows - 1) / kRows)),
+                            dim3(kRows * T), st, 0, p);
+  if constexpr (sizeof...(MORE) > 0) return launch_norm_rows<X, OUT, VEC, NORM, MORE...>(p, st);
+  else return launch_dependent(norm_long_kernel<X, OUT, NORM>, dim3((unsigned)p.M), dim3(1024), st, 0, p);
 }
 
 template <typename X, int OUT, bool NORM>
@@ -602,41 +607,55 @@ cudaError_t launch_norm_vec(const NormArgs &p, cudaStream_t st) {
   const bool vec = p.N % 8 == 0 && at16(p.x) && at16(p.residual) && at16(p.sum_out) && at16(p.weight) && at16(p.out) &&
                    p.ldx * e % 16 == 0 && p.ldr * e % 16 == 0 && p.lds * e % 16 == 0 &&
                    p.ldo * eo % (eo == 1 ? 8 : 16) == 0;
-  return vec ? launch_norm_rows<X, OUT, true, NORM>(p, st) : launch_norm_rows<X, OUT, false, NORM>(p, st);
+  if (vec && p.M <= kFewRows)
+    return launch_norm_rows<X, OUT, true, NORM, 8, 8, 16, 8, 32, 8, 128, 8, 256, 8, 256, 16, 512, 16, 512, 32>(p, st);
+  if (!vec) return launch_norm_rows<X, OUT, false, NORM, 32, 8, 32, 16, 128, 8, 256, 8, 256, 16, 512, 16, 512, 32>(p, st);
+  if constexpr (sizeof(X) == 4)
+    return launch_norm_rows<X, OUT, true, NORM, 8, 8, 16, 8, 32, 8, 32, 16, 32, 24, 128, 8, 128, 16, 128, 24, 256, 16, 256, 24, 512, 16,
+                            512, 32>(p, st);
+  else
+    return launch_norm_rows<X, OUT, true, NORM, 8, 8, 16, 8, 32, 8, 32, 16, 32, 24, 32, 32, 32, 48, 128, 16, 128, 24, 128, 32, 256, 24,
+                            256, 32, 512, 24, 512, 32>(p, st);
 }
 
-// The gradient kernel of a call: eight elements a thread, and from 8193 columns a cluster of four or
-// eight blocks of 512 threads a row.  4096 x 16384 bf16 / f32 136 / 226 us; with two blocks of 1024
-// 150 / 210; with one block and sixteen elements a thread, which spill, 153 / 277.  320 x 13376 f32
-// (few rows): 29 us, 31 and 41.
+// The gradient kernel of a call.  As forward, threads without columns cost most, and a row's next loads
+// are worth more than more rows: 41 943 040 elements in rows of 1216 bf16 67 us on 64 x 24 (94 on
+// 256 x 8), of 5120 f32 with ds 106 on 256 x 24 (142 on 1024 x 8), of 4096 bf16 52 on 512 x 8 (70 on
+// 256 x 16).  Rows above 8192 columns are shared by clusters: 50 331 648 elements in rows of 12288 f32
+// with ds 5.0 TB/s on two blocks of 256 x 24 (3.9 on four of 512 x 8), of 16384 4.7 on four of
+// 512 x 8 (3.9 on four of 256 x 16).
 struct BwdKernel {
   void (*kern)(const NormBwdArgs, float *);
   int threads, rows;  // of a block
   int cluster;
-  int id;  // a number of its own
+  int id;  // a number of its own, below 160
 };
-template <typename X, bool VEC, int T, int CL = 1>
-BwdKernel bwd_kernel(int id) {
-  // Two rows' pieces fit the registers for bf16 in 16-byte pieces; elsewhere a thread's loads are
-  // enough by themselves.
-  constexpr bool kAhead = VEC && sizeof(X) == 2;
-  return {norm_bwd_kernel<X, VEC, T, 8, CL, kAhead>, kBwdBlock<T>, kBwdBlock<T> / T, CL, id};
+// Whether the next rows' loads start before a row is reduced: not where the registers for two rows would
+// leave too few warps.
+template <typename X, bool VEC, int T>
+constexpr bool bwd_ahead() {
+  return T < 512 || (T == 512 && VEC && sizeof(X) == 2) || (T == 1024 && VEC && sizeof(X) == 2);
+}
+// The first of the kernels whose T threads x E elements x CL blocks hold N columns.
+template <typename X, bool VEC, int T, int E, int CL, int... MORE>
+BwdKernel first_bwd(int64_t N, int id) {
+  if (N <= (int64_t)T * E * CL)
+    return {norm_bwd_kernel<X, VEC, T, E, CL, bwd_ahead<X, VEC, T>()>, kBwdBlock<T>, kBwdBlock<T> / T, CL, id};
+  if constexpr (sizeof...(MORE) > 0) return first_bwd<X, VEC, MORE...>(N, id + 1);
+  else return {norm_bwd_wide_kernel<X, VEC>, 512, 1, 1, id + 1};
 }
 template <typename X, bool VEC>
-BwdKernel pick_bwd(int64_t N, int id) {
-  if constexpr (VEC) {
-    if (N <= 64) return bwd_kernel<X, VEC, 8>(id);
-    if (N <= 128) return bwd_kernel<X, VEC, 16>(id + 1);
-  }
-  if (N <= 256) return bwd_kernel<X, VEC, 32>(id + 2);
-  if (N <= 512) return bwd_kernel<X, VEC, 64>(id + 3);
-  if (N <= 1024) return bwd_kernel<X, VEC, 128>(id + 4);
-  if (N <= 2048) return bwd_kernel<X, VEC, 256>(id + 5);
-  if (N <= 4096) return bwd_kernel<X, VEC, 512>(id + 6);
-  if (N <= 8192) return bwd_kernel<X, VEC, 1024>(id + 7);
-  if (N <= 16384) return bwd_kernel<X, VEC, 512, 4>(id + 8);
-  if (N <= 32768) return bwd_kernel<X, VEC, 512, 8>(id + 9);
-  return {norm_bwd_wide_kernel<X, VEC>, 512, 1, 1, id + 10};
+BwdKernel pick_bwd(int64_t M, int64_t N, int id) {
+  if (M <= kFewRows)
+    return first_bwd<X, VEC, 32, 8, 1, 64, 8, 1, 128, 8, 1, 256, 8, 1, 512, 8, 1, 1024, 8, 1, 512, 8, 4, 512, 8, 8>(N, id + 20);
+  if constexpr (!VEC)
+    return first_bwd<X, VEC, 32, 8, 1, 32, 16, 1, 32, 24, 1, 128, 8, 1, 256, 8, 1, 512, 8, 1, 1024, 8, 1, 512, 8, 4, 512, 8, 8>(N, id);
+  else if constexpr (sizeof(X) == 2)
+    return first_bwd<X, VEC, 8, 8, 1, 16, 8, 1, 32, 8, 1, 32, 16, 1, 32, 24, 1, 64, 16, 1, 64, 24, 1, 128, 16, 1, 512, 8, 1, 1024, 8,
+                     1, 256, 24, 2, 512, 8, 4, 256, 24, 4, 512, 8, 8>(N, id);
+  else
+    return first_bwd<X, VEC, 8, 8, 1, 16, 8, 1, 32, 8, 1, 32, 16, 1, 32, 24, 1, 128, 8, 1, 64, 24, 1, 256, 8, 1, 128, 24, 1, 512, 8, 1,
+                     256, 24, 1, 1024, 8, 1, 256, 24, 2, 512, 8, 4, 256, 24, 4, 512, 8, 8>(N, id);
 }
 
 bool bwd_vec(const NormBwdArgs &p) {
@@ -662,8 +681,8 @@ cudaError_t launch_rms_norm(const NormArgs &p, bool norm, cudaStream_t st) {
 
 static BwdKernel pick_bwd(const NormBwdArgs &p) {
   const bool vec = bwd_vec(p);
-  if (p.x_bf16) return vec ? pick_bwd<__nv_bfloat16, true>(p.N, 0) : pick_bwd<__nv_bfloat16, false>(p.N, 11);
-  return vec ? pick_bwd<float, true>(p.N, 22) : pick_bwd<float, false>(p.N, 33);
+  if (p.x_bf16) return vec ? pick_bwd<__nv_bfloat16, true>(p.M, p.N, 0) : pick_bwd<__nv_bfloat16, false>(p.M, p.N, 40);
+  return vec ? pick_bwd<float, true>(p.M, p.N, 80) : pick_bwd<float, false>(p.M, p.N, 120);
 }
 
 static void cluster_attr(cudaLaunchAttribute &a, int cluster) {
@@ -675,7 +694,7 @@ static void cluster_attr(cudaLaunchAttribute &a, int cluster) {
 // Blocks (or clusters of them) that the SMs hold at once, no more than there are row groups.
 int rms_norm_bwd_blocks(const NormBwdArgs &p) {
   const BwdKernel k = pick_bwd(p);
-  static std::atomic<int> resident[44];
+  static std::atomic<int> resident[160];
   int n = resident[k.id].load(std::memory_order_relaxed);
   if (n == 0) {
     cudaError_t e;
