@@ -16,6 +16,10 @@
 // accesses where the caller's rows allow; elsewhere the eight columns lie 16 apart, so that
 // neighbouring threads' single accesses are neighbouring elements.
 //
+// Bound by HBM, where few tokens read the weights once, and by latency: 1 x 4096 -> 4096 bf16 8.8 us
+// (33.5 MB of weights: 5.1 at the copy rate), 16 x 4096 -> 16384 e4m3 with silu 15.9 us (67 MB: 10.4).
+// Tokens as the tensor core's rows would pay for 128 of them.
+//
 // 256 threads: warp 0 TMA producer, warp 1 MMA issuer, then all eight warps the epilogue.  Every
 // wait is bounded (tf_ptx.cuh), and none begins before the kernel that this launch follows is done.
 #include <cuda.h>

@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_wide_kernel(const NormBwdArgs
 }
 
 // out[c] = sum over r = 0 .. rows - 1, in a fixed order, of part[r * N + c]: 32 columns a block, 32
-// threads share a column's rows.
+// threads share a column's rows.  256 x 16384 7 us, mostly from L2; 63 x 1000 under 4, a launch.
 __global__ void __launch_bounds__(1024) column_sum_kernel(const float *part, int rows, int64_t N, float *out) {
   grid_dependency_wait();
   grid_launch_dependents();

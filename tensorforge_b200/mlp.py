@@ -10,6 +10,11 @@ broadcast once, H and the output stay on the rank that owns the rows.
 
     python -m tensorforge_b200.mlp --shape 65536x4096x16384 --mode fp32        # one GPU
     torchrun --nproc-per-node 8 -m tensorforge_b200.mlp --shape 65536x4096x16384  # M-sharded
+
+`FeedForward` is the transformer block around two layers -- residual, norm, activation, bf16 with its
+gradient or 8-bit operands -- and `--block` times it:
+
+    python -m tensorforge_b200.mlp --block --shape 8192x4096x16384 --mode bf16 --train
 """
 
 from __future__ import annotations
