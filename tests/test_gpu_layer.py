@@ -982,3 +982,34 @@ def test_sums_in_pieces_with_the_whole_epilogue(m, n, k, residual, pad, shift):
     _lib.check(_lib.lib().tforge_debug_linear_kernel(2, 0, 0))
     for pre in (False, True):
         Linear(m, n, k, act="gelu", residual=residual, out=torch.float32, pre=pre, pad=pad, shift=shift).call().check()
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 264, 136), (300, 520, 1000), (2304, 2560, 2048)])
+@pytest.mark.parametrize("bias", [True, False])
+def test_gradients_in_a_row(m, n, k, bias):
+    """The gradient's products run beside its column sums and one another; whoever comes next -- here a
+    norm that reads dA and dB, and the next gradient, which overwrites them -- finds all complete."""
+    st = torch.cuda.current_stream().cuda_stream
+    first = rand(m, n, dtype=torch.bfloat16)
+    dout, pre = torch.empty_like(first), rand(m, n, dtype=torch.bfloat16, seed=1)
+    a, b = rand(m, k, dtype=torch.bfloat16, seed=2), rand(n, k, dtype=torch.bfloat16, seed=3)
+    da, db, dbias = torch.empty_like(a), torch.empty_like(b), torch.empty(n, device="cuda")
+    ya, yb = torch.empty_like(a), torch.empty_like(b)
+    outs = []
+    for i in range(12):
+        f = 2.0 ** (i % 5)
+        torch.mul(first, f, out=dout)
+        da.zero_()
+        db.zero_()
+        _lib.linear_backward(ptr(dout), ptr(a), ptr(b), m, n, k, "relu", ptr(pre), dA=ptr(da), dB=ptr(db),
+                             dbias=ptr(dbias) if bias else None, trans_b=True, stream=st)
+        _lib.rms_norm(ptr(da), ptr(ya), m, k, 0.0, stream=st)
+        _lib.rms_norm(ptr(db), ptr(yb), n, k, 0.0, stream=st)
+        outs.append([(da / f).clone(), (db / f).clone(), ya.clone(), yb.clone()] + ([dbias / f] if bias else []))
+    for o in outs[1:]:
+        for got, want in zip(o, outs[0]):  # powers of two go through without a rounding
+            assert torch.equal(got, want)
+    dz = torch.where(pre > 0, first, torch.zeros_like(first)).double()
+    for got, want, length in ((outs[0][0], dz @ b.double(), n), (outs[0][1], dz.T @ a.double(), m)):
+        mag = (dz.abs() @ b.double().abs()) if got is outs[0][0] else (dz.abs().T @ a.double().abs())
+        assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + (length + 4) * 2.0 ** -23 * mag).all())
