@@ -346,20 +346,21 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
 // ---- the gradient's elementwise pass ---------------------------------------------------------------
 
 // dz = dout * act'(pre) rounded to bf16 (dz null: not written), and part[b, n] = the f32 sum of the
-// unrounded dz over row block b (part null: not wanted).  A warp takes 256 columns (a lane eight:
-// neighbouring ones with VEC, else 32 apart); `across` of a block's eight warps lie side by side, so
-// that wide rows are read 4 KB at a time, and the others take every (8 / across)-th row of row
-// block blockIdx.y.  Bound by HBM (reads two values and writes one an element) and the slope's
-// arithmetic: 8192 x 16384 bf16 with tanh gelu 130 us, 6.2 TB/s.
+// unrounded dz over row block b (part null: not wanted).  A block takes 256 columns (a lane eight:
+// neighbouring ones with VEC, else 32 apart) of row block blockIdx.y, a warp every eighth row.  (Warps
+// side by side on wider rows instead leave threads without columns: 6661 x 4264 bf16 with tanh gelu
+// 15 us more, 4096 x 11008 too; 8192 x 16384 the same.)  Bound by HBM (reads two values and writes
+// one an element) and the slope's arithmetic: 8192 x 16384 bf16 with tanh gelu 130 us, 6.2 TB/s.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-    activation_grad_kernel(int act, int across, const T *dout, int64_t lddo, const T *pre, int64_t ldp, __nv_bfloat16 *dz,
+    activation_grad_kernel(int act, const T *dout, int64_t lddo, const T *pre, int64_t ldp, __nv_bfloat16 *dz,
                            int64_t ldz, float *part, int64_t M, int64_t N) {
   grid_dependency_wait();
   grid_launch_dependents();
-  __shared__ float sm[8][256];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, deep = 8 / across;
-  const int64_t c0 = ((int64_t)blockIdx.x * across + warp % across) * 256;
+  constexpr int kWarps = 8;
+  __shared__ float sm[kWarps][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c0 = (int64_t)blockIdx.x * 256;
   const int64_t per = (M + gridDim.y - 1) / gridDim.y, r0 = per * blockIdx.y, r1 = r0 + per < M ? r0 + per : M;
   auto off = [&](int j) { return VEC ? lane * 8 + j : j * 32 + lane; };
   float sum[8];
@@ -413,16 +414,16 @@ __global__ void __launch_bounds__(256)
       }
     };
     // Two rows' loads in flight.
-    int64_t m = r0 + warp / across;
-    for (; m + deep < r1; m += 2 * deep) {
+    int64_t m = r0 + warp;
+    for (; m + kWarps < r1; m += 2 * kWarps) {
       Raw d[2], z[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        read(dout + (m + i * deep) * lddo, d[i]);
-        if constexpr (ACT != TFORGE_ACT_NONE) read(pre + (m + i * deep) * ldp, z[i]);
+        read(dout + (m + i * kWarps) * lddo, d[i]);
+        if constexpr (ACT != TFORGE_ACT_NONE) read(pre + (m + i * kWarps) * ldp, z[i]);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) finish(m + i * deep, d[i], z[i]);
+      for (int i = 0; i < 2; ++i) finish(m + i * kWarps, d[i], z[i]);
     }
     if (m < r1) {
       Raw d, z;
@@ -432,53 +433,31 @@ __global__ void __launch_bounds__(256)
     }
   });
   if (!part) return;
-  float *row = part + (int64_t)blockIdx.y * N;
-  if (deep == 1) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c0 + off(j) < N) row[c0 + off(j)] = sum[j];
-    return;
-  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) sm[warp][off(j)] = sum[j];
   __syncthreads();
-  for (int i = threadIdx.x; i < across * 256; i += 256) {
-    float v = 0.f;
-    for (int w = 0; w < deep; ++w) v += sm[w * across + i / 256][i % 256];
-    const int64_t c = (int64_t)blockIdx.x * across * 256 + i;
-    if (c < N) row[c] = v;
-  }
+  float v = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) v += sm[w][threadIdx.x];
+  if (c0 + threadIdx.x < N) part[(int64_t)blockIdx.y * N + c0 + threadIdx.x] = v;
 }
 
-// Warps side by side: as many of eight as the columns fill.
-int grad_across(int64_t N) {
-  int a = 1;
-  while (a < 8 && a * 256 < N) a *= 2;
-  return a;
-}
-// Row blocks: up to 16 blocks an SM in all (several rounds of resident ones, so that the last is a
-// small part), each of at least 32 rows, so that the block sums are a few percent of what is read --
-// or fewer rows while there are fewer blocks than would fill the SMs once, down to 8.  At most 256
-// blocks of rows: narrow matrices' block sums would take longer to add than to make.
+// Row blocks: eight blocks an SM in all (two rounds of resident ones), each of at least eight rows, a
+// warp one.  At most 256: narrow matrices' block sums would take longer to add than to make.
 int grad_row_blocks(int64_t M, int64_t N) {
-  const int across = grad_across(N);
-  const int64_t cols = (N + 256 * across - 1) / (256 * across);
-  int64_t rows = 32;
-  while (rows > 8 && (M + rows - 1) / rows * cols < 148 * 4) rows /= 2;
-  int64_t r = 148 * 16 / cols;
-  r = std::min<int64_t>(std::min<int64_t>(r, 256), (M + rows - 1) / rows);
+  const int64_t cols = (N + 255) / 256, r = std::min<int64_t>(std::min<int64_t>(148 * 8 / cols, 256), (M + 7) / 8);
   return r < 1 ? 1 : (int)r;
 }
 
 template <typename T>
 cudaError_t launch_activation_grad(int act, const void *dout, int64_t lddo, const void *pre, int64_t ldp, void *dz,
                                    int64_t ldz, float *part, int row_blocks, int64_t M, int64_t N, cudaStream_t st) {
-  const int e = sizeof(T), across = grad_across(N);
+  const int e = sizeof(T);
   const bool vec = N % 8 == 0 && at(dout, 16) && lddo * e % 16 == 0 &&
                    (act == TFORGE_ACT_NONE || (at(pre, 16) && ldp * e % 16 == 0));
-  const dim3 g((unsigned)((N + 256 * across - 1) / (256 * across)), (unsigned)row_blocks);
+  const dim3 g((unsigned)((N + 255) / 256), (unsigned)row_blocks);
   auto kern = vec ? activation_grad_kernel<T, true> : activation_grad_kernel<T, false>;
-  return launch_dependent(kern, g, dim3(256), st, 0, act, across, static_cast<const T *>(dout), lddo, static_cast<const T *>(pre),
+  return launch_dependent(kern, g, dim3(256), st, 0, act, static_cast<const T *>(dout), lddo, static_cast<const T *>(pre),
                           ldp, static_cast<__nv_bfloat16 *>(dz), ldz, part, M, N);
 }
 
@@ -598,7 +577,7 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
     if (e != cudaSuccess) return cuda_failure(e, "cudaMemsetAsync(dbias)");
   }
   // The two products need dz and the copies, which are complete once the column sums (or the first
-  // product) have begun: they start beside those and join them at their end.  500 x 1000 x 1000 16.8 us, one after the other 21.0.
+  // product) have begun: they start beside those and join them at their end.  500 x 1000 x 1000 takes 4 of 19 us less.
   LinearParams p{};
   p.act = TFORGE_ACT_NONE;
   p.out_bf16 = a.grad_dtype == TFORGE_BF16;
