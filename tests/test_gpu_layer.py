@@ -1013,3 +1013,90 @@ def test_gradients_in_a_row(m, n, k, bias):
     for got, want, length in ((outs[0][0], dz @ b.double(), n), (outs[0][1], dz.T @ a.double(), m)):
         mag = (dz.abs() @ b.double().abs()) if got is outs[0][0] else (dz.abs().T @ a.double().abs())
         assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + (length + 4) * 2.0 ** -23 * mag).all())
+
+
+EDGES = [64, 72, 128, 136, 256, 264, 512, 520, 768, 776, 1024, 1032, 1536, 1544, 2048, 2056, 2560, 4096, 4104, 6144, 6152, 8192,
+         8200, 12288, 12296, 16384, 16392, 24576, 24584, 32768]
+
+
+@pytest.mark.parametrize("n", EDGES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rms_norm_at_every_kernels_edges(n, dtype):
+    """The widths at which the kernels for 16-byte pieces change, and between them for single elements,
+    with few rows (148) and more."""
+    for m in (148, 149):
+        for w in (n, n + 3):
+            check_rms_norm(m, w, dtype, torch.bfloat16 if m == 148 else torch.float8_e4m3fn)
+            check_rms_norm_backward(m, w, dtype)
+
+
+def test_offsets_beyond_32_bits():
+    """Arrays of more than 2^31 elements: the first rows and the last."""
+    m, n, k = (1 << 17) + 8, (1 << 14) + 8, 64
+    st = torch.cuda.current_stream().cuda_stream
+    rows = torch.tensor([0, 1, m // 2, m - 2, m - 1], device="cuda")
+    a, b = rand(m, k, dtype=torch.bfloat16), rand(n, k, dtype=torch.bfloat16, seed=1, scale=1 / 8)
+    for ld in (n, n + 3):  # by TMA, and element by element
+        out = torch.empty(m * ld, device="cuda", dtype=torch.bfloat16).view(m, ld)[:, :n]
+        _lib.linear(ptr(a), ptr(b), ptr(out), m, n, k, trans_b=True, ldo=ld, stream=st)
+        want = a[rows].double() @ b.double().T
+        assert_within(out[rows], want, 2.0 ** -8 * want.abs() + (k + 4) * 2.0 ** -23 * (a[rows].double().abs() @ b.double().abs().T))
+        y, sc, rstd = torch.empty(m * ld, device="cuda", dtype=torch.float8_e4m3fn).view(m, ld)[:, :n], *torch.empty(2, m, device="cuda")
+        _lib.rms_norm(ptr(out), ptr(y), m, n, 1e-5, rstd=ptr(rstd), scale=ptr(sc), out_dtype=_lib.E4M3, ldx=ld, ldo=ld, stream=st)
+        s64 = out[rows].double()
+        r64 = (s64.square().mean(1) + 1e-5).rsqrt()
+        assert_within(rstd[rows], r64, 2.0 ** -23 * (n / 64 + 24) * r64)
+        v = s64 * r64[:, None] / sc[rows].double()[:, None]
+        assert_within(y[rows].float(), v, 2.0 ** -23 * (n / 16) * v.abs() + torch.clamp(v.abs() * 2.0 ** -4, min=2.0 ** -10))
+        dx, dw = torch.empty(m * ld, device="cuda", dtype=torch.bfloat16).view(m, ld)[:, :n], torch.empty(n, device="cuda")
+        _lib.rms_norm_backward(ptr(out), ptr(out), ptr(rstd), ptr(dx), m, n, dweight=ptr(dw), lddy=ld, lds=ld, lddx=ld, stream=st)
+        r = rstd[rows].double()[:, None]
+        h = s64 * r
+        c = (s64 * h).mean(1, keepdim=True)
+        want = r * (s64 - h * c)
+        e = r * h.abs() * 2.0 ** -23 * (n / 32 + 40) * (s64 * h).abs().mean(1, keepdim=True) + 2.0 ** -21 * r * (s64.abs() + (h * c).abs())
+        assert_within(dx[rows], want, e * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs())
+        cols = torch.tensor([0, n - 1], device="cuda")
+        z = out[:, cols].double()
+        assert_within(dw[cols], (z * z * rstd.double()[:, None]).sum(0), (m + 8) * 2.0 ** -23 * (z * z * rstd.double()[:, None]).sum(0))
+        del y, dx
+        da, db = torch.empty_like(a), torch.empty_like(b)
+        _lib.linear_backward(ptr(out), ptr(a), ptr(b), m, n, k, dA=ptr(da), dB=ptr(db), trans_b=True, lddo=ld, stream=st)
+        want = s64 @ b.double()
+        assert_within(da[rows], want, 2.0 ** -8 * want.abs() + (n + 4) * 2.0 ** -23 * (s64.abs() @ b.double().abs()))
+        want = z.T @ a.double()
+        assert_within(db[cols], want, 2.0 ** -8 * want.abs() + (m + 4) * 2.0 ** -23 * (z.abs().T @ a.double().abs()))
+        del out
+
+
+def test_two_threads_at_once():
+    """Two host threads, each on its own stream."""
+    import threading
+
+    calls = [Linear(200, 264, 133, act="gelu", residual=torch.bfloat16, seed=k) for k in range(2)]
+    want = []
+    for c in calls:
+        c.call()
+        torch.cuda.synchronize()
+        want.append(c.out.clone())
+        c.out.zero_()
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(c):
+        try:
+            st = torch.cuda.Stream()
+            for _ in range(100):
+                c.call(st.cuda_stream)
+            st.synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for c, w in zip(calls, want):
+        assert torch.equal(c.out, w)
