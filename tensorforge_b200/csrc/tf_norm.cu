@@ -588,8 +588,10 @@ bool at16(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 // elements on few threads, two steps a power of two: threads without columns cost most, and blocks that
 // end at a barrier soonest (50 331 648 elements bf16 to bf16 in rows of 640 5.3 TB/s on 32 x 24, 2.5 on
 // 128 x 8; of 1024 5.7 on 32 x 32, 3.8 on 128 x 8; of 4160 5.1 on 256 x 24, 3.8 on 512 x 16).  f32
-// rows of 1024 with residual 6.8 on 128 x 8, 6.4 on 32 x 32.  Single elements: 2 to 4 TB/s in bf16,
-// the more threads the better (rows of 1660 4.1 on 256 x 8, 2.7 on 128 x 16).
+// rows of 1024 with residual 6.8 on 128 x 8, 6.4 on 32 x 32.  Single elements: 2 to 5 TB/s in bf16,
+// the more threads the better above a warp (rows of 1660 4.1 on 256 x 8, 2.7 on 128 x 16; of 4095 3.8 on
+// 512 x 8, 2.7 on 256 x 16; of 300 2.2 on 32 x 16, 1.2 on 64 x 8).  Aligned pairs of bf16 for such rows,
+// singles at their ends, measured slower (rows of 1111 1.7 against 3.0).
 template <typename X, int OUT, bool VEC, bool NORM, int T, int E, int... MORE>
 cudaError_t launch_norm_rows(const NormArgs &p, cudaStream_t st) {
   constexpr int kRows = T <= 32 ? 256 / T : 1;
@@ -609,7 +611,9 @@ cudaError_t launch_norm_vec(const NormArgs &p, cudaStream_t st) {
                    p.ldo * eo % (eo == 1 ? 8 : 16) == 0;
   if (vec && p.M <= kFewRows)
     return launch_norm_rows<X, OUT, true, NORM, 8, 8, 16, 8, 32, 8, 128, 8, 256, 8, 256, 16, 512, 16, 512, 32>(p, st);
-  if (!vec) return launch_norm_rows<X, OUT, false, NORM, 32, 8, 32, 16, 128, 8, 256, 8, 256, 16, 512, 16, 512, 32>(p, st);
+  if (!vec)
+    return launch_norm_rows<X, OUT, false, NORM, 32, 4, 32, 8, 32, 16, 128, 8, 256, 8, 256, 12, 512, 8, 512, 12, 1024, 8, 1024, 16>(
+        p, st);
   if constexpr (sizeof(X) == 4)
     return launch_norm_rows<X, OUT, true, NORM, 8, 8, 16, 8, 32, 8, 32, 16, 32, 24, 128, 8, 128, 16, 128, 24, 256, 16, 256, 24, 512, 16,
                             512, 32>(p, st);
