@@ -211,8 +211,6 @@ struct LinearParams {
   // f32 outputs: stages of k after which the tensor core's sum is put aside and begun anew
   // (tf_epilogue.cuh); 0: not.
   int32_t sum_stages;
-  // Waits for the kernel that this launch follows at its end, not its beginning.
-  int32_t late;
   // Every array of the epilogue that is there starts its rows on 16-byte boundaries: the pair kernel
   // then stores tiles by TMA (tmO, tmP), the slim kernel eight columns at a time.
   int32_t vec;

@@ -211,7 +211,6 @@ class Copies {
     job_[n_] = {o.p, nullptr, o.rows, o.cols, o.ld, ldd, dtype};
     operand_[n_++] = &o;
   }
-  bool any() const { return n_ > 0; }
   // After scratch.take(): launches the copies and points the operands at them.
   int run(const Scratch &scratch, cudaStream_t st) {
     if (!n_) return TFORGE_OK;
@@ -355,8 +354,8 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     activation_grad_kernel(int act, const T *dout, int64_t lddo, const T *pre, int64_t ldp, __nv_bfloat16 *dz,
-                           int64_t ldz, float *part, int64_t M, int64_t N, bool late) {
-  if (!late) grid_dependency_wait();  // late: what it reads was complete before the operands' copies began
+                           int64_t ldz, float *part, int64_t M, int64_t N) {
+  grid_dependency_wait();
   grid_launch_dependents();
   constexpr int kWarps = 8;
   __shared__ float sm[kWarps][256];
@@ -433,7 +432,6 @@ __global__ void __launch_bounds__(256)
       finish(m, d, z);
     }
   });
-  if (late) grid_dependency_wait();
   if (!part) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) sm[warp][off(j)] = sum[j];
@@ -453,15 +451,14 @@ int grad_row_blocks(int64_t M, int64_t N) {
 
 template <typename T>
 cudaError_t launch_activation_grad(int act, const void *dout, int64_t lddo, const void *pre, int64_t ldp, void *dz,
-                                   int64_t ldz, float *part, int row_blocks, int64_t M, int64_t N, bool late,
-                                   cudaStream_t st) {
+                                   int64_t ldz, float *part, int row_blocks, int64_t M, int64_t N, cudaStream_t st) {
   const int e = sizeof(T);
   const bool vec = N % 8 == 0 && at(dout, 16) && lddo * e % 16 == 0 &&
                    (act == TFORGE_ACT_NONE || (at(pre, 16) && ldp * e % 16 == 0));
   const dim3 g((unsigned)((N + 255) / 256), (unsigned)row_blocks);
   auto kern = vec ? activation_grad_kernel<T, true> : activation_grad_kernel<T, false>;
   return launch_dependent(kern, g, dim3(256), st, 0, act, static_cast<const T *>(dout), lddo, static_cast<const T *>(pre),
-                          ldp, static_cast<__nv_bfloat16 *>(dz), ldz, part, M, N, late);
+                          ldp, static_cast<__nv_bfloat16 *>(dz), ldz, part, M, N);
 }
 
 int check_linear_types(int act, int trans_b, int a_dtype, int b_dtype) {
@@ -564,28 +561,22 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
     dz.p = scratch.at(z_at);
     dz.ld = padded(a.N, 2);
   }
-  bool part_launched = false;
   if (some && (need_dz || want_bias)) {
     void *z = need_dz ? const_cast<void *>(dz.p) : nullptr;
     float *part = want_bias && rb > 1 ? reinterpret_cast<float *>(scratch.at(part_at)) : nullptr;
     float *sums = part ? part : (want_bias ? a.dbias : nullptr);
     cudaError_t e = a.dtype == TFORGE_BF16
-                        ? launch_activation_grad<__nv_bfloat16>(a.activation, a.dout, a.lddo, a.pre, a.ldp, z, dz.ld, sums, rb, a.M, a.N, copies.any(), st)
-                        : launch_activation_grad<float>(a.activation, a.dout, a.lddo, a.pre, a.ldp, z, dz.ld, sums, rb, a.M, a.N, copies.any(), st);
+                        ? launch_activation_grad<__nv_bfloat16>(a.activation, a.dout, a.lddo, a.pre, a.ldp, z, dz.ld, sums, rb, a.M, a.N, st)
+                        : launch_activation_grad<float>(a.activation, a.dout, a.lddo, a.pre, a.ldp, z, dz.ld, sums, rb, a.M, a.N, st);
     if (e == cudaSuccess && part) e = launch_column_sum(part, rb, a.N, a.dbias, st);
     if (e != cudaSuccess) return cuda_failure(e, "activation gradient");
-    part_launched = part != nullptr;
   } else if (want_bias) {
     cudaError_t e = cudaMemsetAsync(a.dbias, 0, (size_t)a.N * 4, st);
     if (e != cudaSuccess) return cuda_failure(e, "cudaMemsetAsync(dbias)");
   }
-  // The activation's pass needs nothing of the copies; the two products need dz and the copies, which
-  // are complete once the column sums (or the first product) have begun.  Each starts beside the kernel
-  // ahead of it and joins it at its end: 500 x 1000 x 1000 takes 4 of 19 us less.
   LinearParams p{};
   p.act = TFORGE_ACT_NONE;
   p.out_bf16 = a.grad_dtype == TFORGE_BF16;
-  p.late = part_launched;
   if (want_a) {
     p.out = a.dA;
     p.ldo = a.ldda;
@@ -593,7 +584,6 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
     if (rc) return rc;
   }
   if (want_b) {
-    p.late |= want_a;
     p.out = a.dB;
     p.ldo = a.lddb;
     rc = a.trans_b ? product(dz, true, A, true, false, a.N, a.K, a.M, p, st)

@@ -277,9 +277,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_D
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Nothing of global memory is read or written, and no bounded wait begins, before this (p.late: what
-  // this launch reads was complete before the kernel that it follows began, which it joins at its end).
-  if (!p.late) grid_dependency_wait();
+  // Nothing of global memory is read or written, and no bounded wait begins, before this.
+  grid_dependency_wait();
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer (both CTAs) ----------------
     grid_launch_dependents();
@@ -568,7 +567,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_D
     }
   }
 
-  if (p.late) grid_dependency_wait();
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // no CTA leaves while the pair MMA may still read its memory

@@ -222,9 +222,8 @@ __global__ void __launch_bounds__(256)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Nothing of global memory is read or written, and no bounded wait begins, before this (p.late: what
-  // this launch reads was complete before the kernel that it follows began, which it joins at its end).
-  if (!p.late) grid_dependency_wait();
+  // Nothing of global memory is read or written, and no bounded wait begins, before this.
+  grid_dependency_wait();
   if (warp == 0 && lane == 0) {
     grid_launch_dependents();
     int kb = 0;
@@ -338,7 +337,6 @@ __global__ void __launch_bounds__(256)
       else finish8<false>(p, g, m0, n0, part, sbase, splits);
     }
   }
-  if (p.late) grid_dependency_wait();
   tc_fence_before();
   __syncthreads();
   if (splits > 1) cluster_sync();  // no CTA leaves while another may read its sums

@@ -185,10 +185,12 @@ __device__ __forceinline__ void named_barrier(uint32_t id, uint32_t count) {
 // Programmatic dependent launch.  grid_dependency_wait: block until the grid this launch
 // depends on has completed and its memory writes are visible (immediately, when the launch
 // had no programmatic dependency).  grid_launch_dependents: let the grids that depend on this
-// one start launching (their CTAs can set up while this grid finishes).  A kernel that waits reads what
-// an earlier grid may have written by plain loads only, not by __ldg or through const __restrict__
-// pointers: those promise that the memory does not change while the kernel exists, and may be moved
-// above the wait.
+// one start launching (their CTAs can set up while this grid finishes).  A grid so launched sees what
+// earlier grids wrote only behind its own wait: that the grid which let it start had waited does not
+// make their writes visible to it, so no kernel may leave the wait out or read ahead of it.  Behind
+// it, what an earlier grid may have written is read by plain loads only, not by __ldg or through
+// const __restrict__ pointers: those promise that the memory does not change while the kernel
+// exists, and may be moved above the wait.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
