@@ -35,15 +35,22 @@ __device__ __forceinline__ float gate(float w) { return rcp_approx(1.0f + ex2_ap
 constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluC3 = 0.044715f * kGeluC;
 
-// The normal distribution's Phi, by the rational approximation 7.1.26 of Abramowitz and Stegun's
-// Handbook of Mathematical Functions to erfc(|z| / sqrt 2) (absolute error of erf 1.5e-7), whose
-// exp(-z^2 / 2) is also the density's: `e`.  The lower tail comes without cancellation.
+// The normal distribution's Phi, and e = exp(-z^2 / 2), its density's shape.  The lower tail is
+//   Phi(-x) = t q(t) exp(-x^2 / 2),  t = 1 / (1 + 0.305 x),
+// with q of degree 7: the minimax fit, by linear programming, of the tail's relative error over 0 <= x <=
+// 14 (8.5e-8), beyond where the exponential leaves f32.  With the roundings, half of them the
+// exponent's, the tail is off by at most (9 + 0.75 z^2) 2^-23 of its value: 1e-6 near 0, 7e-6 at -8,
+// where 1 + erf would have lost every digit.  Three steps more than a fit of the absolute error (1.5e-7,
+// which is 5e-5 of the value at -3 and 1 % at -8).
 __device__ __forceinline__ float normal_cdf(float z, float &e) {
-  const float t = rcp_approx(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
-  float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-  q = fmaf(q, t, 0.5f * 1.421413741f);
-  q = fmaf(q, t, 0.5f * -0.284496736f);
-  q = fmaf(q, t, 0.5f * 0.254829592f);
+  const float t = rcp_approx(fmaf(0.305f, fabsf(z), 1.0f));
+  float q = fmaf(0.0365097337f, t, -0.152187902f);
+  q = fmaf(q, t, 0.184324571f);
+  q = fmaf(q, t, -0.0366914935f);
+  q = fmaf(q, t, 0.120345789f);
+  q = fmaf(q, t, 0.103622146f);
+  q = fmaf(q, t, 0.122435505f);
+  q = fmaf(q, t, 0.121641693f);
   e = ex2_approx(z * z * (-0.5f * kLog2e));
   const float tail = q * t * e;  // Phi(-|z|)
   return z > 0.0f ? 1.0f - tail : tail;

@@ -3,6 +3,8 @@
 Tolerances are worked out from the roundings on the way, in units of u = 2^-23.
 """
 
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -17,6 +19,46 @@ U = 2.0 ** -23
 
 def stream():
     return torch.cuda.current_stream().cuda_stream
+
+
+# ---- gelu ---------------------------------------------------------------------------------------------
+
+
+def phi64(z):
+    return 0.5 * torch.special.erfc(-z / math.sqrt(2))
+
+
+# Phi(-|z|) = t q(t) exp(-z^2 / 2): the fit 0.7 u, t (a rounding and an approximate reciprocal) 1.5 u, q's
+# steps 2.5 u, two products 1 u, ex2.approx 2 u, and the product with z 0.5 u: under 9 u.  The exponent
+# z^2 / 2 log2 e has three roundings of half a u, each 2^-24 z^2 / 2 of the value: 0.75 z^2 u.  Phi above 0
+# is 1 less a tail, nearer still.
+def phi_bound(z):
+    return (9 + 0.75 * z * z) * U
+
+
+@pytest.mark.parametrize("force", [(0, 0, 0), (1, 16, 1), (2, 0, 0)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_gelu_keeps_its_relative_accuracy(force, out):
+    """Far below 0 gelu is small, not lost: products of zeros, so that z is the bias."""
+    n = 8192
+    z = torch.linspace(-12.5, 8, n, device="cuda")
+    a, b = torch.zeros(3, 64, device="cuda").bfloat16(), torch.zeros(n, 64, device="cuda").bfloat16()
+    y = torch.empty(3, n, device="cuda", dtype=out)
+    _lib.check(_lib.lib().tforge_debug_linear_kernel(*force))
+    _lib.linear(ptr(a), ptr(b), ptr(y), 3, n, 64, "gelu", ptr(z), out_dtype=CODE[out], trans_b=True, stream=stream())
+    z = z.double()
+    want = z * phi64(z)
+    hs = half_step(out)
+    assert_within(y, want.expand(3, n), (phi_bound(z) * (1 + hs) + hs) * want.abs())
+
+
+def test_gelu_slope_keeps_its_relative_accuracy():
+    n = 8192
+    z, dout, slope = torch.linspace(-12.5, 8, n, device="cuda"), torch.ones(n, device="cuda"), torch.empty(n, device="cuda")
+    _lib.linear_backward(ptr(dout), None, None, 1, n, 8, "gelu", ptr(z), dbias=ptr(slope), dtype=_lib.F32, stream=stream())
+    z = z.double()
+    p, d = phi64(z), z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    assert_within(slope, p + d, phi_bound(z) * (p + d.abs()))
 
 
 # ---- one call after the other ------------------------------------------------------------------------
