@@ -203,8 +203,9 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
 /* Root-mean-square norm of rows, with the residual's addition before it:
  *   s = x + residual (sum_out = s);  r = (mean(s^2) + eps)^-1/2 (rstd = r);  out = s r weight
  * in f32, each output rounded once.  out is f32, bf16 or E4M3; E4M3 rows come with scale[m] =
- * max(max|out| / 448, 2^-126), the f32 factor back to out's values; a row that holds a NaN, or an
- * infinity in s, has a NaN scale and NaN values.  residual, weight (1), sum_out, rstd may be NULL.
+ * max(max|out| / 448, 2^-126), the f32 factor back to out's values, and hold e4m3(out * (1 / scale[m])),
+ * the reciprocal and the product each rounded to f32; a row that holds a NaN, or an infinity in s, has a
+ * NaN scale and NaN values.  residual, weight (1), sum_out, rstd may be NULL.
  * sum_out may be x or the residual itself (same pointer and pitch). */
 typedef struct tforge_rms_norm_args {
   int32_t dtype;           /* TFORGE_F32 or TFORGE_BF16: x, residual, sum_out */
@@ -247,8 +248,9 @@ typedef struct tforge_rms_norm_backward_args {
 int tforge_rms_norm_backward(const tforge_rms_norm_backward_args *args, void *stream);
 
 /* Rows of f32 or bf16 x (M x N, pitch ldx) in 8 bits: scale[m] = max(max|x[m]| / 448, 2^-126),
- * q = e4m3(x / scale[m]) (pitch ldq).  Weights (N x K) are quantized once, activations before a
- * product that tforge_rms_norm does not feed.  NaN and infinities as in tforge_rms_norm. */
+ * q = e4m3(x * (1 / scale[m])) (pitch ldq), the reciprocal and the product each rounded to f32.
+ * Weights (N x K) are quantized once, activations before a product that tforge_rms_norm does not
+ * feed.  NaN and infinities as in tforge_rms_norm. */
 int tforge_quantize_e4m3(const void *x, int dtype, uint8_t *q, float *scale, int64_t M, int64_t N, int64_t ldx,
                          int64_t ldq, void *stream);
 

@@ -3,7 +3,7 @@
 //
 // Forward, row by row, in f32:
 //   s = x + residual;  rstd = (mean(s^2) + eps)^-1/2;  y = (s w) rstd
-//   8-bit output: scale = max(max|y| / 448, 2^-126), q = e4m3(y / scale)
+//   8-bit output: scale = max(max|y| / 448, 2^-126), q = e4m3(y (1 / scale))
 // The row stays in registers between its one read and its one write: t = s w is kept, and because
 // rounding is monotone max|y| is fl(max|t| * rstd), so the sum of squares and the maximum come out
 // of the same block reduction.  The maximum is taken over bit patterns, in which a NaN is larger
@@ -176,7 +176,10 @@ __device__ __forceinline__ void out1(const NormArgs &p, int64_t m, int64_t c, fl
 }
 
 // Writes the row's rstd and scale (one thread).  What out holds of t = s weight: t rstd, for 8 bits
-// (t rstd) / scale -- in two steps, since rstd / scale overflows for a row of zeros.
+// (t rstd) (1 / scale) -- in two steps, since rstd / scale overflows for a row of zeros, and by the
+// rounded reciprocal: one value in ten thousand, which lies within 2^-23 of the middle between two
+// e4m3 numbers, goes to the other one than its quotient would.  Dividing every value makes the norm of
+// 16384 x 8192 bf16 165 us instead of 142, the quantizer of 16384 x 16384 191 instead of 134.
 template <int OUT, bool NORM>
 struct RowFactors {
   float rstd = 1.f, inv = 1.f;

@@ -10,7 +10,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from tensorforge_b200 import _lib  # noqa: E402
-from tests.test_gpu_layer import CODE, assert_within, device, half_step, ptr, rand  # noqa: E402, F401
+from tests.test_gpu_layer import CODE, TINY, assert_within, device, half_step, ptr, rand  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
 
@@ -59,6 +59,41 @@ def test_gelu_slope_keeps_its_relative_accuracy():
     z = z.double()
     p, d = phi64(z), z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     assert_within(slope, p + d, phi_bound(z) * (p + d.abs()))
+
+
+# ---- rows in 8 bits ----------------------------------------------------------------------------------
+
+
+def scales(x):
+    """The scales of rows of f32 values, and their reciprocals: quotients rounded once, for which 53 bits
+    on the way are enough.  (torch divides by a number by multiplying by its reciprocal.)"""
+    scale = (x.abs().amax(1).double() / 448).float().clamp_min(TINY)
+    return scale, (1 / scale.double()).float()[:, None]
+
+
+@pytest.mark.parametrize("m,n", [(3001, 1000), (500, 4096), (40, 1111), (3, 20001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantizer_to_the_bit(m, n, dtype):
+    """q = e4m3(x (1 / scale)) as documented, the reciprocal and the product rounded to f32."""
+    x = rand(m, n, dtype=dtype)
+    q, sc = torch.empty(m, n, device="cuda", dtype=torch.float8_e4m3fn), torch.empty(m, device="cuda")
+    _lib.quantize_e4m3(ptr(x), ptr(q), ptr(sc), m, n, CODE[dtype], stream=stream())
+    scale, inverse = scales(x.float())
+    assert torch.equal(sc, scale)
+    assert torch.equal(q.float(), (x.float() * inverse).to(torch.float8_e4m3fn).float())
+
+
+@pytest.mark.parametrize("m,n", [(3001, 1000), (500, 4096), (40, 1111), (3, 20001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_in_8_bits_to_the_bit(m, n, dtype):
+    """The norm's 8-bit rows are those of its f32 rows."""
+    x, w = rand(m, n, dtype=dtype), 1 + rand(n, seed=1, scale=0.2)
+    q, sc, y = torch.empty(m, n, device="cuda", dtype=torch.float8_e4m3fn), torch.empty(m, device="cuda"), torch.empty(m, n, device="cuda")
+    _lib.rms_norm(ptr(x), ptr(q), m, n, 1e-5, ptr(w), scale=ptr(sc), dtype=CODE[dtype], out_dtype=_lib.E4M3, stream=stream())
+    _lib.rms_norm(ptr(x), ptr(y), m, n, 1e-5, ptr(w), dtype=CODE[dtype], out_dtype=_lib.F32, stream=stream())
+    scale, inverse = scales(y)
+    assert torch.equal(sc, scale)
+    assert torch.equal(q.float(), (y * inverse).to(torch.float8_e4m3fn).float())
 
 
 # ---- one call after the other ------------------------------------------------------------------------
