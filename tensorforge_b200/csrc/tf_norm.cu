@@ -192,6 +192,8 @@ struct RowFactors {
     if constexpr (OUT == OUT_E4M3) {
       float scale = __fdiv_rn(__uint_as_float(amax_bits) * rstd, kE4m3Max);
       scale = scale < kTinyScale ? kTinyScale : scale;  // keeps a NaN
+      // An infinite value: the whole row is NaN, where its other values would be zeros.
+      if (isinf(scale)) scale = __int_as_float(0x7FFFFFFF);
       if (writer) p.scale[m] = scale;
       inv = __frcp_rn(scale);
     }

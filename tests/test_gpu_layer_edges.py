@@ -96,6 +96,23 @@ def test_norm_in_8_bits_to_the_bit(m, n, dtype):
     assert torch.equal(q.float(), (y * inverse).to(torch.float8_e4m3fn).float())
 
 
+@pytest.mark.parametrize("n", [8, 200, 1111, 20001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantizer_poisoned_rows(n, dtype):
+    """A NaN or an infinity of either sign makes its own row's scale and values NaN, and no other's."""
+    x = rand(7, n, dtype=dtype)
+    q, sc = torch.empty(7, n, device="cuda", dtype=torch.float8_e4m3fn), torch.empty(7, device="cuda")
+    _lib.quantize_e4m3(ptr(x), ptr(q), ptr(sc), 7, n, CODE[dtype], stream=stream())
+    clean, clean_sc = q.float().clone(), sc.clone()
+    x[1, n // 2], x[3, n - 1], x[5, 0] = float("nan"), float("inf"), -float("inf")
+    _lib.quantize_e4m3(ptr(x), ptr(q), ptr(sc), 7, n, CODE[dtype], stream=stream())
+    for i in range(7):
+        if i in (1, 3, 5):
+            assert bool(sc[i].isnan()) and bool(q[i].float().isnan().all()), i
+        else:
+            assert torch.equal(q[i].float(), clean[i]) and sc[i] == clean_sc[i]
+
+
 # ---- one call after the other ------------------------------------------------------------------------
 
 
