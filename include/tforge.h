@@ -314,7 +314,8 @@ int tforge_set_config(const tforge_config *cfg);
  * the synchronization itself failed. */
 int tforge_device_status(void *stream);
 
-/* Device-side wait limit in nanoseconds (default 1e9); 0 restores the default. */
+/* Device-side wait limit in nanoseconds (default 1e9); 0 restores the default.  The wait for one of
+ * tforge_linear's sums over a long k gets it again for each 2^20 of k (bf16; 2^21 e4m3). */
 int tforge_set_wait_limit_ns(uint64_t ns);
 
 /* Test hook: 1 makes the next GEMM launches' producer skip its first stage's load, so

@@ -204,6 +204,7 @@ struct LinearParams {
   int32_t res_bf16, out_bf16;
   uint32_t *status;               // device status word
   uint64_t limit_ns;              // bounded-wait limit
+  uint64_t sum_limit_ns;          // the same for a wait that lasts a whole sum over k
   int32_t debug_skip;             // test hook: skip the first stage's loads
   int32_t splits;                 // slim kernel: CTAs that share a tile's k (1, 2, 4 or 8)
   // 1: the rows' (columns') operand is MN-major and its map has blocks (encode_mn_map).

@@ -63,8 +63,7 @@ int check_arrays(const Array (&ins)[NI], const Array (&outs)[NO], int share = -1
   return TFORGE_OK;
 }
 
-// Up to 2^30: rounded up to a tile a coordinate stays in 32 bits, and the longest sum stays far below the
-// default limit of a wait.
+// Up to 2^30: rounded up to a tile a coordinate stays in 32 bits.
 bool dims_ok(int64_t a, int64_t b, int64_t c = 0) {
   constexpr int64_t most = (int64_t)1 << 30;
   return a >= 0 && b >= 0 && c >= 0 && a <= most && b <= most && c <= most;
@@ -315,6 +314,10 @@ int product(const Operand &rows, bool t_mn, const Operand &cols, bool w_mn, bool
   if ((c.tile == 0 && K == 0) || (c.tile != 0 && t_mn && c.tile < 64)) return TFORGE_ERR_UNSUPPORTED;
   // f32 outputs: sums in pieces (of the pair kernel; the slim kernel divides its k by its accumulators).
   const int64_t stages = (K * esz + 127) / 128, piece = f8 ? 64 : 12;
+  // The epilogue waits for a CTA's whole sum at once, which may well take longer than a stage may: 2^21
+  // stages (K 2^30 on eight CTAs) 0.6 s, of a default limit of 1 s.  It gets the limit for each 2^14.
+  const uint64_t times = 1 + (uint64_t)(stages / c.splits >> 14);
+  p.sum_limit_ns = p.limit_ns > UINT64_MAX / times ? UINT64_MAX : p.limit_ns * times;
   p.sum_stages = !p.out_bf16 && stages > piece ? (int32_t)piece : 0;
   if (c.tile == 0) {
     CUtensorMap tmA{}, tmB{}, tmO{}, tmP{}, tmR{};

@@ -239,7 +239,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_D
                  drainf = acce0 + 16, resf0 = drainf + 8;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::kNumBars);
   volatile uint32_t *abort_flag = tmem_slot + 1;
-  const WaitCtl wc{abort_flag, p.status, p.limit_ns};
+  const WaitCtl wc{abort_flag, p.status, p.limit_ns}, wsum{abort_flag, p.status, p.sum_limit_ns};
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -473,7 +473,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairL<FORM == FORM_D
         const int c = part + 4 * k, col0 = n0 + 32 * c;
         const bool live = inside(m0, col0);
         if (!SUMS && k == 0) {
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(accf0 + 8 * b, (u >> 1) & 1, wc, 64));
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(accf0 + 8 * b, (u >> 1) & 1, wsum, 64));
           if (!ok) break;
           tc_fence_after();
         }

@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(256)
   // Warp w reads TMEM lanes 32 (w % 4) .. + 31, tokens in chunks of 16 by its half.  Value (token j,
   // column r) goes to float j * 128 + r of the ring (every load has been consumed).
   const int q = warp & 3, half = warp >> 2, r = q * 32 + lane;
-  const bool ok = nkb == 0 || (mbar_wait(accf, 0, wc) && !*abort_flag);
+  const bool ok = nkb == 0 || (mbar_wait(accf, 0, WaitCtl{abort_flag, p.status, p.sum_limit_ns}) && !*abort_flag);
   tc_fence_after();
   const int tokens = p.M - m0 < BT ? p.M - m0 : BT;
   float *part = reinterpret_cast<float *>(smem);

@@ -172,3 +172,22 @@ def test_gradients_and_norms_repeat_themselves():
         got = [t.clone() for t in (da, db, dbias, q.view(torch.uint8), sc, rstd, dx, dw)]
         first = first or got
         assert all(torch.equal(x, y) for x, y in zip(got, first))
+
+
+# ---- limits ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("force,k", [((0, 0, 0), 1 << 27), ((1, 16, 1), 1 << 24), ((2, 0, 0), 1 << 24)])
+def test_a_sum_may_take_longer_than_the_wait_limit(force, k):
+    """The limit is for a step of the work: whoever waits for a whole sum over k gets one for each 2^14
+    stages of it (here 131072 a CTA and 262144, over 20 ms)."""
+    a, b, out = (torch.ones(r, c, device="cuda", dtype=torch.bfloat16) for r, c in ((1, k), (1, k), (1, 1)))
+    L = _lib.lib()
+    _lib.check(L.tforge_debug_linear_kernel(*force))
+    L.tforge_set_wait_limit_ns(20_000_000)
+    try:
+        _lib.linear(ptr(a), ptr(b), ptr(out), 1, 1, k, trans_b=True, stream=stream())
+        assert _lib.device_status(stream()) == _lib.OK
+    finally:
+        L.tforge_set_wait_limit_ns(0)
+    assert float(out) == k  # a power of two, and so is every partial sum's unit
