@@ -30,7 +30,10 @@ std::atomic<int> g_debug_skip{0};
 std::mutex g_cfg_mu;
 tforge_config g_cfg{};  // kernel == 0: use the table
 
+// The failure is reported once, by the status and the text: left behind as CUDA's last error it would
+// be found again by the next launch's check, the library's or the caller's.
 int cuda_fail(cudaError_t e, const char *what) {
+  cudaGetLastError();
   g_last_error = std::string(what) + ": " + cudaGetErrorString(e);
   return TFORGE_ERR_CUDA;
 }

@@ -3,6 +3,7 @@
 Tolerances are worked out from the roundings on the way, in units of u = 2^-23.
 """
 
+import ctypes as C
 import math
 
 import pytest
@@ -191,3 +192,16 @@ def test_a_sum_may_take_longer_than_the_wait_limit(force, k):
     finally:
         L.tforge_set_wait_limit_ns(0)
     assert float(out) == k  # a power of two, and so is every partial sum's unit
+
+
+def test_a_failed_call_leaves_no_error_behind():
+    """Scratch that no GPU has (a copy of 2^30 x 512 operands in 1 TB) fails the call before any launch;
+    the error is the status and the text, and is not found again by whoever asks CUDA next."""
+    args = _lib.LinearArgs(trans_b=1, a_dtype=_lib.F32, b_dtype=_lib.BF16, out_dtype=_lib.BF16, A=1 << 45, B=1 << 20, out=1 << 30,
+                           M=1 << 30, N=1, K=512)
+    assert _lib.lib().tforge_linear(C.byref(args), stream()) == _lib.ERR_CUDA
+    assert b"memory" in _lib.lib().tforge_last_error()
+    x = torch.ones(8, device="cuda")
+    y = torch.empty_like(x)
+    _lib.check(_lib.lib().tforge_add(ptr(x), ptr(x), ptr(y), 1, 8, stream()))
+    assert bool((x + y == 3).all())
