@@ -94,6 +94,10 @@ class FeedForward:
     x, residual, s and out are bf16, M x D; W1 is D x H, W2 H x D.  mode "bf16": weights in bf16 as
     given.  mode "fp8": each output feature's weights in 8 bits with a scale, the activations in 8
     bits with a scale a row -- the norm writes the first product's, the quantizer the second's.
+    bf16 weights and f32 vectors that are contiguous are used where they are, so that steps of an
+    optimizer reach the block; others, and all weights in mode "fp8", are copied as they are now.
+    autograd does not see the block: x and the residual may not need a gradient where autograd records
+    (ValueError).
     x is on the weights' GPU, and calls run on its current stream.  `__call__(..., keep=True)` keeps what
     `backward` needs until it is called, on the same stream (mode "bf16"): x or s among it, which may
     not change before then."""
@@ -111,7 +115,8 @@ class FeedForward:
         if w1.device.type != "cuda" or any(t.device != w1.device for t in (b1, w2, b2, norm_weight)):
             raise ValueError("FeedForward expects its weights on one GPU")
         self.mode, self.activation, self.eps = mode, activation, eps
-        self.b1, self.b2, self.norm_weight = (t.float().contiguous() for t in (b1, b2, norm_weight))
+        w1, w2 = w1.detach(), w2.detach()
+        self.b1, self.b2, self.norm_weight = (t.detach().float().contiguous() for t in (b1, b2, norm_weight))
         self.kept = None
         if mode == "bf16":
             self.w1, self.w2 = w1.bfloat16().contiguous(), w2.bfloat16().contiguous()
@@ -148,6 +153,8 @@ class FeedForward:
             raise ValueError("FeedForward takes rows on its weights' GPU")
         if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape or not residual.is_contiguous()):
             raise ValueError("the residual is like x")
+        if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+            raise ValueError("FeedForward's gradients come from its backward(): detach its inputs")
         if keep and self.mode != "bf16":
             raise ValueError("only mode 'bf16' has a gradient")
         m, fp8 = x.shape[0], self.mode == "fp8"

@@ -11,7 +11,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from tensorforge_b200 import _lib  # noqa: E402
-from tests.test_gpu_layer import CODE, TINY, assert_within, device, half_step, ptr, rand  # noqa: E402, F401
+from tests.test_gpu_layer import CODE, TINY, assert_within, block, device, half_step, ptr, rand  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
 
@@ -205,3 +205,34 @@ def test_a_failed_call_leaves_no_error_behind():
     y = torch.empty_like(x)
     _lib.check(_lib.lib().tforge_add(ptr(x), ptr(x), ptr(y), 1, 8, stream()))
     assert bool((x + y == 3).all())
+
+
+# ---- the block -----------------------------------------------------------------------------------------
+
+
+def test_block_refuses_inputs_that_need_a_gradient():
+    """autograd does not see the block: an input that needs a gradient would silently get none."""
+    m = block(64, 128, "silu", "bf16")
+    x, r = rand(4, 64, dtype=torch.bfloat16), rand(4, 64, dtype=torch.bfloat16, seed=1)
+    for bad in (lambda: m(x.clone().requires_grad_()), lambda: m(x, r.clone().requires_grad_())):
+        with pytest.raises(ValueError):
+            bad()
+        with torch.no_grad():
+            out, _ = bad()
+        assert not out.requires_grad
+    assert torch.equal(m(x.clone().requires_grad_().detach())[0], m(x)[0])
+
+
+def test_block_sees_weights_as_documented():
+    """bf16 weights and f32 vectors are the caller's own, others copies of what they were."""
+    from tensorforge_b200.mlp import FeedForward
+
+    w1, w2 = (torch.nn.Parameter(rand(*s, dtype=torch.bfloat16, scale=0.1)) for s in ((64, 128), (128, 64)))
+    b1, b2, g = torch.zeros(128, device="cuda"), torch.zeros(64, device="cuda"), torch.ones(64, device="cuda")
+    x = rand(4, 64, dtype=torch.bfloat16)
+    own, copied = FeedForward(w1, b1, w2, b2, g, "silu"), FeedForward(w1.float(), b1, w2.float(), b2, g, "silu")
+    before = own(x)[0].clone()
+    assert torch.equal(copied(x)[0], before) and not before.requires_grad
+    with torch.no_grad():
+        w1.mul_(2)
+    assert not torch.equal(own(x)[0], before) and torch.equal(copied(x)[0], before)
