@@ -100,7 +100,8 @@ class FeedForward:
     (ValueError).
     x is on the weights' GPU, and calls run on its current stream.  `__call__(..., keep=True)` keeps what
     `backward` needs until it is called, on the same stream (mode "bf16"): x or s among it, which may
-    not change before then."""
+    not change before then.  `backward` gives it back, so the two are captured into a graph together or
+    not at all."""
 
     def __init__(self, w1, b1, w2, b2, norm_weight, activation: str = "gelu_tanh", mode: str = "bf16", eps: float = 1e-5):
         import torch
@@ -160,6 +161,7 @@ class FeedForward:
         m, fp8 = x.shape[0], self.mode == "fp8"
         with torch.cuda.device(x.device):
             st = self._stream(x)
+            capturing = keep and torch.cuda.is_current_stream_capturing()
 
             def new(*shape, dtype=torch.bfloat16):
                 return torch.empty(shape, device=x.device, dtype=dtype)
@@ -187,7 +189,7 @@ class FeedForward:
                 _lib.linear(hid.data_ptr(), self.w2.data_ptr(), out.data_ptr(), m, self.d, self.h, bias=self.b2.data_ptr(),
                             residual=s.data_ptr(), stream=st)
         if keep:
-            self.kept = (s, rstd, n, pre, hid, st)
+            self.kept = (s, rstd, n, pre, hid, st, capturing)
         return out, s
 
     def backward(self, dout) -> dict:
@@ -197,14 +199,16 @@ class FeedForward:
 
         if self.kept is None:
             raise ValueError("backward needs a call with keep=True before it")
-        s, rstd, n, pre, hid, st = self.kept
+        s, rstd, n, pre, hid, st, capturing = self.kept
         if dout.dtype != torch.bfloat16 or dout.shape != s.shape or not dout.is_contiguous() or dout.device != s.device:
             raise ValueError("backward takes out's gradient: contiguous bf16 rows like out's")
         if self._stream(s) != st:
             raise ValueError("backward runs on the stream of the call that it follows")
-        self.kept = None
         m = s.shape[0]
         with torch.cuda.device(s.device):
+            if torch.cuda.is_current_stream_capturing() != capturing:
+                raise ValueError("backward is captured together with the call that it follows, or neither is")
+            self.kept = None
 
             def new(*shape, dtype=torch.bfloat16):
                 return torch.empty(shape, device=s.device, dtype=dtype)

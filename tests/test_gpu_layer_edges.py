@@ -236,3 +236,31 @@ def test_block_sees_weights_as_documented():
     with torch.no_grad():
         w1.mul_(2)
     assert not torch.equal(own(x)[0], before) and torch.equal(copied(x)[0], before)
+
+
+def test_block_gradient_is_captured_with_its_call():
+    """What an eager call kept is given back once its gradient is done: a graph of the gradient alone would
+    read it after that, and an eager gradient what a capture has not yet made."""
+    m = block(64, 128, "silu", "bf16")
+    x, dout = rand(4, 64, dtype=torch.bfloat16), rand(4, 64, dtype=torch.bfloat16, seed=1)
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        m(x, keep=True)
+        want = {k: v.clone() for k, v in m.backward(dout).items()}
+        m(x, keep=True)
+        st.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with pytest.raises(ValueError):
+            with torch.cuda.graph(g, stream=st):
+                m.backward(dout)
+        got = m.backward(dout)  # what was kept is still there
+        assert all(torch.equal(got[k], want[k]) for k in want)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            m(x, keep=True)
+        with pytest.raises(ValueError):
+            m.backward(dout)
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=st):
+            m(x, keep=True)
+            m.backward(dout)
+        st.synchronize()
