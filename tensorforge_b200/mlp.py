@@ -233,25 +233,96 @@ def flops(m: int, d: int, h: int) -> float:
     return 2.0 * m * d * h * 2
 
 
+def block_errors(model, x, residual, out, rows, dout=None, grads=None, units=None, chunk: int = 1024) -> dict:
+    """Relative errors (of norms) of a FeedForward block's output in `rows` and, with `grads`, of its
+    gradients, against 64 bits from the block's own 8- or 16-bit weights (tanh gelu): dx in `rows`,
+    what belongs to the hidden `units` of dw1, db1 and dw2, all of db2, and the norm weight's in as
+    many columns, for which every row goes through both products, `chunk` at a time."""
+    import math
+
+    import torch
+
+    if model.mode == "fp8":
+        w1, w2 = (model.w1.double() * model.s1.double()[:, None]).t(), (model.w2.double() * model.s2.double()[:, None]).t()
+    else:
+        w1, w2 = model.w1.double(), model.w2.double()
+    weight, b1, b2 = model.norm_weight.double(), model.b1.double(), model.b2.double()
+    c = math.sqrt(2 / math.pi)
+
+    def forward(at):
+        s = x[at].double() + (residual[at].double() if residual is not None else 0.0)
+        rstd = (s.square().mean(1, keepdim=True) + model.eps).rsqrt()
+        return s, rstd, s * rstd * weight
+
+    def act(z):
+        """The activation and its slope."""
+        t = torch.tanh(c * (z + 0.044715 * z ** 3))
+        return 0.5 * z * (1 + t), 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * c * (1 + 3 * 0.044715 * z * z)
+
+    def error(got, want):
+        return float((got.double() - want).norm() / want.norm())
+
+    s, rstd, n = forward(rows)
+    hid, slope = act(n @ w1 + b1)
+    errors = {"out": error(out[rows], s + hid @ w2 + b2)}
+    if grads is None:
+        return errors
+    d = dout[rows].double()
+    dn = (d @ w2.t() * slope) @ w1.t()
+    g, h = dn * weight, s * rstd
+    errors["dx"] = error(grads["dx"][rows], rstd * (g - h * (g * h).mean(1, keepdim=True)) + d)
+    cols = units % x.shape[1]
+    dw1, dw2 = torch.zeros_like(w1[:, units]), torch.zeros_like(w2[units])
+    db1, db2, dweight = torch.zeros_like(b1[units]), torch.zeros_like(b2), torch.zeros_like(weight[cols])
+    for r0 in range(0, x.shape[0], chunk):
+        at = slice(r0, r0 + chunk)
+        s, rstd, n = forward(at)
+        d = dout[at].double()
+        hid, slope = act(n @ w1 + b1)
+        dz = d @ w2.t() * slope
+        dw1 += n.t() @ dz[:, units]
+        db1 += dz[:, units].sum(0)
+        dw2 += hid[:, units].t() @ d
+        db2 += d.sum(0)
+        dweight += (dz @ w1[cols].t() * (s * rstd)[:, cols]).sum(0)
+    for name, got, want in (("dw1", grads["dw1"][:, units], dw1), ("db1", grads["db1"][units], db1), ("dw2", grads["dw2"][units], dw2),
+                            ("db2", grads["db2"], db2), ("dnorm_weight", grads["dnorm_weight"][cols], dweight)):
+        errors[name] = error(got, want)
+    return errors
+
+
+def block_bound(mode: str, name: str) -> float:
+    """How far block_errors may be.  Of the output, the whole row's: two roundings of the activations (2^-8
+    each way, or 2^-4 in 8 bits) and one of the output; of a gradient at most six values on the way in
+    bf16 (n, pre, hid, dhid, dz, dn), half a step each."""
+    if name != "out":
+        return 6 * 2.0 ** -8
+    return 2.0 ** -3 if mode == "fp8" else 2.0 ** -6
+
+
 def run_block(args, x, w1, b1, w2, b2, world: int, rank: int) -> int:
     """Times the FeedForward block (with --train and its gradient) on this rank's rows and checks a
-    seeded subset of them against 64 bits, from the block's own 8- or 16-bit weights."""
+    seeded subset of its outputs and gradients against 64 bits."""
     import numpy as np
     import torch
     import torch.distributed as dist
 
     dev = x.device
-    norm_weight = torch.ones(args.d, device=dev)
+    g = torch.Generator(device=dev)
+    g.manual_seed(9)  # the same norm weight on every rank
+    norm_weight = 1 + 0.2 * torch.randn(args.d, device=dev, generator=g)
     model = FeedForward(w1, b1, w2, b2, norm_weight, mode=args.mode)
     x = x.bfloat16()
-    dout = (x * 0.01).contiguous()
+    g.manual_seed(200 + rank)
+    residual = torch.randn(x.shape, device=dev, generator=g).bfloat16()
+    dout = (0.01 * torch.randn(x.shape, device=dev, generator=g)).bfloat16()
 
     def step():
-        out, _ = model(x, keep=args.train)
+        out, _ = model(x, residual, keep=args.train)
         return out, model.backward(dout) if args.train else None
 
     for _ in range(args.warmup):
-        out, _ = step()
+        step()
     torch.cuda.synchronize()
     stream = torch.cuda.current_stream(dev)
     e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -259,7 +330,7 @@ def run_block(args, x, w1, b1, w2, b2, world: int, rank: int) -> int:
         dist.barrier()
     e0.record(stream)
     for _ in range(args.steps):
-        out, _ = step()
+        out, grads = step()
     e1.record(stream)
     torch.cuda.synchronize()
     ms = torch.tensor([e0.elapsed_time(e1) / args.steps], device=dev, dtype=torch.float64)
@@ -267,32 +338,25 @@ def run_block(args, x, w1, b1, w2, b2, world: int, rank: int) -> int:
         dist.all_reduce(ms, op=dist.ReduceOp.MAX)
     status = _lib.device_status(stream.cuda_stream)
 
-    rows = x.shape[0]
-    sel = torch.from_numpy(np.sort(np.random.default_rng(rank).choice(rows, min(args.check_rows, rows), replace=False))).to(dev)
-    s64 = x[sel].double()
-    n64 = s64 * (s64.square().mean(1, keepdim=True) + model.eps).rsqrt()
-    if args.mode == "fp8":
-        d1, d2 = model.w1.double() * model.s1.double()[:, None], model.w2.double() * model.s2.double()[:, None]
-        d1, d2 = d1.t(), d2.t()
-    else:
-        d1, d2 = model.w1.double(), model.w2.double()
-    z = n64 @ d1 + b1.double()
-    hid = 0.5 * z * (1 + torch.tanh((2 / np.pi) ** 0.5 * (z + 0.044715 * z ** 3)))
-    want = s64 + hid @ d2 + b2.double()
-    err = float((out[sel].double() - want).norm() / want.norm())
-    # Relative to the whole row: two roundings of the activations (2^-8 each way, or 2^-4 in 8 bits)
-    # and one of the output.
-    bound = 2.0 ** -3 if args.mode == "fp8" else 2.0 ** -6
-    ok = torch.tensor([int(err <= bound and status == 0)], device=dev)
+    rng = np.random.default_rng(rank)
+    pick = lambda n: torch.from_numpy(np.sort(rng.choice(n, min(args.check_rows, n), replace=False))).to(dev)  # noqa: E731
+    sel = pick(x.shape[0])
+    errors = block_errors(model, x, residual, out, sel, dout, grads, pick(args.h)) if len(sel) else {"out": 0.0}
+    # (A NaN is not within its bound.)
+    ok = torch.tensor([int(status == 0 and all(e <= block_bound(args.mode, name) for name, e in errors.items()))], device=dev)
     if world > 1:
         dist.all_reduce(ok, op=dist.ReduceOp.MIN)
     if rank == 0:
         t = float(ms.item())
         fl = flops(args.m, args.d, args.h) * (3 if args.train else 1)
-        print(json.dumps({"workload": f"feed-forward block X {args.m}x{args.d}, W1 {args.d}x{args.h}, W2 {args.h}x{args.d}",
-                          "mode": args.mode, "gradient": bool(args.train), "n_gpus": world, "ms_per_step": t,
-                          "tflops": fl / (t * 1e-3) / 1e12, "rel_err": err, "rel_err_bound": bound,
-                          "checked_rows_per_rank": int(len(sel)), "pass": bool(ok.item())}), flush=True)
+        line = {"workload": f"feed-forward block X {args.m}x{args.d}, W1 {args.d}x{args.h}, W2 {args.h}x{args.d}",
+                "mode": args.mode, "gradient": bool(args.train), "n_gpus": world, "ms_per_step": t,
+                "tflops": fl / (t * 1e-3) / 1e12, "rel_err": errors["out"], "rel_err_bound": block_bound(args.mode, "out"),
+                "checked_rows_per_rank": int(len(sel)), "pass": bool(ok.item())}
+        if args.train:
+            line["gradient_rel_err"] = {k: e for k, e in errors.items() if k != "out"}
+            line["gradient_rel_err_bound"] = block_bound(args.mode, "dx")
+        print(json.dumps(line), flush=True)
     return 0 if ok.item() else 1
 
 

@@ -264,3 +264,17 @@ def test_block_gradient_is_captured_with_its_call():
             m(x, keep=True)
             m.backward(dout)
         st.synchronize()
+
+
+@pytest.mark.parametrize("argv", [["--mode", "bf16", "--train"], ["--mode", "bf16"], ["--mode", "fp8"]])
+@pytest.mark.parametrize("shape", ["300x256x512", "5x136x264"])
+def test_block_command_checks_what_it_times(argv, shape, capsys):
+    import json
+
+    from tensorforge_b200 import mlp
+
+    assert mlp.main(["--block", "--shape", shape, "--steps", "2", "--warmup", "1", *argv]) == 0
+    line = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert line["pass"] and line["rel_err"] <= line["rel_err_bound"]
+    checked = {"dx", "dw1", "db1", "dw2", "db2", "dnorm_weight"} if "--train" in argv else set()
+    assert set(line.get("gradient_rel_err", {})) == checked
