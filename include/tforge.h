@@ -139,7 +139,7 @@ int tforge_convert_bf16(const float *x, uint16_t *y, int64_t n, void *stream);
 
 /* ---- transformer-layer operators --------------------------------------------------------------
  * All asynchronous on `stream`, which belongs to the current device, as all pointers do.  Pitches
- * are in elements, 0 = packed.  Any size up to 2^30, any pitch and any element-aligned pointer works;
+ * are in elements, 0 = packed; those of arrays that are not there are not looked at.  Any size up to 2^30, any pitch and any element-aligned pointer works;
  * rows that start on 16-byte boundaries save an operand's copy (tforge_linear) or take wider
  * accesses.  An output may not overlap another output or an input, but where its entry says so
  * (else TFORGE_ERR_ALIAS); column slices of one buffer do not overlap.  M = 0 or N = 0 is a no-op

@@ -69,9 +69,10 @@ bool dims_ok(int64_t a, int64_t b, int64_t c = 0) {
   return a >= 0 && b >= 0 && c >= 0 && a <= most && b <= most && c <= most;
 }
 // Fills a zero pitch in; false when a pitch is shorter than its row (or unreasonably long: byte
-// offsets stay within 63 bits).
-bool pitch(int64_t &ld, int64_t cols) {
-  if (ld == 0) ld = cols;
+// offsets stay within 63 bits).  The pitch of an array that is not there says nothing, and is made the
+// packed one, which keeps no kernel from wide accesses.
+bool pitch(int64_t &ld, int64_t cols, bool there = true) {
+  if (ld == 0 || !there) ld = cols;
   return ld >= cols && ld <= (int64_t)1 << 31;
 }
 
@@ -485,7 +486,8 @@ int tforge_linear(const tforge_linear_args *args, void *stream) {
   if (f8 && !a.trans_b) return TFORGE_ERR_UNSUPPORTED;
   if (!dims_ok(a.M, a.N, a.K)) return TFORGE_ERR_SHAPE;
   const int64_t brows = a.trans_b ? a.N : a.K, bcols = a.trans_b ? a.K : a.N;
-  if (!pitch(a.lda, a.K) || !pitch(a.ldb, bcols) || !pitch(a.ldr, a.N) || !pitch(a.ldo, a.N) || !pitch(a.ldp, a.N))
+  if (!pitch(a.lda, a.K) || !pitch(a.ldb, bcols) || !pitch(a.ldr, a.N, a.residual) || !pitch(a.ldo, a.N) ||
+      !pitch(a.ldp, a.N, a.pre))
     return TFORGE_ERR_SHAPE;
   if (a.M == 0 || a.N == 0) return TFORGE_OK;
   if (!a.out || (a.K > 0 && (!a.A || !a.B)) || (f8 && (!a.a_scale || !a.b_scale))) return TFORGE_ERR_NULL;
@@ -529,8 +531,8 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
   if (!is_float(a.dtype) || !is_float(a.grad_dtype)) return TFORGE_ERR_MODE;
   if (!dims_ok(a.M, a.N, a.K)) return TFORGE_ERR_SHAPE;
   const int64_t brows = a.trans_b ? a.N : a.K, bcols = a.trans_b ? a.K : a.N;
-  if (!pitch(a.lddo, a.N) || !pitch(a.ldp, a.N) || !pitch(a.lda, a.K) || !pitch(a.ldb, bcols) || !pitch(a.ldda, a.K) ||
-      !pitch(a.lddb, bcols))
+  if (!pitch(a.lddo, a.N) || !pitch(a.ldp, a.N, a.pre && a.activation != TFORGE_ACT_NONE) || !pitch(a.lda, a.K, a.A && a.dB) ||
+      !pitch(a.ldb, bcols, a.B && a.dA) || !pitch(a.ldda, a.K, a.dA) || !pitch(a.lddb, bcols, a.dB))
     return TFORGE_ERR_SHAPE;
   const bool want_a = a.dA && a.M > 0 && a.K > 0, want_b = a.dB && a.N > 0 && a.K > 0, want_bias = a.dbias && a.N > 0;
   if (!want_a && !want_b && !want_bias) return TFORGE_OK;
@@ -603,7 +605,8 @@ int tforge_rms_norm(const tforge_rms_norm_args *args, void *stream) {
       !(is_float(a.out_dtype) || a.out_dtype == TFORGE_E4M3))
     return TFORGE_ERR_MODE;
   if (!dims_ok(a.M, a.N) || !(a.eps >= 0.0f) || std::isinf(a.eps)) return TFORGE_ERR_SHAPE;
-  if (!pitch(a.ldx, a.N) || !pitch(a.ldr, a.N) || !pitch(a.lds, a.N) || !pitch(a.ldo, a.N)) return TFORGE_ERR_SHAPE;
+  if (!pitch(a.ldx, a.N) || !pitch(a.ldr, a.N, a.residual) || !pitch(a.lds, a.N, a.sum_out) || !pitch(a.ldo, a.N))
+    return TFORGE_ERR_SHAPE;
   if (a.M == 0 || a.N == 0) return TFORGE_OK;
   if (!a.x || !a.out || (a.out_dtype == TFORGE_E4M3 && !a.scale)) return TFORGE_ERR_NULL;
   const int e = elem_size(a.dtype);
@@ -641,7 +644,8 @@ int tforge_rms_norm_backward(const tforge_rms_norm_backward_args *args, void *st
   tforge_rms_norm_backward_args a = *args;
   if (!is_float(a.dtype) || (a.weight && !is_float(a.weight_dtype))) return TFORGE_ERR_MODE;
   if (!dims_ok(a.M, a.N)) return TFORGE_ERR_SHAPE;
-  if (!pitch(a.lddy, a.N) || !pitch(a.lds, a.N) || !pitch(a.ldds, a.N) || !pitch(a.lddx, a.N)) return TFORGE_ERR_SHAPE;
+  if (!pitch(a.lddy, a.N) || !pitch(a.lds, a.N) || !pitch(a.ldds, a.N, a.ds) || !pitch(a.lddx, a.N))
+    return TFORGE_ERR_SHAPE;
   if (a.N == 0) return TFORGE_OK;
   if (a.M > 0 && (!a.dy || !a.s || !a.rstd || !a.dx)) return TFORGE_ERR_NULL;
   const int e = elem_size(a.dtype);
