@@ -5,7 +5,8 @@
 // The tensor core cuts where it adds to an f32 accumulator, so a sum over bf16 products shrinks by
 // about 1.0e-6 of its value per 1024 of k (measured: 1.9e-5 at 16384; f32 additions that round leave
 // 4e-7); e4m3's by 1.1e-6 at 16384.  That is lost in a bf16 output, not in an f32 one, whose sums are
-// therefore taken in pieces -- of at most 768 (bf16) or 8192 (e4m3) -- and joined by rounding f32 additions.
+// therefore taken in pieces -- of at most 768 (bf16) or 8192 (e4m3) -- and joined by rounding f32 additions:
+// 7.4e-7 off at k = 4096 to 16384, and at worst 2^-24 of the sums for each piece joined.
 #pragma once
 #include <cuda_bf16.h>
 

@@ -250,7 +250,11 @@ struct Choice {
 };
 
 // The pair kernel where its tiles fill the 74 pairs once; else the least estimated time in us over it
-// and the slim kernel's tiles and splits.  The estimates are fits to a sweep of 162 problems (M 1 ..
+// and the slim kernel's tiles and splits.  Such products need no estimate, few stages of k among them:
+// bf16 8192 x 8192 with k = 32 .. 512 takes pairs 59 to 71 us and the slim kernel's best tile 104 to
+// 138, 2560 x 2048 (80 tiles) 11 to 14 and 14 to 18, 32768 x 640 27 to 33 and 36 to 51, with f32 out,
+// gelu or a residual the same way; of 90 forms only some of 9472 x 512 went to the slim kernel, by 2 to
+// 8 % (k = 64 with gelu 11.2 and 10.3).  The estimates are fits to a sweep of 162 problems (M 1 ..
 // 4096, nine N x K from 128 x 2048 to 16384 x 4096, bf16 and e4m3) by every kernel: the choice is
 // 2.8 % slower than the fastest on average, and at worst 25 % (2048 x 1024 x 1024: 13.8 us, 11.0).
 //   memory: operands and output once at the measured copy rate.

@@ -16,10 +16,11 @@
 // is brought into the staging by TMA one chunk ahead, so a tile's first while its MMAs run.
 //
 // Bound by the tensor pipe: 4096 x 4096 -> 16384 bf16 with tanh gelu and pre 377 us (1458 TFLOP/s; ncu
-// 85 % busy), 8192 x 16384 -> 4096 e4m3 with residual 392 us (2805; 79 %).  With few stages of k a
-// tile is bound by this epilogue: 4096 x 256 -> 8192 bf16 with silu takes 56 us with eight warps in two
-// groups that meet at barriers and read the residual themselves, 48 as it is here; with the bf16
-// residual 95 and 59.
+// 85 % busy), 8192 x 16384 -> 4096 e4m3 with residual 392 us (2805; 79 %), replayed from graphs in short
+// bursts; 440 to 460 and 460 to 490 in a long run of calls, at the clock that the power cap leaves.
+// With few stages of k a tile is bound by this epilogue: 4096 x 256 -> 8192 bf16 with silu takes 56 us
+// with eight warps in two groups that meet at barriers and read the residual themselves, 48 as it is
+// here; with the bf16 residual 95 and 59.
 //
 // 640 threads: warp 0 TMA producer (both CTAs), warp 1 MMA issuer (leader), warps 4..19 epilogue.
 // Every wait is bounded (tf_ptx.cuh); after an expiry each role stops, the producer, the issuer and
