@@ -202,10 +202,11 @@ int tforge_linear_backward(const tforge_linear_backward_args *args, void *stream
 
 /* Root-mean-square norm of rows, with the residual's addition before it:
  *   s = x + residual (sum_out = s);  r = (mean(s^2) + eps)^-1/2 (rstd = r);  out = s r weight
- * in f32 (squares beyond its range make r 0), each output rounded once.  out is f32, bf16 or E4M3; E4M3 rows come with scale[m] =
- * max(max|out| / 448, 2^-126), the f32 factor back to out's values, and hold e4m3(out * (1 / scale[m])),
- * the reciprocal and the product each rounded to f32; a row that holds a NaN, or an infinity in s, has a
- * NaN scale and NaN values.  residual, weight (1), sum_out, rstd may be NULL.
+ * in f32 (squares beyond its range make r 0), each output rounded once.  out is f32, bf16 or E4M3;
+ * E4M3 rows come with scale[m] = max(max|out| / 448, 2^-126), the f32 factor back to out's values, and
+ * hold e4m3(out * (1 / scale[m])), the reciprocal and the product each rounded to f32; a row that holds
+ * a NaN, or an infinity in s, has a NaN scale and NaN values.  residual, weight (1), sum_out, rstd may
+ * be NULL.
  * sum_out may be x or the residual itself (same pointer and pitch). */
 typedef struct tforge_rms_norm_args {
   int32_t dtype;           /* TFORGE_F32 or TFORGE_BF16: x, residual, sum_out */
