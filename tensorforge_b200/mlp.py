@@ -95,7 +95,8 @@ class FeedForward:
     given.  mode "fp8": each output feature's weights in 8 bits with a scale, the activations in 8
     bits with a scale a row -- the norm writes the first product's, the quantizer the second's.
     bf16 weights and f32 vectors that are contiguous are used where they are, so that steps of an
-    optimizer reach the block; others, and all weights in mode "fp8", are copied as they are now.
+    optimizer reach the block; others, and all weights in mode "fp8", are copied as they are now, on the
+    current stream (a call on another one waits for it first, as for any tensor made there).
     autograd does not see the block: x and the residual may not need a gradient where autograd records
     (ValueError).
     x is on the weights' GPU, and calls run on its current stream.  `__call__(..., keep=True)` keeps what
